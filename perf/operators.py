@@ -65,9 +65,11 @@ def draw(rng):
                     skew=rng.choice([0.0, 0.5, 1.1]), type=dtype)
     if kind == "ffn":
         experts = rng.randint(2, 32)
-        of = experts * rng.choice([1, 1, 4])
         topk = rng.randint(1, min(8, experts))
-        return dict(op="ffn", tokens=_log(rng, 1, 16384 // topk), topk=topk, experts=experts, of=of, hidden=8 * _log(rng, 32, 512),
+        tokens = _log(rng, 1, 16384 // topk)
+        # a shard has slots of its own unless the batch is tiny
+        of = experts * (rng.choice([1, 1, 4]) if tokens >= 32 else 1)
+        return dict(op="ffn", tokens=tokens, topk=topk, experts=experts, of=of, hidden=8 * _log(rng, 32, 512),
                     inter=8 * _log(rng, 16, 256), skew=rng.choice([0.0, 0.3, 1.1]), type=dtype)
     return dict(op="lora", tokens=_log(rng, 1, 8192), adapters=rng.randint(1, 64), k=8 * _log(rng, 32, 768),
                 n=_log(rng, 256, 6144), rank=_log(rng, 4, 64), bare=rng.choice([0.0, 0.1, 0.5]), type=dtype,
