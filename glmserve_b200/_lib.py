@@ -61,6 +61,8 @@ def lib():
         L.gsb_comm_set_wait_cycles.argtypes = [C.c_void_p, C.c_longlong]
         L.gsb_comm_open_loopback.argtypes = [C.c_void_p]
         L.gsb_prefill_wait_profile.argtypes = [C.c_void_p]
+        L.gsb_moe_expert_ffn_w16_workspace_bytes.restype = C.c_size_t
+        L.gsb_lora_scratch_bytes.restype = C.c_size_t
         _lib = L
     return _lib
 

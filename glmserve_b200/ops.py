@@ -101,6 +101,108 @@ def moe_expert_ffn(x, topk_ids, topk_w, gate_w, up_w, down_w):
     return out
 
 
+_TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+def _need16(x, *named):
+    """x: a bf16 or fp16 CUDA tensor; (t, dtype or None = x's, dims, name) the others, all on x's device."""
+    if not x.is_cuda or x.dtype not in (torch.bfloat16, torch.float16) or not x.is_contiguous() or x.dim() != 2:
+        raise ValueError("x: expected a contiguous 2-D CUDA tensor of torch.bfloat16 or torch.float16")
+    for t, dtype, dims, name in named:
+        if t is None:
+            continue
+        dtype = dtype or x.dtype
+        if not t.is_cuda or t.device != x.device or t.dtype != dtype or not t.is_contiguous() or t.dim() != dims:
+            raise ValueError(f"{name}: expected a contiguous {dims}-D tensor of {dtype} on {x.device}")
+
+
+def _out16(out, shape, x, out_dtype, name="out"):
+    if out is None:
+        out_dtype = out_dtype or x.dtype
+        if out_dtype not in (x.dtype, torch.float32):
+            raise ValueError(f"out_dtype: expected {x.dtype} or torch.float32")
+        return torch.empty(shape, dtype=out_dtype, device=x.device)
+    if not out.is_cuda or out.device != x.device or out.dtype not in (x.dtype, torch.float32) or \
+            not out.is_contiguous() or tuple(out.shape) != tuple(shape) or out_dtype not in (None, out.dtype):
+        raise ValueError(f"{name}: expected a contiguous tensor {tuple(shape)} of {x.dtype} or torch.float32 on {x.device}")
+    return out
+
+
+def grouped_gemm(x, w, expert_offsets, rows=None, out=None, out_dtype=None):
+    """Ragged product grouped by expert: ``y[p] = w[e] @ x[rows[p]]`` for the rows p of expert e's segment
+    ``expert_offsets[e] <= p < expert_offsets[e + 1]``.  x bf16/fp16 [n,K], w the same type [E,N,K],
+    expert_offsets int32 [E+1] and rows int32 [P] as ``moe_dispatch`` returns them (offsets, sorted_token_ids);
+    without ``rows`` row p is x[p].  Returns y [P,N] of x's type (or float32 with ``out_dtype`` / ``out``).  Rows
+    that no segment covers are left as they were in ``out``; without ``out`` their contents are undefined."""
+    _need16(x, (w, None, 3, "w"), (expert_offsets, torch.int32, 1, "expert_offsets"), (rows, torch.int32, 1, "rows"))
+    n, K = x.shape
+    E, N = w.shape[:2]
+    if w.shape[2] != K or expert_offsets.shape[0] != E + 1:
+        raise ValueError("grouped_gemm: expected w [E,N,K] with x's K and expert_offsets [E+1]")
+    P = n if rows is None else rows.shape[0]
+    out = _out16(out, (P, N), x, out_dtype)
+    with torch.cuda.device(x.device):
+        check(lib().gsb_grouped_gemm(_p(x), _p(w), _TYPE[x.dtype], _p(expert_offsets), _p(rows), n, P, K, N, E,
+                                     _p(out), _TYPE[out.dtype], _stream()), "grouped_gemm")
+    return out
+
+
+def moe_expert_ffn_w16(x, topk_ids, topk_w, gate_w, up_w, down_w, out=None, out_dtype=None):
+    """``moe_expert_ffn`` with bf16/fp16 activations and weights on the tensor cores: x [n,H], topk_ids int32 and
+    topk_w float32 [n,topk], gate_w/up_w [E,I,H], down_w [E,H,I] -> out [n,H] of x's type (or float32).  A slot
+    whose id is outside [0,E) adds nothing (padding, or an expert on another GPU)."""
+    _need16(x, (topk_ids, torch.int32, 2, "ids"), (topk_w, torch.float32, 2, "w"), (gate_w, None, 3, "gate_w"),
+            (up_w, None, 3, "up_w"), (down_w, None, 3, "down_w"))
+    n, H = x.shape
+    E, I = gate_w.shape[:2]
+    topk = topk_ids.shape[1]
+    if gate_w.shape != (E, I, H) or up_w.shape != (E, I, H) or down_w.shape != (E, H, I) or \
+            topk_ids.shape != (n, topk) or topk_w.shape != (n, topk):
+        raise ValueError("moe_expert_ffn_w16: expected gate_w, up_w [E,I,H], down_w [E,H,I], ids and w [n,topk]")
+    out = _out16(out, (n, H), x, out_dtype)
+    nbytes = int(lib().gsb_moe_expert_ffn_w16_workspace_bytes(n, topk, H, I, E))
+    with torch.cuda.device(x.device):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        check(lib().gsb_moe_expert_ffn_w16(_p(x), _p(topk_ids), _p(topk_w), _p(gate_w), _p(up_w), _p(down_w),
+                                           _TYPE[x.dtype], n, topk, H, I, E, _p(out), _TYPE[out.dtype], _p(ws),
+                                           C.c_size_t(nbytes), _stream()), "moe_expert_ffn_w16")
+    return out
+
+
+def lora_add(y, x, A, B, adapter_offsets, rows, ranks=None, scales=None):
+    """Adapters of many requests beside a shared projection: ``y[t] += scales[a] * B[a] @ (A[a] @ x[t])`` in place
+    for ``t = rows[p]``, ``adapter_offsets[a] <= p < adapter_offsets[a + 1]``.  x bf16/fp16 [n,K], A [nA,R,K] and
+    B [nA,N,R] of the same type, y [n,N] float32 (what ``gemm_w4a16`` returns) or x's type, ranks int32 [nA]
+    (columns of B and rows of A behind an adapter's rank are not used), scales float32 [nA].  The lists come from
+    ``moe_dispatch(adapter_ids[:, None], nA)``, once per batch: offsets and sorted_token_ids; an id of -1 = no
+    adapter.  ``rows`` may be longer than the segments: what lies behind the last one is ignored."""
+    _need16(x, (A, None, 3, "A"), (B, None, 3, "B"), (adapter_offsets, torch.int32, 1, "adapter_offsets"),
+            (rows, torch.int32, 1, "rows"), (ranks, torch.int32, 1, "ranks"), (scales, torch.float32, 1, "scales"))
+    n, K = x.shape
+    nA, R = A.shape[:2]
+    N = B.shape[1]
+    if A.shape != (nA, R, K) or B.shape != (nA, N, R) or adapter_offsets.shape[0] != nA + 1 or \
+            (ranks is not None and ranks.shape[0] != nA) or (scales is not None and scales.shape[0] != nA):
+        raise ValueError("lora_add: expected A [nA,R,K], B [nA,N,R], adapter_offsets [nA+1], ranks and scales [nA]")
+    P = rows.shape[0]
+    if y is None:
+        raise ValueError("y: expected the projection's result")
+    _out16(y, (n, N), x, None, "y")
+    nbytes = int(lib().gsb_lora_scratch_bytes(P, R, nA))
+    with torch.cuda.device(x.device):
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        check(lib().gsb_lora_add(_p(x), _p(A), _p(B), _TYPE[x.dtype], _p(adapter_offsets), _p(rows), _p(ranks),
+                                 _p(scales), n, P, K, N, nA, R, _p(y), _TYPE[y.dtype], _p(scratch),
+                                 C.c_size_t(nbytes), _stream()), "lora_add")
+    return y
+
+
+def operators16_status(device=None) -> int:
+    """0, or 4 when a bounded device wait of the 16-bit operators gave up since the last call; synchronises."""
+    with torch.cuda.device(device):
+        return int(lib().gsb_operators16_status())
+
+
 def gemm_w4a16(x, qW, scales, group, bias=None):
     """cuda/kernels.cuh:48 gemm_w4a16: y[n,out] = x W^T (+ bias)."""
     _need(x, torch.float32, "x"); _need(qW, torch.uint8, "qW"); _need(scales, torch.float32, "scales")

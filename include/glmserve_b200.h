@@ -117,6 +117,54 @@ GSB_API int gsb_gemm_w4a16(const float* x, const uint8_t* qW, const float* scale
 GSB_API int gsb_operator_cache_enable(size_t max_weight_bytes);
 GSB_API size_t gsb_operator_cache_bytes(void);
 
+/* Element types of the 16-bit operators below. */
+enum { GSB_TYPE_F32 = 0, GSB_TYPE_BF16 = 1, GSB_TYPE_F16 = 2 };
+
+/* Ragged product grouped by expert, 16-bit weights (no counterpart in the reference, whose expert weights are
+ * fp32 or quantised):  y[p, :] = W[e] x[rows[p], :]  for expert_offsets[e] <= p < expert_offsets[e + 1].
+ * x [n,in] and w [E,out,in] of `type` (BF16 or F16), rows i32 [P] (NULL: row p itself, P <= n), expert_offsets
+ * i32 [E+1] ascending as gsb_moe_dispatch writes it (rows = its sorted_token_ids), y [P,out] of y_type (`type`,
+ * or F32).  Sums in fp32, one rounding at the end.  Rows of y that no segment covers, or whose rows[p] is outside
+ * [0,n), are left as they were; an expert with an empty segment costs nothing.  Offsets outside [0,P] are clamped.
+ * in % 8 == 0, E <= 1024, P <= 2^30; x and w 16-byte aligned; y must not overlap the inputs. */
+GSB_API int gsb_grouped_gemm(const void* x, const void* w, int type, const int* expert_offsets,
+                             const int* rows, int n, int P, int in, int out, int E, void* y,
+                             int y_type, void* stream);
+
+/* moe_expert_ffn with 16-bit weights and activations, tensor-core form of gsb_moe_expert_ffn:
+ * out[t] = sum_k w[t,k] * down(silu(gate x) * up x), slots added in order.  x [n,hidden], gate_w/up_w
+ * [E,moe_inter,hidden], down_w [E,hidden,moe_inter] of `type`; out [n,hidden] of out_type (`type`, or F32) is
+ * OVERWRITTEN.  A slot whose id is outside [0,E) adds nothing (padding, or an expert that lives on another GPU);
+ * a token without a slot gets zeros.  Sums in fp32; silu(gate x) * up x is rounded once to `type`, in fp16
+ * saturating at +-65504.  hidden and moe_inter multiples of 8, E <= 1024, n * topk <= 2^30; all pointers but ids
+ * and weights 16-byte aligned; workspace 256-byte aligned, any contents; two calls that may overlap on the GPU
+ * need a workspace each. */
+GSB_API size_t gsb_moe_expert_ffn_w16_workspace_bytes(int n, int topk, int hidden, int moe_inter, int E);
+GSB_API int gsb_moe_expert_ffn_w16(const void* x, const int* topk_ids, const float* topk_weights,
+                                   const void* gate_w, const void* up_w, const void* down_w, int type,
+                                   int n, int topk, int hidden, int moe_inter, int E, void* out,
+                                   int out_type, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Low-rank adapters of many requests beside a shared projection (gsb_gemm_w4a16, or any other that left its
+ * result in y):  y[t, :] += scales[a] * B[a] (A[a] x[t, :])  for t = rows[p], adapter_offsets[a] <= p <
+ * adapter_offsets[a + 1].  x [n,in], A [n_adapters,max_rank,in] and B [n_adapters,out,max_rank] of `type` (BF16 or
+ * F16), y [n,out] of y_type (`type`, or F32), updated in place.  ranks i32 [n_adapters] (NULL: max_rank): what lies
+ * behind an adapter's rank is not used, whatever it holds; scales f32 [n_adapters] (NULL: 1).  The lists are those
+ * of gsb_moe_dispatch on one adapter id a row (topk = 1, E = n_adapters, an id outside the range = no adapter), made
+ * once per batch and used for every projection of the model; rows that no list names are left as they were, indices
+ * outside [0,n) are skipped, a row must not be listed twice.  A x is kept in fp32, B is applied to it without
+ * rounding it to `type`; y is rounded once.  in % 8 == 0, 1 <= max_rank <= 256, n_adapters <= 1024; x and A 16-byte aligned;
+ * scratch of gsb_lora_scratch_bytes() bytes, 256-byte aligned, any contents, not shared by calls that may overlap. */
+GSB_API size_t gsb_lora_scratch_bytes(int P, int max_rank, int n_adapters);
+GSB_API int gsb_lora_add(const void* x, const void* A, const void* B, int type, const int* adapter_offsets,
+                         const int* rows, const int* ranks, const float* scales, int n, int P, int in,
+                         int out, int n_adapters, int max_rank, void* y, int y_type, void* scratch,
+                         size_t scratch_bytes, void* stream);
+
+/* Status of the 16-bit operators' bounded device-side waits on the current device: GSB_OK, or GSB_ERR_TIMEOUT when
+ * a kernel gave up since the last call (its output is then incomplete); clears it.  Synchronises the device. */
+GSB_API int gsb_operators16_status(void);
+
 /* Replace silu_mul / add_inplace / rmsnorm (cuda/kernels.cuh:18-19, :282-283), the glue the
  * reference runs around the shared expert and the residual (src/model_gpu.cpp:1430,
  * :1486-1502).  rmsnorm sums squares in double like the CPU reference. */

@@ -1,0 +1,304 @@
+"""16-bit expert products (grouped_gemm, moe_expert_ffn_w16) against plain 64-bit forms of the same formulas.
+
+Tolerances are bounds on the arithmetic, element by element: an fp32 sum of m products is off by at most
+(m + 8) * 2^-23 times the sum of the absolute products (the tensor core may truncate, hence 2^-23 and not 2^-24), a
+rounding to 16 bits by half a step (bf16 2^-8, fp16 2^-11 of the value, or 2^-25 below fp16's normal range).  The FFN's
+bound on h would hide a mistake of a few percent behind its worst case, so its result is also held to the root mean
+square of two independent roundings, each at most half a step / sqrt(3), with a factor 1.5."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+TINY = {torch.bfloat16: 0.0, torch.float16: 2.0 ** -25, torch.float32: 0.0}
+U = 2.0 ** -23
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    return torch.device("cuda:0")
+
+
+def _randn(shape, dtype, dev, seed, scale=1.0):
+    g = torch.Generator(device=dev)
+    g.manual_seed(seed)
+    return (torch.randn(shape, generator=g, device=dev) * scale).to(dtype)
+
+
+def _i32(v, dev):
+    return torch.tensor(np.asarray(v, np.int32), device=dev)
+
+
+def _offsets(counts, dev):
+    return _i32(np.concatenate([[0], np.cumsum(counts)]), dev)
+
+
+def _grouped_ref(x, w, offs, rows):
+    """y, bound on an fp32 sum, and which rows are written."""
+    P = rows.numel()
+    y = torch.zeros((P, w.shape[1]), dtype=torch.float64, device=x.device)
+    b = torch.zeros_like(y)
+    written = torch.zeros(P, dtype=torch.bool, device=x.device)
+    o = offs.tolist()
+    for e in range(w.shape[0]):
+        if o[e + 1] <= o[e]:
+            continue
+        r = rows[o[e]:o[e + 1]].long()
+        ok = (r >= 0) & (r < x.shape[0])
+        xe = x[r.clamp(0, x.shape[0] - 1)].double()
+        we = w[e].double()
+        y[o[e]:o[e + 1]] = xe @ we.T
+        b[o[e]:o[e + 1]] = xe.abs() @ we.abs().T * ((x.shape[1] + 8) * U)
+        written[o[e]:o[e + 1]] = ok
+    return y, b, written
+
+
+def _check(y, ref, bound, what):
+    d = (y.double() - ref).abs()
+    bad = ~(d <= bound)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((d - bound).max()):.3e} over the bound"
+
+
+CASES = [  # counts of every expert, n tokens, K, N
+    ([1], 1, 8, 1),
+    ([1, 0, 0, 2], 2, 64, 16),
+    ([0, 0, 7], 3, 72, 65),
+    ([16, 17, 0, 15, 1, 33], 50, 128, 130),
+    ([5, 300, 0, 129, 64], 200, 520, 257),
+    ([1] * 40, 7, 1024, 512),
+    ([3, 0, 1, 9] * 16, 64, 264, 96),
+    ([257, 511, 256, 1, 255], 700, 1032, 515),
+    ([1100], 1100, 456, 1000),
+    ([0, 0, 0], 4, 64, 64),
+    ([700, 2, 0, 1400], 900, 2048, 640),
+    ([40, 24, 70], 100, 6144, 320),
+]
+
+
+@pytest.mark.parametrize("case", range(len(CASES)))
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("out_f32", [False, True])
+def test_grouped_gemm(dev, case, dtype, out_f32):
+    from glmserve_b200 import ops
+    counts, n, K, N = CASES[case]
+    P, pad = int(sum(counts)), 5
+    x, w = _randn((n, K), dtype, dev, case), _randn((len(counts), N, K), dtype, dev, 100 + case, 0.05)
+    rng = np.random.default_rng(case)
+    rows = _i32(rng.integers(0, n, P + pad), dev)
+    offs = _offsets(counts, dev)
+    od = torch.float32 if out_f32 else dtype
+    out = torch.full((P + pad, N), 7.0, dtype=od, device=dev)
+    got = ops.grouped_gemm(x, w, offs, rows=rows, out=out)
+    assert got is out and ops.operators16_status() == 0
+    ref, b, _ = _grouped_ref(x, w, offs, rows)
+    _check(out[:P], ref[:P], b[:P] + HALF[od] * ref[:P].abs() * (1 + U) + TINY[od], "grouped_gemm")
+    assert bool((out[P:] == 7.0).all()), "rows behind the last segment were written"
+    again = ops.grouped_gemm(x, w, offs, rows=rows, out=torch.full_like(out, 7.0))
+    assert torch.equal(again, out)
+
+
+def test_grouped_gemm_without_rows_and_first_segment_not_at_zero(dev):
+    from glmserve_b200 import ops
+    x, w = _randn((90, 136), torch.bfloat16, dev, 1), _randn((3, 200, 136), torch.bfloat16, dev, 2)
+    offs = _i32([4, 30, 30, 77], dev)
+    out = torch.full((90, 200), -3.0, dtype=torch.bfloat16, device=dev)
+    ops.grouped_gemm(x, w, offs, out=out)
+    ref, b, _ = _grouped_ref(x, w, offs, torch.arange(90, device=dev))
+    _check(out[4:77], ref[4:77], b[4:77] + HALF[torch.bfloat16] * ref[4:77].abs() * (1 + U), "no rows")
+    assert bool((out[:4] == -3).all() and (out[77:] == -3).all())
+
+
+def test_grouped_gemm_skips_rows_out_of_range(dev):
+    from glmserve_b200 import ops
+    x, w = _randn((20, 64), torch.float16, dev, 3), _randn((2, 48, 64), torch.float16, dev, 4)
+    rows = _i32([0, -1, 19, 20, 5, 2 ** 31 - 1, -2 ** 31, 7], dev)
+    offs = _i32([0, 5, 8], dev)
+    out = torch.full((8, 48), 9.0, dtype=torch.float16, device=dev)
+    ops.grouped_gemm(x, w, offs, rows=rows, out=out)
+    ref, b, written = _grouped_ref(x, w, offs, rows)
+    assert written.tolist() == [True, False, True, False, True, False, False, True]
+    _check(out[written], ref[written], (b + HALF[torch.float16] * ref.abs() * (1 + U) + 2.0 ** -25)[written], "written rows")
+    assert bool((out[~written] == 9.0).all())
+
+
+def test_grouped_gemm_nan_and_inf_stay_in_their_row(dev):
+    from glmserve_b200 import ops
+    x, w = _randn((40, 200), torch.bfloat16, dev, 5), _randn((2, 70, 200), torch.bfloat16, dev, 6)
+    x[3] = float("nan")
+    x[11, 199] = float("inf")
+    offs = _i32([0, 25, 40], dev)
+    clean = x.clone()
+    clean[3] = 0
+    clean[11] = 0
+    y, yc = ops.grouped_gemm(x, w, offs), ops.grouped_gemm(clean, w, offs)
+    assert bool(y[3].isnan().all()) and not bool(y[11].isfinite().any())
+    keep = [i for i in range(40) if i not in (3, 11)]
+    assert torch.equal(y[keep], yc[keep])
+
+
+def test_grouped_gemm_weights_beyond_two_to_the_31_elements(dev):
+    from glmserve_b200 import ops
+    E, N, K = 40, 4096, 16384
+    w = torch.zeros((E, N, K), dtype=torch.bfloat16, device=dev)
+    w[39] = _randn((N, K), torch.bfloat16, dev, 8, 0.02)
+    x = _randn((3, K), torch.bfloat16, dev, 9)
+    offs = _i32([0] * 39 + [0, 3], dev)
+    y = ops.grouped_gemm(x, w, offs, out_dtype=torch.float32)
+    ref, b, _ = _grouped_ref(x, w, offs, torch.arange(3, device=dev))
+    _check(y, ref, b + HALF[torch.float32] * ref.abs(), "large weights")
+
+
+def _ffn_ref(x, ids, wt, gate, up, down, dtype):
+    n, H = x.shape
+    E, I = gate.shape[:2]
+    out = torch.zeros((n, H), dtype=torch.float64, device=x.device)
+    bound, mag = torch.zeros_like(out), torch.zeros_like(out)
+    for e in range(E):
+        t, k = (ids == e).nonzero(as_tuple=True)
+        if not t.numel():
+            continue
+        xe, w = x[t].double(), wt[t, k].double()[:, None]
+        g64, u64, d64 = gate[e].double(), up[e].double(), down[e].double()
+        g, u = xe @ g64.T, xe @ u64.T
+        h = torch.nn.functional.silu(g) * u
+        dg, du = (xe.abs() @ g64.abs().T) * ((H + 8) * U), (xe.abs() @ u64.abs().T) * ((H + 8) * U)
+        # |silu'| <= 1.1; silu itself evaluated to 2^-20
+        dh = (1.1 * dg * (u.abs() + du) + torch.nn.functional.silu(g).abs() * du) * (1 + U) + (HALF[dtype] + 2.0 ** -20) * h.abs() + TINY[dtype]
+        y, ya = h @ d64.T, h.abs() @ d64.abs().T
+        dy = dh @ d64.abs().T + ya * ((I + 8) * U)
+        out.index_add_(0, t, w * y)
+        bound.index_add_(0, t, w.abs() * dy)
+        mag.index_add_(0, t, w.abs() * y.abs())
+    return out, bound + mag * ((ids.shape[1] + 2) * U)
+
+
+FFN = [  # n, topk, E, ids below `of`, H, I
+    (1, 1, 1, 1, 8, 8),
+    (1, 8, 32, 32, 1024, 512),
+    (3, 2, 4, 16, 136, 72),
+    (17, 4, 16, 16, 256, 128),
+    (64, 8, 32, 256, 1024, 264),
+    (333, 3, 5, 5, 520, 264),
+    (700, 2, 8, 8, 1024, 1032),
+    (2500, 4, 6, 6, 264, 136),
+]
+
+
+def _ffn_case(case, dtype, dev):
+    n, topk, E, of, H, I = FFN[case]
+    x = _randn((n, H), dtype, dev, case)
+    gate, up = _randn((E, I, H), dtype, dev, 10 + case, 0.05), _randn((E, I, H), dtype, dev, 20 + case, 0.05)
+    down = _randn((E, H, I), dtype, dev, 30 + case, 0.05)
+    rng = np.random.default_rng(case)
+    ids = np.stack([rng.permutation(of)[:topk] for _ in range(n)]).astype(np.int32)
+    ids[ids >= E] = [-1, E, 2 ** 31 - 1][case % 3]
+    wt = torch.from_numpy((rng.random((n, topk)) + 0.1).astype(np.float32)).to(dev)
+    return x, torch.from_numpy(ids).to(dev), wt, gate, up, down
+
+
+@pytest.mark.parametrize("case", range(len(FFN)))
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("out_f32", [False, True])
+def test_expert_ffn(dev, case, dtype, out_f32):
+    from glmserve_b200 import ops
+    args = _ffn_case(case, dtype, dev)
+    od = torch.float32 if out_f32 else dtype
+    out = ops.moe_expert_ffn_w16(*args, out_dtype=od)
+    assert ops.operators16_status() == 0 and out.dtype == od
+    ref, b = _ffn_ref(*args, dtype)
+    _check(out, ref, b + HALF[od] * ref.abs() + TINY[od], "ffn")
+    if ref.numel() >= 4096:
+        rel = float((out.double() - ref).norm() / ref.norm())
+        assert rel <= 1.5 * ((HALF[dtype] ** 2 + HALF[od] ** 2) / 3) ** 0.5, rel
+    assert torch.equal(ops.moe_expert_ffn_w16(*args, out_dtype=od), out)
+
+
+def test_expert_ffn_token_without_a_slot_is_zero_and_repeated_expert_counts_twice(dev):
+    from glmserve_b200 import ops
+    x, ids, wt, gate, up, down = _ffn_case(3, torch.bfloat16, dev)
+    ids[0] = -1
+    ids[1] = 5
+    out = ops.moe_expert_ffn_w16(x, ids, wt, gate, up, down, out=torch.full_like(x, float("nan")))
+    assert bool((out[0] == 0).all())
+    ref, b = _ffn_ref(x, ids, wt, gate, up, down, torch.bfloat16)
+    _check(out, ref, b + HALF[torch.bfloat16] * ref.abs(), "repeated expert")
+    none = ops.moe_expert_ffn_w16(x, torch.full_like(ids, -1), wt, gate, up, down)
+    assert bool((none == 0).all())
+
+
+def test_expert_ffn_intermediate_beyond_fp16_saturates(dev):
+    from glmserve_b200 import ops
+    x = torch.full((1, 64), 100.0, dtype=torch.float16, device=dev)
+    gate = torch.full((1, 64, 64), 1.0, dtype=torch.float16, device=dev)
+    down = torch.full((1, 64, 64), 2.0 ** -10, dtype=torch.float16, device=dev)
+    down[:, :, 1::2] *= -1
+    ids, wt = torch.zeros((1, 1), dtype=torch.int32, device=dev), torch.ones((1, 1), device=dev)
+    out = ops.moe_expert_ffn_w16(x, ids, wt, gate, gate, down)   # h = 6400^2, then sums that cancel
+    assert bool((out == 0).all())
+
+
+def test_router_dispatch_products_and_ffn_together(dev):
+    """The operators as a layer uses them: router, dispatch, gate and up products, down product by hand
+    against the fused FFN; and the fp32-weight operator on the same values."""
+    from glmserve_b200 import ops
+    n, E, topk, H, I = 77, 16, 4, 256, 128
+    dtype = torch.bfloat16
+    x = _randn((n, H), dtype, dev, 1)
+    gate, up, down = (_randn(s, dtype, dev, 2 + i, 0.05) for i, s in enumerate([(E, I, H), (E, I, H), (E, H, I)]))
+    ids, wt = ops.moe_router(_randn((n, E), torch.float32, dev, 9), None, topk)
+    offs, tok, col = ops.moe_dispatch(ids, E)
+    g, u = (ops.grouped_gemm(x, m, offs, rows=tok, out_dtype=torch.float32) for m in (gate, up))
+    h = (torch.nn.functional.silu(g) * u).to(dtype)
+    y = ops.grouped_gemm(h, down, offs, out_dtype=torch.float32)
+    by_hand = torch.zeros((n, H), dtype=torch.float64, device=dev)
+    by_hand.index_add_(0, tok.long(), wt[tok.long(), col.long()].double()[:, None] * y.double())
+    out = ops.moe_expert_ffn_w16(x, ids, wt, gate, up, down, out_dtype=torch.float32)
+    ref, b = _ffn_ref(x, ids, wt, gate, up, down, dtype)
+    _check(out, ref, b + HALF[torch.float32] * ref.abs(), "fused")
+    _check(by_hand, ref, b + HALF[torch.float32] * ref.abs(), "by hand")
+    old = ops.moe_expert_ffn(x.float(), ids, wt, gate.float(), up.float(), down.float())
+    _check(out, old.double(), 2 * b + 2 * HALF[torch.float32] * ref.abs(), "fp32 operator")
+
+
+def test_expert16_graph_replay_and_two_streams(dev):
+    from glmserve_b200 import ops
+    a, b = _ffn_case(4, torch.bfloat16, dev), _ffn_case(6, torch.bfloat16, dev)
+    want_a, want_b = ops.moe_expert_ffn_w16(*a), ops.moe_expert_ffn_w16(*b)
+    offs, tok, _ = ops.moe_dispatch(b[1], b[3].shape[0])
+    want_g = ops.grouped_gemm(b[0], b[3], offs, rows=tok)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(4):
+        with torch.cuda.stream(s1):
+            outs.append((want_a, ops.moe_expert_ffn_w16(*a)))
+        with torch.cuda.stream(s2):
+            outs.append((want_b, ops.moe_expert_ffn_w16(*b)))
+            outs.append((want_g, ops.grouped_gemm(b[0], b[3], offs, rows=tok)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(w, o) for w, o in outs)
+    x = b[0].clone()
+    out, y = torch.empty_like(x), torch.empty_like(want_g)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.moe_expert_ffn_w16(x, *b[1:], out=out)
+        ops.grouped_gemm(x, b[3], offs, rows=tok, out=y)
+    for scale in (1.0, 0.5):
+        x.copy_(b[0] * scale)
+        out.zero_(), y.zero_()
+        graph.replay()
+        assert torch.equal(out, ops.moe_expert_ffn_w16(x, *b[1:])) and torch.equal(y, ops.grouped_gemm(x, b[3], offs, rows=tok))
+    assert torch.equal(out, out) and ops.operators16_status() == 0
+
+
+def test_empty_batches(dev):
+    from glmserve_b200 import ops
+    x0 = torch.empty((0, 64), dtype=torch.bfloat16, device=dev)
+    w = _randn((2, 32, 64), torch.bfloat16, dev, 1)
+    offs = _i32([0, 0, 0], dev)
+    assert ops.grouped_gemm(x0, w, offs).shape == (0, 32)
+    ids, wt = torch.empty((0, 2), dtype=torch.int32, device=dev), torch.empty((0, 2), device=dev)
+    assert ops.moe_expert_ffn_w16(x0, ids, wt, w, w, w.transpose(1, 2).contiguous()).shape == (0, 64)

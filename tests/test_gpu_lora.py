@@ -1,0 +1,154 @@
+"""Low-rank adapters (lora_add) against a plain 64-bit form.  Bounds as in test_gpu_expert16.py: an fp32 sum of m
+products is off by (m + 8) * 2^-23 of the sum of absolute products; B is applied to the fp32 values A x in pieces
+that keep at least 21 bits (2^-21 of every product); y is rounded once."""
+import numpy as np
+import pytest
+
+from test_gpu_expert16 import HALF, TINY, U, _check, _i32, _randn
+
+pytestmark = pytest.mark.gpu
+torch = pytest.importorskip("torch")
+
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "GPU tests need a CUDA device"
+    return torch.device("cuda:0")
+
+
+def _ref(y0, x, A, B, offs, rows, ranks, scales):
+    y = y0.double().clone()
+    bound = torch.zeros_like(y)
+    o = offs.tolist()
+    for a in range(A.shape[0]):
+        t = rows[o[a]:o[a + 1]].long()
+        t = t[(t >= 0) & (t < x.shape[0])]
+        if not t.numel():
+            continue
+        r = int(ranks[a]) if ranks is not None else A.shape[1]
+        s = float(scales[a]) if scales is not None else 1.0
+        xa, Aa, Ba = x[t].double(), A[a, :r].double(), B[a, :, :r].double()
+        v, va = s * (xa @ Aa.T), abs(s) * (xa.abs() @ Aa.abs().T)
+        d, da = v @ Ba.T, v.abs() @ Ba.abs().T
+        y[t] += d
+        bound[t] = va @ Ba.abs().T * ((x.shape[1] + 10) * U) + da * ((r + 8) * U + 2.0 ** -21) + (y0[t].double().abs() + d.abs()) * U
+    return y, bound
+
+
+CASES = [  # n, K, N, adapters, R, ranks, share without an adapter
+    (1, 8, 1, 1, 1, None, 0.0),
+    (1, 1024, 1024, 8, 16, None, 0.0),
+    (3, 72, 65, 2, 5, "mixed", 0.4),
+    (64, 512, 520, 64, 16, None, 0.1),
+    (64, 6144, 640, 7, 16, None, 0.0),
+    (100, 264, 1030, 3, 24, "mixed", 0.3),
+    (517, 1032, 2050, 21, 33, "mixed", 0.3),
+    (1030, 128, 136, 4, 64, None, 0.0),
+    (300, 2048, 300, 2, 256, "mixed", 0.2),
+    (2000, 256, 264, 1000, 8, "zeros", 0.5),
+    (700, 520, 1024, 5, 128, "mixed", 1.0),
+    (40, 16, 6144, 2, 7, None, 0.0),
+]
+
+
+def _case(i, dtype, ydt, dev):
+    n, K, N, nA, R, ranks, bare = CASES[i]
+    rng = np.random.default_rng(i)
+    ids = rng.integers(0, nA, n).astype(np.int32)
+    ids[rng.random(n) < bare] = -1
+    x, A, B = _randn((n, K), dtype, dev, i), _randn((nA, R, K), dtype, dev, 40 + i, 0.05), _randn((nA, N, R), dtype, dev, 80 + i, 0.05)
+    rk = None
+    if ranks:
+        rk = rng.integers(0 if ranks == "zeros" else 1, R + 1, nA).astype(np.int32)
+        for a in range(nA):    # what lies behind a rank must not matter
+            A[a, rk[a]:] = float("nan")
+            B[a, :, rk[a]:] = float("nan")
+        rk = torch.from_numpy(rk).to(dev)
+    scales = torch.from_numpy(rng.uniform(0.5, 2.0, nA).astype(np.float32)).to(dev) if i % 2 else None
+    return _randn((n, N), ydt, dev, 120 + i), x, A, B, torch.from_numpy(ids).to(dev), rk, scales
+
+
+@pytest.mark.parametrize("case", range(len(CASES)))
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("y_f32", [True, False])
+def test_lora_add(dev, case, dtype, y_f32):
+    from glmserve_b200 import ops
+    ydt = torch.float32 if y_f32 else dtype
+    y0, x, A, B, ids, ranks, scales = _case(case, dtype, ydt, dev)
+    offs, rows, _ = ops.moe_dispatch(ids[:, None].contiguous(), A.shape[0])
+    y = y0.clone()
+    assert ops.lora_add(y, x, A, B, offs, rows, ranks=ranks, scales=scales) is y
+    ref, b = _ref(y0, x, A, B, offs, rows, ranks, scales)
+    _check(y, ref, b + HALF[ydt] * (ref.abs() + b) + TINY[ydt], "lora")
+    assert torch.equal(y[ids < 0], y0[ids < 0])
+    again = y0.clone()
+    assert torch.equal(ops.lora_add(again, x, A, B, offs, rows, ranks=ranks, scales=scales), y)
+
+
+def test_lora_rows_out_of_range_are_skipped(dev):
+    from glmserve_b200 import ops
+    y0, x, A, B, _, _, _ = _case(3, torch.bfloat16, torch.float32, dev)
+    rows = _i32([5, -1, 64, 2 ** 31 - 1, 9, 0], dev)
+    offs = _i32([0] * 10 + [4] + [6] * 54, dev)
+    y = ops.lora_add(y0.clone(), x, A, B, offs, rows)
+    ref, b = _ref(y0, x, A, B, offs, rows, None, None)
+    _check(y, ref, b + HALF[torch.float32] * (ref.abs() + b), "lora")
+    keep = [i for i in range(64) if i not in (5, 9, 0)]
+    assert torch.equal(y[keep], y0[keep])
+
+
+def test_lora_beside_the_int4_projection(dev):
+    """gemm_w4a16 and the adapters of a mixed batch, as a projection with adapters runs."""
+    import oracle
+    from glmserve_b200 import ops
+    from glmserve_b200.quant import quantize_w4_np
+    rng = np.random.default_rng(0)
+    n, K, N, nA, R = 9, 256, 192, 3, 8
+    q, sc = quantize_w4_np((rng.standard_normal((N, K)) * 0.02).astype(np.float32), 128)
+    x = _randn((n, K), torch.bfloat16, dev, 1)
+    A, B = _randn((nA, R, K), torch.bfloat16, dev, 2, 0.05), _randn((nA, N, R), torch.bfloat16, dev, 3, 0.05)
+    ids = _i32([0, 2, -1, 1, 2, 2, -1, 0, 1], dev)
+    offs, rows, _ = ops.moe_dispatch(ids[:, None].contiguous(), nA)
+    base = ops.gemm_w4a16(x.float(), torch.from_numpy(q).to(dev), torch.from_numpy(sc).to(dev), 128)
+    np.testing.assert_allclose(base.cpu().numpy(), oracle.gemm_w4a16(x.float().cpu().numpy(), q, sc, 128), rtol=0, atol=1e-4)
+    y = ops.lora_add(base.clone(), x, A, B, offs, rows)
+    ref, b = _ref(base, x, A, B, offs, rows, None, None)
+    _check(y, ref, b + HALF[torch.float32] * (ref.abs() + b), "projection with adapters")
+
+
+def test_lora_graph_replay_with_another_batch_and_two_streams(dev):
+    from glmserve_b200 import ops
+    y0, x, A, B, ids, ranks, scales = _case(6, torch.float16, torch.float32, dev)
+    offs, rows, _ = ops.moe_dispatch(ids[:, None].contiguous(), A.shape[0])
+    want = ops.lora_add(y0.clone(), x, A, B, offs, rows, ranks=ranks, scales=scales)
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for s in (s1, s2):
+            with torch.cuda.stream(s):
+                got.append(ops.lora_add(y0.clone(), x, A, B, offs, rows, ranks=ranks, scales=scales))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+    y = y0.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.lora_add(y, x, A, B, offs, rows, ranks=ranks, scales=scales)
+    y.copy_(y0)
+    graph.replay()
+    assert torch.equal(y, want)
+    other = torch.roll(ids, 7).contiguous()          # the same graph serves the next batch's lists
+    o2, r2, _ = ops.moe_dispatch(other[:, None].contiguous(), A.shape[0])
+    m = int(o2[-1])
+    offs.copy_(o2), rows[:m].copy_(r2[:m]), y.copy_(y0)
+    graph.replay()
+    ref, b = _ref(y0, x, A, B, o2, r2[:m], ranks, scales)
+    _check(y, ref, b + HALF[torch.float32] * (ref.abs() + b), "replayed")
+
+
+def test_lora_empty_lists(dev):
+    from glmserve_b200 import ops
+    y0, x, A, B, ids, _, _ = _case(3, torch.bfloat16, torch.float32, dev)
+    offs, rows, _ = ops.moe_dispatch(torch.full_like(ids, -1)[:, None].contiguous(), A.shape[0])
+    assert torch.equal(ops.lora_add(y0.clone(), x, A, B, offs, rows), y0)
+    assert torch.equal(ops.lora_add(y0.clone(), x, A, B, offs, rows[:0]), y0)
