@@ -4,8 +4,11 @@
 //   h[p, :] = silu(gate[e] x) * (up[e] x),  y[p, :] = down[e] h[p, :],  out[t, :] = sum_k w[t, k] y[slot(t, k), :].
 // Products are summed in fp32; h is rounded once to the weights' type (the tensor cores read it in that type,
 // fp16 saturating at +-65504), the per-slot rows y stay fp32 and the sum over slots is taken in slot order.
-#include "common.cuh"
+#include <atomic>
+#include <type_traits>
+
 #include "launchers.cuh"
+#include "tc5.cuh"
 
 namespace gsb {
 
@@ -37,68 +40,360 @@ template <> __device__ __forceinline__ __half h_from_f(float v) { return sat_hal
 // never an access outside the buffers.
 __device__ __forceinline__ int seg_bound(const int* offsets, int e, int P) { return min(max(__ldg(offsets + e), 0), P); }
 
-// Plain form: 64 rows x 64 features per block, 4 x 4 per thread.
-template <typename T, typename Y, bool GU>
-__global__ void __launch_bounds__(256)
-grouped_simple_kernel(const GroupedArgs a) {
-    __shared__ float sx[64][17], sw[64][17], su[GU ? 64 : 1][17];
-    __shared__ int seg[3], srow[64];
-    const int tid = threadIdx.x;
-    const T* x = reinterpret_cast<const T*>(a.x);
+// ---- the tensor-core kernel -------------------------------------------------------------------
+// One item = 128 weight rows x up to NT token rows of one expert, as D[weight row, token] = sum_k W[row, k] X[token, k]
+// (M = 128 weight rows in the 128 TMEM lanes, N = tokens rounded up to 16): a decode batch pads tokens to 16, not to 128.
+// The 128 rows are two boxes of 64: consecutive rows of one matrix, or 64 gate rows and their 64 up rows, so that SwiGLU
+// pairs meet in the epilogue.  X rows are gathered by TMA (four rows an instruction), so no sorted copy is made.
+// A cluster of S CTAs works on one item, each on 1/S of K: the partial tiles are exchanged through distributed shared
+// memory, CTA r finishing the r-th part of the columns, and added in rank order - no atomics, the same bits every time.
+constexpr int kGrThreads = 256;            // warps: 0 weights, 1 MMA, 2 TMEM, 3 token rows, 4-7 epilogue
+constexpr int kMaxE = 1024;
+constexpr int kCh = 16;                    // accumulator columns a pass of the epilogue exchanges
+constexpr int kABytes = 128 * 128;         // 128 weight rows x 64 columns
+constexpr long long kGrWaitLimit = 2000000000LL;
+
+template <int NT> struct GrCfg {
+    static constexpr int kps = NT <= 16 ? 2 : 1;                   // k-blocks of 64 columns per stage
+    static constexpr int stages = NT <= 16 ? 5 : NT <= 64 ? 8 : 4;
+    static constexpr int bbytes = NT * 128;
+    static constexpr int stage_bytes = kps * (kABytes + bbytes);
+    static constexpr int red_bytes = 2 * kCh * 128 * 4;
+    static constexpr int tmem_cols = 2 * NT < 32 ? 32 : 2 * NT;
+    static constexpr size_t smem = (size_t)stages * stage_bytes + red_bytes + (kMaxE + 4) * 4 + 256;
+    static_assert(smem <= 227 * 1024, "stages exceed the shared memory of an SM");
+};
+
+__device__ int g_op16_status;
+
+struct GrItem { int e, p0, cnt, f0; };
+
+// item i: experts in order; inside one, all token tiles of a feature block run next to each other (they read the
+// same weights, which the second one finds in L2).  `e` only moves forward.
+template <int NT, int FW>
+__device__ __forceinline__ GrItem gr_item(const GroupedArgs& a, const int* pre, int i, int fb_count, int& e) {
+    while (i >= pre[e + 1] * fb_count) ++e;
+    const int nt = pre[e + 1] - pre[e], local = i - pre[e] * fb_count;
+    const int fb = local / nt, tt = local - fb * nt;
+    GrItem it;
+    it.e = e;
+    it.f0 = fb * FW;
+    const int lo = seg_bound(a.offsets, e, a.P), hi = seg_bound(a.offsets, e + 1, a.P);
+    it.p0 = lo + tt * NT;
+    it.cnt = min(NT, hi - it.p0);
+    return it;
+}
+
+__device__ __forceinline__ void gr_timeout(volatile int* abort_flag) {
+    *abort_flag = 1;
+    atomicCAS(&g_op16_status, 0, GSB_ERR_TIMEOUT);
+}
+
+template <int NT, typename T, typename Y, bool GU>
+__global__ void __launch_bounds__(kGrThreads, 1)
+grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_w2,
+               const __grid_constant__ CUtensorMap tm_x) {
+    using Cfg = GrCfg<NT>;
+    constexpr int FW = GU ? 64 : 128;      // output features of an item
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* s_stage = smem;
+    float* s_red = reinterpret_cast<float*>(smem + Cfg::stages * Cfg::stage_bytes);
+    int* pre = reinterpret_cast<int*>(s_red + 2 * kCh * 128);               // [E + 1] token tiles before expert e
+    uint64_t* full = reinterpret_cast<uint64_t*>(pre + kMaxE + 4);
+    uint64_t* empty = full + Cfg::stages;
+    uint64_t* acc_full = empty + Cfg::stages;
+    uint64_t* acc_empty = acc_full + 2;
+    uint64_t* red_full = acc_empty + 2;
+    uint64_t* red_free = red_full + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(red_free + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int S = (int)tc5::cluster_size(), rank = (int)tc5::cluster_rank();
     if (tid == 0) {
-        int t = blockIdx.y;
-        seg[0] = -1;
-        for (int e = 0; e < a.E; ++e) {
-            const int lo = seg_bound(a.offsets, e, a.P), hi = seg_bound(a.offsets, e + 1, a.P);
-            const int nt = hi > lo ? (hi - lo + 63) / 64 : 0;
-            if (t < nt) { seg[0] = e; seg[1] = lo + t * 64; seg[2] = min(64, hi - lo - t * 64); break; }
-            t -= nt;
+        for (int i = 0; i < Cfg::stages; ++i) { mbar_init(&full[i], 2); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 4);
+            mbar_init(&red_full[i], 4 * S); mbar_init(&red_free[i], 4 * S);
         }
+        *abort_flag = 0;
+        fence_barrier_init();
     }
-    __syncthreads();
-    const int e = seg[0], p0 = seg[1], cnt = seg[2], f0 = blockIdx.x * 64;
-    if (e < 0) return;
-    if (tid < 64) {
-        const int r = tid < cnt ? (a.rows ? __ldg(a.rows + p0 + tid) : p0 + tid) : -1;
-        srow[tid] = r >= 0 && r < a.n ? r : -1;
-    }
-    const T* w = reinterpret_cast<const T*>(a.w) + (int64_t)e * a.N * a.K;
-    const T* u = reinterpret_cast<const T*>(a.w2) + (int64_t)e * a.N * a.K;
-    float acc[4][4] = {}, acu[4][4] = {};
-    const int tr = tid >> 4, tf = tid & 15;
-    for (int k0 = 0; k0 < a.K; k0 += 16) {
-        __syncthreads();
-        for (int i = tid; i < 64 * 16; i += 256) {
-            const int r = i >> 4, k = k0 + (i & 15), f = f0 + r;
-            sx[r][i & 15] = srow[r] >= 0 && k < a.K ? to_f(x[(int64_t)srow[r] * a.K + k]) : 0.f;
-            sw[r][i & 15] = f < a.N && k < a.K ? to_f(w[(int64_t)f * a.K + k]) : 0.f;
-            if (GU) su[r][i & 15] = f < a.N && k < a.K ? to_f(u[(int64_t)f * a.K + k]) : 0.f;
+    if (warp == 2) { tc5::tmem_alloc(tmem_slot, Cfg::tmem_cols); tc5::tmem_relinquish(); }
+    int descending = (smem_u32(smem) & 1023u) != 0;    // (the swizzled tiles need a 1 KiB boundary: as good as no list)
+    {   // token tiles before every expert: 4 experts a thread, then a scan over the block
+        int c[4], sum = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int e = tid * 4 + j;
+            c[j] = sum;
+            if (e < a.E) {
+                const int lo = seg_bound(a.offsets, e, a.P), hi = seg_bound(a.offsets, e + 1, a.P);
+                sum += hi > lo ? (hi - lo + NT - 1) / NT : 0;
+                descending |= hi < lo;
+            }
         }
+        int incl = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += u;
+        }
+        int* wsum = reinterpret_cast<int*>(s_red);
+        if (lane == 31) wsum[warp] = incl;
         __syncthreads();
+        int base = incl - sum;
+        for (int w = 0; w < warp; ++w) base += wsum[w];
 #pragma unroll
-        for (int k = 0; k < 16; ++k)
+        for (int j = 0; j < 4; ++j)
+            if (tid * 4 + j <= a.E) pre[tid * 4 + j] = base + c[j];
+        if (tid == kGrThreads - 1 && a.E == kMaxE) pre[kMaxE] = base + sum;
+    }
+    tc5::fence_before();
+    descending = __syncthreads_or(descending);
+    tc5::fence_after();
+    if (S > 1) tc5::cluster_sync_all();    // the peers' barriers exist before anyone arrives on them
+    const uint32_t tmem = *tmem_slot;
+    const int nkb = (a.K + 63) >> 6, kb0 = nkb * rank / S, kb1 = nkb * (rank + 1) / S;
+    const int FB = (a.N + FW - 1) / FW;
+    // at most (E + P / NT) * FB, which the host has checked to fit; a list that is not ascending is no list
+    const int items = descending ? 0 : pre[a.E] * FB;
+    const int first = blockIdx.x / S, step = gridDim.x / S;
+
+    if (warp == 0) {
+        if (lane == 0) {                   // ---- weights
+            uint32_t st = 0, ph = 0;
+            int e = 0;
+            bool dead = false;
+            for (int i = first; i < items && !dead && !*abort_flag; i += step) {
+                const GrItem it = gr_item<NT, FW>(a, pre, i, FB, e);
+                for (int kb = kb0; kb < kb1; kb += Cfg::kps) {
+                    if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
+                    const int nk = min(Cfg::kps, kb1 - kb);
+                    mbar_arrive_expect_tx(&full[st], (uint32_t)nk * kABytes);
+                    uint8_t* dst = s_stage + st * Cfg::stage_bytes;
+                    for (int j = 0; j < nk; ++j) {
+                        tc5::tma_load_3d(dst + j * kABytes, &tm_w, (kb + j) * 64, it.f0, it.e, &full[st]);
+                        tc5::tma_load_3d(dst + j * kABytes + kABytes / 2, GU ? &tm_w2 : &tm_w, (kb + j) * 64,
+                                         GU ? it.f0 : it.f0 + 64, it.e, &full[st]);
+                    }
+                    if (++st == Cfg::stages) { st = 0; ph ^= 1u; }
+                }
+            }
+            // after a time-out elsewhere: nothing may still be copying into this block's memory when it ends
+            if (*abort_flag)
+                for (int j = 0; j < Cfg::stages; ++j) {
+                    if (st == 0) { st = Cfg::stages; ph ^= 1u; }
+                    --st;
+                    mbar_wait(&full[st], ph, kGrWaitLimit / 16);
+                }
+        }
+    } else if (warp == 3) {                // ---- token rows
+        uint32_t st = 0, ph = 0;
+        int e = 0;
+        bool dead = false;
+        constexpr int G = NT > 128 ? NT / 128 : 1;    // groups of four rows per lane
+        for (int i = first; i < items && !dead && !*abort_flag; i += step) {
+            const GrItem it = gr_item<NT, FW>(a, pre, i, FB, e);
+            const int nr = (it.cnt + 15) & ~15;
+            int r[G][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int g = 0; g < G; ++g)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    acc[i][j] = fmaf(sx[tr * 4 + i][k], sw[j * 16 + tf][k], acc[i][j]);
-                    if (GU) acu[i][j] = fmaf(sx[tr * 4 + i][k], su[j * 16 + tf][k], acu[i][j]);
+                    const int q = (g * 32 + lane) * 4 + j;
+                    // columns behind the tile's last row, and rows that do not exist, read row 0; neither is stored
+                    int v = 0;
+                    if (q < it.cnt) v = a.rows ? __ldg(a.rows + it.p0 + q) : it.p0 + q;
+                    r[g][j] = v >= 0 && v < a.n ? v : 0;
                 }
-    }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int r = tr * 4 + i, f = f0 + j * 16 + tf;
-            if (srow[r] < 0 || f >= a.N) continue;
-            reinterpret_cast<Y*>(a.y)[(int64_t)(p0 + r) * a.N + f] =
-                GU ? h_from_f<Y>(__fmul_rn(silu_ref(acc[i][j]), acu[i][j])) : from_f<Y>(acc[i][j]);
+            for (int kb = kb0; kb < kb1; kb += Cfg::kps) {
+                if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
+                const int nk = min(Cfg::kps, kb1 - kb);
+                if (lane == 0) mbar_arrive_expect_tx(&full[st], (uint32_t)(nk * nr * 128));
+                __syncwarp();
+                uint8_t* dst = s_stage + st * Cfg::stage_bytes + Cfg::kps * kABytes;
+                for (int j = 0; j < nk; ++j)
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const int q = (g * 32 + lane) * 4;
+                        if (q < nr) tc5::tma_gather4(dst + j * Cfg::bbytes + q * 128, &tm_x, (kb + j) * 64, r[g][0], r[g][1], r[g][2], r[g][3], &full[st]);
+                    }
+                if (++st == Cfg::stages) { st = 0; ph ^= 1u; }
+            }
+            dead = __any_sync(0xffffffffu, dead);
         }
+    } else if (warp == 1) {
+        if (lane == 0) {                   // ---- MMA issue
+            uint32_t st = 0, ph = 0, tl = 0;
+            int e = 0;
+            bool dead = false;
+            constexpr uint32_t ab = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+            const uint64_t d0 = tc5::desc_sw128(smem_u32(s_stage));
+            for (int i = first; i < items && !dead && !*abort_flag; i += step, ++tl) {
+                const GrItem it = gr_item<NT, FW>(a, pre, i, FB, e);
+                const uint32_t buf = tl & 1u;
+                if (!mbar_wait(&acc_empty[buf], ((tl >> 1) & 1u) ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); break; }
+                tc5::fence_after();
+                const uint32_t idesc = tc5::idesc_f16(ab, 128, (uint32_t)((it.cnt + 15) & ~15));
+                uint32_t acc = 0;
+                for (int kb = kb0; kb < kb1; kb += Cfg::kps) {
+                    if (!mbar_wait(&full[st], ph, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
+                    tc5::fence_after();
+                    const int nk = min(Cfg::kps, kb1 - kb);
+                    const uint64_t ad = d0 + (uint64_t)(st * (uint32_t)(Cfg::stage_bytes >> 4));
+                    const uint64_t bd = ad + (uint64_t)(Cfg::kps * kABytes >> 4);
+                    for (int j = 0; j < nk; ++j)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            tc5::mma_f16_ss(tmem + buf * NT, ad + (uint64_t)(j * (kABytes >> 4) + k * 2),
+                                            bd + (uint64_t)(j * (Cfg::bbytes >> 4) + k * 2), idesc, acc);
+                            acc = 1u;
+                        }
+                    tc5::commit(&empty[st]);
+                    if (++st == Cfg::stages) { st = 0; ph ^= 1u; }
+                }
+                if (!dead) tc5::commit(&acc_full[buf]);
+            }
+        }
+    } else if (warp >= 4) {                // ---- epilogue: this thread's TMEM lane = weight row
+        const int q = warp & 3, row = q * 32 + lane;
+        const int lsh = S == 4 ? 2 : S == 2 ? 1 : 0, per = kCh >> lsh;     // columns of a pass that one CTA finishes
+        const uint32_t red0 = smem_u32(s_red);
+        uint32_t tl = 0, cc = 0;
+        int e = 0;
+        bool dead = false;
+        Y* y = reinterpret_cast<Y*>(a.y);
+        for (int i = first; i < items && !dead; i += step, ++tl) {
+            const GrItem it = gr_item<NT, FW>(a, pre, i, FB, e);
+            const uint32_t buf = tl & 1u;
+            if (*abort_flag || !mbar_wait(&acc_full[buf], (tl >> 1) & 1u, kGrWaitLimit)) {
+                if (!*abort_flag) gr_timeout(abort_flag);
+                break;
+            }
+            tc5::fence_after();
+            for (int c0 = 0; c0 < it.cnt; c0 += kCh, ++cc) {
+                const uint32_t rb = cc & 1u, rph = (cc >> 1) & 1u;
+                uint32_t v[kCh];
+                tc5::tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + buf * NT + (uint32_t)c0, v);
+                tc5::tmem_ld_wait();
+                if (!tc5::wait_cluster(&red_free[rb], rph ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
+#pragma unroll
+                for (int j = 0; j < kCh; ++j) {
+                    const int owner = j >> (4 - lsh), jl = j & (per - 1);
+                    tc5::st_cluster(tc5::map_rank(red0 + (uint32_t)(((rb * kCh + rank * per + jl) * 128 + row) * 4), (uint32_t)owner),
+                                    __uint_as_float(v[j]));
+                }
+                __syncwarp();
+                if (lane < S) tc5::arrive_cluster(tc5::map_rank(smem_u32(&red_full[rb]), (uint32_t)lane));
+                if (!tc5::wait_cluster(&red_full[rb], rph, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
+                const float* red = s_red + rb * kCh * 128;
+                const int f = it.f0 + (GU ? (row & 63) : row);
+                for (int jl = GU ? row >> 6 : 0; jl < per; jl += GU ? 2 : 1) {
+                    const int c = c0 + rank * per + jl;
+                    if (c >= it.cnt || f >= a.N) continue;
+                    const int p = it.p0 + c;
+                    if (a.rows) { const int r = __ldg(a.rows + p); if (r < 0 || r >= a.n) continue; }
+                    float s0 = 0.f, s1 = 0.f;
+                    for (int src = 0; src < S; ++src) {
+                        s0 += red[(src * per + jl) * 128 + (GU ? (row & 63) : row)];
+                        if (GU) s1 += red[(src * per + jl) * 128 + (row & 63) + 64];
+                    }
+                    y[(int64_t)p * a.N + f] = GU ? h_from_f<Y>(__fmul_rn(silu_ref(s0), s1)) : from_f<Y>(s0);
+                }
+                __syncwarp();
+                if (lane < S) tc5::arrive_cluster(tc5::map_rank(smem_u32(&red_free[rb]), (uint32_t)lane));
+            }
+            tc5::fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&acc_empty[buf]);
+        }
+    }
+    __syncwarp();
+    tc5::fence_before();
+    __syncthreads();
+    if (S > 1) tc5::cluster_sync_all();    // peers may still read or signal this block's memory
+    if (warp == 2) { tc5::fence_after(); tc5::tmem_dealloc(tmem, Cfg::tmem_cols); }
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+    static const EncodeTiledFn fn = [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                        q == cudaDriverEntryPointSuccess;
+        return ok ? reinterpret_cast<EncodeTiledFn>(p) : nullptr;
+    }();
+    return fn;
+}
+
+// [d2, d1, d0] row-major 16-bit tensor (d2 = 0: two dims), boxes of 64 columns x box_rows rows, 128-byte swizzle.
+bool encode(CUtensorMap* m, const void* base, bool bf16, uint64_t d0, uint64_t d1, uint64_t d2, uint32_t box_rows) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return false;
+    const cuuint64_t dims[3] = {d0, d1, d2}, strides[2] = {d0 * 2, d0 * d1 * 2};
+    const cuuint32_t box[3] = {64, box_rows, 1}, estr[3] = {1, 1, 1};
+    return fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, d2 ? 3 : 2, const_cast<void*>(base),
+              dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int sm_count_of(int dev) {
+    static std::atomic<int> cached[64];
+    int v = dev < 64 ? cached[dev].load() : 0;
+    if (!v) {
+        if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+        if (dev < 64) cached[dev].store(v);
+    }
+    return v;
+}
+
+template <int NT, typename T, typename Y, bool GU>
+int run_grouped_nt(const GroupedArgs& a, int S, cudaStream_t s) {
+    using Cfg = GrCfg<NT>;
+    constexpr int FW = GU ? 64 : 128;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return GSB_ERR_CUDA;
+    const int sms = sm_count_of(dev);
+    if (!sms) return GSB_ERR_CUDA;
+    auto kernel = grouped_kernel<NT, T, Y, GU>;
+    static std::atomic<uint64_t> ready{0};     // devices on which the shared-memory size was raised
+    if (dev >= 64 || !((ready.load() >> dev) & 1u)) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg::smem) != cudaSuccess) return GSB_ERR_CUDA;
+        if (dev < 64) ready.fetch_or(1ull << dev);
+    }
+    const int64_t fbs = (a.N + FW - 1) / FW, tiles = (a.E < a.P ? a.E : a.P) + a.P / NT;
+    const int64_t items = tiles * fbs;
+    if (items + sms >= (int64_t)1 << 31) return GSB_ERR_TOO_LARGE;
+    CUtensorMap tw, tw2, tx;
+    constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
+    if (!encode(&tw, a.w, bf, a.K, a.N, a.E, 64) || !encode(&tw2, GU ? a.w2 : a.w, bf, a.K, a.N, a.E, 64) ||
+        !encode(&tx, a.x, bf, a.K, a.n, 0, 1))
+        return GSB_ERR_CUDA;
+    const int64_t groups = items < sms / S ? items : sms / S;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(groups * S)); cfg.blockDim = dim3(kGrThreads); cfg.dynamicSmemBytes = Cfg::smem; cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = (unsigned)S; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a, tw, tw2, tx) == cudaSuccess ? GSB_OK : GSB_ERR_LAUNCH;
 }
 
 template <typename T, typename Y, bool GU>
 int run_grouped(const GroupedArgs& a, cudaStream_t s) {
-    const int tiles = a.P / 64 + (a.E < a.P ? a.E : a.P);
-    grouped_simple_kernel<T, Y, GU><<<dim3((a.N + 63) / 64, tiles), 256, 0, s>>>(a);
-    return launch_status();
+    const int64_t per_expert = a.P / a.E, nkb = (a.K + 63) / 64;
+    const int nt = per_expert <= 16 ? 16 : per_expert <= 64 ? 64 : 256;
+    const int64_t fbs = (a.N + (GU ? 63 : 127)) / (GU ? 64 : 128), items = ((a.E < a.P ? a.E : a.P) + a.P / nt) * fbs;
+    int S = items >= 1184 ? 1 : items >= 592 ? 2 : 4;
+    while (S > nkb) S >>= 1;
+    if (nt == 16) return run_grouped_nt<16, T, Y, GU>(a, S, s);
+    if (nt == 64) return run_grouped_nt<64, T, Y, GU>(a, S, s);
+    return run_grouped_nt<256, T, Y, GU>(a, S, s);
 }
 
 template <typename T>
@@ -224,5 +519,9 @@ extern "C" int gsb_moe_expert_ffn_w16(const void* x, const int* topk_ids, const 
 }
 
 extern "C" int gsb_operators16_status(void) {
-    return cudaDeviceSynchronize() == cudaSuccess ? GSB_OK : GSB_ERR_CUDA;
+    int st = 0;
+    const int zero = 0;
+    if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyFromSymbol(&st, g_op16_status, sizeof(int)) != cudaSuccess) return GSB_ERR_CUDA;
+    if (st && cudaMemcpyToSymbol(g_op16_status, &zero, sizeof(int)) != cudaSuccess) return GSB_ERR_CUDA;
+    return st;
 }

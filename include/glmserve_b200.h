@@ -125,7 +125,8 @@ enum { GSB_TYPE_F32 = 0, GSB_TYPE_BF16 = 1, GSB_TYPE_F16 = 2 };
  * x [n,in] and w [E,out,in] of `type` (BF16 or F16), rows i32 [P] (NULL: row p itself, P <= n), expert_offsets
  * i32 [E+1] ascending as gsb_moe_dispatch writes it (rows = its sorted_token_ids), y [P,out] of y_type (`type`,
  * or F32).  Sums in fp32, one rounding at the end.  Rows of y that no segment covers, or whose rows[p] is outside
- * [0,n), are left as they were; an expert with an empty segment costs nothing.  Offsets outside [0,P] are clamped.
+ * [0,n), are left as they were; an expert with an empty segment costs nothing.  Offsets are clamped to [0,P]; with
+ * offsets that descend nothing is written.
  * in % 8 == 0, E <= 1024, P <= 2^30; x and w 16-byte aligned; y must not overlap the inputs. */
 GSB_API int gsb_grouped_gemm(const void* x, const void* w, int type, const int* expert_offsets,
                              const int* rows, int n, int P, int in, int out, int E, void* y,
