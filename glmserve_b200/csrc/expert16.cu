@@ -4,41 +4,11 @@
 //   h[p, :] = silu(gate[e] x) * (up[e] x),  y[p, :] = down[e] h[p, :],  out[t, :] = sum_k w[t, k] y[slot(t, k), :].
 // Products are summed in fp32; h is rounded once to the weights' type (the tensor cores read it in that type,
 // fp16 saturating at +-65504), the per-slot rows y stay fp32 and the sum over slots is taken in slot order.
-#include <atomic>
-#include <type_traits>
-
-#include "launchers.cuh"
-#include "tc5.cuh"
+#include "expert16.cuh"
 
 namespace gsb {
 
 namespace {
-
-struct GroupedArgs {
-    const void* x;          // [n, K]
-    const void* w;          // [E, N, K]; the gate matrices when w2 is given
-    const void* w2;         // [E, N, K] up matrices or null
-    const int* offsets;     // [E + 1]
-    const int* rows;        // [P] row of x for every p, or null (row p)
-    int n, P, K, N, E;
-    void* y;                // [P, N]
-};
-
-template <typename T> __device__ __forceinline__ float to_f(T v);
-template <> __device__ __forceinline__ float to_f(float v) { return v; }
-template <> __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <> __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-template <typename T> __device__ __forceinline__ T from_f(float v);
-template <> __device__ __forceinline__ float from_f(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
-// h of the FFN: fp16 saturates instead of turning into infinity and then NaN in the next product
-template <typename T> __device__ __forceinline__ T h_from_f(float v) { return from_f<T>(v); }
-template <> __device__ __forceinline__ __half h_from_f(float v) { return sat_half(v); }
-
-// Segment bounds as read from device memory, forced into [0, P]: a list that is not ascending gives wrong rows,
-// never an access outside the buffers.
-__device__ __forceinline__ int seg_bound(const int* offsets, int e, int P) { return min(max(__ldg(offsets + e), 0), P); }
 
 // ---- the tensor-core kernel -------------------------------------------------------------------
 // One item = 128 weight rows x up to NT token rows of one expert, as D[weight row, token] = sum_k W[row, k] X[token, k]
@@ -48,10 +18,8 @@ __device__ __forceinline__ int seg_bound(const int* offsets, int e, int P) { ret
 // A cluster of S CTAs works on one item, each on 1/S of K: the partial tiles are exchanged through distributed shared
 // memory, CTA r finishing the r-th part of the columns, and added in rank order - no atomics, the same bits every time.
 constexpr int kGrThreads = 256;            // warps: 0 weights, 1 MMA, 2 TMEM, 3 token rows, 4-7 epilogue
-constexpr int kMaxE = 1024;
 constexpr int kCh = 16;                    // accumulator columns a pass of the epilogue exchanges
 constexpr int kABytes = 128 * 128;         // 128 weight rows x 64 columns
-constexpr long long kGrWaitLimit = 2000000000LL;
 
 template <int NT> struct GrCfg {
     static constexpr int kps = NT <= 16 ? 2 : 1;                   // k-blocks of 64 columns per stage
@@ -65,8 +33,6 @@ template <int NT> struct GrCfg {
 };
 
 __device__ int g_op16_status;
-
-struct GrItem { int e, p0, cnt, f0; };
 
 // item i: experts in order; inside one, all token tiles of a feature block run next to each other (they read the
 // same weights, which the second one finds in L2).  `e` only moves forward.
@@ -121,34 +87,7 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
     }
     if (warp == 2) { tc5::tmem_alloc(tmem_slot, Cfg::tmem_cols); tc5::tmem_relinquish(); }
     int descending = (smem_u32(smem) & 1023u) != 0;    // (the swizzled tiles need a 1 KiB boundary: as good as no list)
-    {   // token tiles before every expert: 4 experts a thread, then a scan over the block
-        int c[4], sum = 0;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int e = tid * 4 + j;
-            c[j] = sum;
-            if (e < a.E) {
-                const int lo = seg_bound(a.offsets, e, a.P), hi = seg_bound(a.offsets, e + 1, a.P);
-                sum += hi > lo ? (hi - lo + NT - 1) / NT : 0;
-                descending |= hi < lo;
-            }
-        }
-        int incl = sum;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, incl, o);
-            if (lane >= o) incl += u;
-        }
-        int* wsum = reinterpret_cast<int*>(s_red);
-        if (lane == 31) wsum[warp] = incl;
-        __syncthreads();
-        int base = incl - sum;
-        for (int w = 0; w < warp; ++w) base += wsum[w];
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (tid * 4 + j <= a.E) pre[tid * 4 + j] = base + c[j];
-        if (tid == kGrThreads - 1 && a.E == kMaxE) pre[kMaxE] = base + sum;
-    }
+    descending |= gr_scan<NT>(a, pre, reinterpret_cast<int*>(s_red));
     tc5::fence_before();
     descending = __syncthreads_or(descending);
     tc5::fence_after();
@@ -316,42 +255,6 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
     if (warp == 2) { tc5::fence_after(); tc5::tmem_dealloc(tmem, Cfg::tmem_cols); }
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-    static const EncodeTiledFn fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-                        q == cudaDriverEntryPointSuccess;
-        return ok ? reinterpret_cast<EncodeTiledFn>(p) : nullptr;
-    }();
-    return fn;
-}
-
-// [d2, d1, d0] row-major 16-bit tensor (d2 = 0: two dims), boxes of 64 columns x box_rows rows, 128-byte swizzle.
-bool encode(CUtensorMap* m, const void* base, bool bf16, uint64_t d0, uint64_t d1, uint64_t d2, uint32_t box_rows) {
-    EncodeTiledFn fn = encode_fn();
-    if (!fn) return false;
-    const cuuint64_t dims[3] = {d0, d1, d2}, strides[2] = {d0 * 2, d0 * d1 * 2};
-    const cuuint32_t box[3] = {64, box_rows, 1}, estr[3] = {1, 1, 1};
-    return fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, d2 ? 3 : 2, const_cast<void*>(base),
-              dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-int sm_count_of(int dev) {
-    static std::atomic<int> cached[64];
-    int v = dev < 64 ? cached[dev].load() : 0;
-    if (!v) {
-        if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-        if (dev < 64) cached[dev].store(v);
-    }
-    return v;
-}
-
 template <int NT, typename T, typename Y, bool GU>
 int run_grouped_nt(const GroupedArgs& a, int S, cudaStream_t s) {
     using Cfg = GrCfg<NT>;
@@ -403,6 +306,7 @@ int run_grouped_any(const GroupedArgs& a, int y_type, cudaStream_t s) {
 }
 
 int launch_grouped(const GroupedArgs& a, int type, int y_type, cudaStream_t s) {
+    if (a.P / a.E > 64) return launch_grouped_pair(a, type, y_type, s);
     return type == GSB_TYPE_BF16 ? run_grouped_any<__nv_bfloat16>(a, y_type, s) : run_grouped_any<__half>(a, y_type, s);
 }
 
@@ -523,5 +427,6 @@ extern "C" int gsb_operators16_status(void) {
     const int zero = 0;
     if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyFromSymbol(&st, g_op16_status, sizeof(int)) != cudaSuccess) return GSB_ERR_CUDA;
     if (st && cudaMemcpyToSymbol(g_op16_status, &zero, sizeof(int)) != cudaSuccess) return GSB_ERR_CUDA;
-    return st;
+    const int pair = take_pair_status();
+    return st ? st : pair;
 }

@@ -1,0 +1,328 @@
+// The grouped product for many rows per expert: two CTAs of a cluster share one tile (tcgen05 cta_group::2).
+//
+// D[weight row, token] = sum_k W[row, k] X[token, k]: 256 weight rows (128 in each CTA's TMEM lanes) x up to 256 token
+// rows of one expert.  Each CTA stages its own 128 weight rows and half of the tokens; the tensor cores of both read
+// both halves, so a byte of shared memory feeds twice the products of a one-CTA tile - with a 128 x 256 tile per CTA the
+// operand reads plus the writes of the copies need 1.5 times the shared-memory bandwidth of an SM.
+// Weights come by TMA.  Token rows come by TMA as well when they lie in order (the down product); through a row list
+// eight warps gather them with 16-byte cp.async, writing the swizzled tile themselves: TMA's gather takes ~70 cycles per
+// four rows, 4.5 times the 512 cycles a 64-column k-block of this tile multiplies for (250 TFLOP/s with it), and a
+// sorted copy of the rows would cost an extra pass over them.
+// SwiGLU: a CTA's 128 weight rows are 64 gate rows and their 64 up rows; the epilogue warps swap halves through shared
+// memory.  Two accumulators (2 x 256 TMEM columns), so the epilogue of a tile runs under the next one's main loop.
+#include "expert16.cuh"
+
+namespace gsb {
+
+namespace {
+
+constexpr int kPrNT = 256;                 // token rows per tile at most
+constexpr int kPrStages = 6;
+constexpr int kPrHalf = 128 * 128;         // 128 rows x 64 columns: weights, or this CTA's tokens
+constexpr int kPrStageBytes = 2 * kPrHalf;
+constexpr int kPrXch = 2 * 2 * 16 * 64 * 4; // two buffers of 2 x 16 columns x 64 rows fp32
+constexpr int kPrThreads = 512;            // warps: 0 weights, 1 MMA, 2 TMEM, 3 tokens (TMA), 4-7 epilogue, 8-15 gather
+constexpr size_t kPrSmem = (size_t)kPrStages * kPrStageBytes + kPrXch + (kMaxE + 4) * 4 + 256;
+static_assert(kPrSmem <= 227 * 1024, "stages exceed the shared memory of an SM");
+
+__device__ int g_pair_status;
+
+__device__ __forceinline__ void pr_timeout(volatile int* abort_flag) {
+    *abort_flag = 1;
+    atomicCAS(&g_pair_status, 0, GSB_ERR_TIMEOUT);
+}
+
+// Item i: experts in order, inside one the token tiles of a feature block next to each other (same weights).  An
+// expert's rows are cut into equal tiles (multiples of 32 rows) instead of full ones and a rest.
+template <int FW>
+__device__ __forceinline__ GrItem pr_item(const GroupedArgs& a, const int* pre, int i, int fb_count, int& e) {
+    while (i >= pre[e + 1] * fb_count) ++e;
+    const int nt = pre[e + 1] - pre[e], local = i - pre[e] * fb_count;
+    const int fb = local / nt, tt = local - fb * nt;
+    const int lo = seg_bound(a.offsets, e, a.P), hi = seg_bound(a.offsets, e + 1, a.P);
+    const int rows = ((hi - lo + nt - 1) / nt + 31) & ~31;
+    GrItem it;
+    it.e = e;
+    it.f0 = fb * FW;
+    it.p0 = lo + tt * rows;
+    it.cnt = min(rows, hi - it.p0);
+    return it;
+}
+
+template <typename T, typename Y, bool GU, bool GATHER>
+__global__ void __launch_bounds__(kPrThreads, 1)
+grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_w2,
+                    const __grid_constant__ CUtensorMap tm_x) {
+    constexpr int FW = GU ? 128 : 256;     // output features of an item (both CTAs)
+    extern __shared__ __align__(1024) uint8_t smem[];
+    float* s_xch = reinterpret_cast<float*>(smem + kPrStages * kPrStageBytes);
+    int* pre = reinterpret_cast<int*>(smem + kPrStages * kPrStageBytes + kPrXch);
+    uint64_t* full = reinterpret_cast<uint64_t*>(pre + kMaxE + 4);     // the leader's are used, for both CTAs' data
+    uint64_t* empty = full + kPrStages;
+    uint64_t* acc_full = empty + kPrStages;
+    uint64_t* acc_empty = acc_full + 2;                                // the leader's are used
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int rank = (int)tc5::cluster_rank();
+    if (tid == 0) {
+        for (int i = 0; i < kPrStages; ++i) {
+            mbar_init(&full[i], GATHER ? 1 + 2 * 2 : 1);   // the weights' byte count, and two gather warps of each CTA
+            mbar_init(&empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 2 * 4); }
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    int descending = (smem_u32(smem) & 1023u) != 0;
+    descending |= gr_scan<kPrNT>(a, pre, reinterpret_cast<int*>(s_xch));
+    descending = __syncthreads_or(descending);
+    tc5::cluster_sync_all();
+    if (warp == 2) { tc5::tmem_alloc2(tmem_slot, 512); tc5::tmem_relinquish2(); }
+    tc5::fence_before();
+    tc5::cluster_sync_all();               // the peer has its barriers and its TMEM
+    tc5::fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int nkb = (a.K + 63) >> 6;
+    const int FB = (a.N + FW - 1) / FW;
+    const int items = descending ? 0 : pre[a.E] * FB;
+    const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+    const int fr = rank * (FW / 2);        // this CTA's features start here inside an item
+
+    if (warp == 0) {
+        if (lane == 0) {                   // ---- weights of this CTA; bytes are counted on the leader's barrier
+            uint32_t st = 0, ph = 0;
+            int e = 0;
+            bool dead = false;
+            for (int i = first; i < items && !dead && !*abort_flag; i += step) {
+                const GrItem it = pr_item<FW>(a, pre, i, FB, e);
+                const int nb = ((it.cnt + 31) / 32 * 16 + 31) / 32;     // token boxes of 32 rows per CTA
+                for (int kb = 0; kb < nkb; ++kb) {
+                    if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { pr_timeout(abort_flag); dead = true; break; }
+                    if (rank == 0) mbar_arrive_expect_tx(&full[st], 2u * (kPrHalf + (GATHER ? 0u : (uint32_t)nb * 4096u)));
+                    const uint32_t bar = tc5::map_rank(smem_u32(&full[st]), 0);
+                    uint8_t* dst = smem + st * kPrStageBytes;
+                    tc5::tma2_load_3d(dst, &tm_w, kb * 64, it.f0 + fr, it.e, bar);
+                    tc5::tma2_load_3d(dst + kPrHalf / 2, GU ? &tm_w2 : &tm_w, kb * 64, GU ? it.f0 + fr : it.f0 + fr + 64, it.e, bar);
+                    if (++st == kPrStages) { st = 0; ph ^= 1u; }
+                }
+            }
+            // the signals of the last MMAs have arrived before the block ends
+            for (int j = 0; j < kPrStages && !*abort_flag; ++j) {
+                mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit);
+                if (++st == kPrStages) { st = 0; ph ^= 1u; }
+            }
+            // after a time-out: nothing may still be copying into this block's memory when it ends
+            if (*abort_flag && rank == 0)
+                for (int j = 0; j < kPrStages; ++j) {
+                    if (st == 0) { st = kPrStages; ph ^= 1u; }
+                    --st;
+                    mbar_wait(&full[st], ph, kGrWaitLimit / 16);
+                }
+        }
+    } else if (warp == 3) {
+        if (!GATHER && lane == 0) {        // ---- this CTA's half of the token rows, in order
+            uint32_t st = 0, ph = 0;
+            int e = 0;
+            bool dead = false;
+            for (int i = first; i < items && !dead && !*abort_flag; i += step) {
+                const GrItem it = pr_item<FW>(a, pre, i, FB, e);
+                const int half = (it.cnt + 31) / 32 * 16, nb = (half + 31) / 32;
+                for (int kb = 0; kb < nkb; ++kb) {
+                    if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { pr_timeout(abort_flag); dead = true; break; }
+                    const uint32_t bar = tc5::map_rank(smem_u32(&full[st]), 0);
+                    for (int b = 0; b < nb; ++b)
+                        tc5::tma2_load_2d(smem + st * kPrStageBytes + kPrHalf + b * 4096, &tm_x, kb * 64, it.p0 + rank * half + b * 32, bar);
+                    if (++st == kPrStages) { st = 0; ph ^= 1u; }
+                }
+            }
+        }
+    } else if (warp >= 8) {
+        if (GATHER) {                      // ---- this CTA's half of the token rows, through the list
+            // Two warps a k-block (64 rows each; eight lanes copy the 128 bytes of a row, four rows an instruction), four
+            // such groups in turn: a group waits for its own copies and fences them before it hands the k-block over, so
+            // what hides that latency is the other three groups' copies.
+            const int group = (warp - 8) >> 1, sub = (warp - 8) & 1, chunk = lane & 7;
+            const T* x = reinterpret_cast<const T*>(a.x) + chunk * 8;
+            uint32_t st = 0, ph = 0, cnt = 0;
+            int e = 0;
+            bool dead = false;
+            for (int i = first; i < items && !dead && !*abort_flag; i += step) {
+                const GrItem it = pr_item<FW>(a, pre, i, FB, e);
+                const int half = (it.cnt + 31) / 32 * 16;
+                int r[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int p = rank * half + sub * 64 + j * 4 + (lane >> 3);
+                    // tokens behind the tile's last, and rows that do not exist, read row 0; neither is stored
+                    r[j] = p < it.cnt ? __ldg(a.rows + it.p0 + p) : 0;
+                    if (r[j] < 0 || r[j] >= a.n) r[j] = 0;
+                }
+                const int nj = max(0, (half - sub * 64 + 3) / 4);          // half is a multiple of 16
+                for (int kb = 0; kb < nkb; ++kb, ++cnt) {
+                    if ((int)(cnt & 3u) == group) {
+                        if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { pr_timeout(abort_flag); dead = true; break; }
+                        const uint32_t base = smem_u32(smem) + st * kPrStageBytes + kPrHalf + (uint32_t)((sub * 64 + (lane >> 3)) * 128);
+                        const bool in = kb * 64 + chunk * 8 < a.K;
+                        const T* xk = in ? x + kb * 64 : x;
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            if (j < nj)     // 128-byte swizzle: 16-byte piece c of row q lies at c ^ (q % 8); sub * 64 is a multiple of 8
+                                tc5::cp_async16(base + (uint32_t)(j * 512 + ((chunk ^ ((j * 4 + (lane >> 3)) & 7)) << 4)), xk + (int64_t)r[j] * a.K, in);
+                        tc5::cp_async_commit();
+                        tc5::cp_async_wait<0>();
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) tc5::arrive_cluster(tc5::map_rank(smem_u32(&full[st]), 0));
+                    }
+                    if (++st == kPrStages) { st = 0; ph ^= 1u; }
+                }
+                dead = __any_sync(0xffffffffu, dead);
+            }
+            tc5::cp_async_wait<0>();
+        }
+    } else if (warp == 1) {
+        if (rank == 0 && lane == 0) {      // ---- MMA issue for the pair
+            uint32_t st = 0, ph = 0, tl = 0;
+            int e = 0;
+            bool dead = false;
+            constexpr uint32_t ab = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+            const uint64_t d0 = tc5::desc_sw128(smem_u32(smem));
+            for (int i = first; i < items && !dead && !*abort_flag; i += step, ++tl) {
+                const GrItem it = pr_item<FW>(a, pre, i, FB, e);
+                const uint32_t buf = tl & 1u;
+                if (!tc5::wait_cluster(&acc_empty[buf], ((tl >> 1) & 1u) ^ 1u, kGrWaitLimit)) { pr_timeout(abort_flag); break; }
+                tc5::fence_after();
+                const uint32_t idesc = tc5::idesc_f16(ab, 256, (uint32_t)((it.cnt + 31) & ~31));
+                uint32_t acc = 0;
+                for (int kb = 0; kb < nkb; ++kb) {
+                    if (!tc5::wait_cluster(&full[st], ph, kGrWaitLimit)) { pr_timeout(abort_flag); dead = true; break; }
+                    tc5::fence_after();
+                    const uint64_t ad = d0 + (uint64_t)(st * (uint32_t)(kPrStageBytes >> 4));
+                    const uint64_t bd = ad + (uint64_t)(kPrHalf >> 4);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        tc5::mma2_f16_ss(tmem + buf * kPrNT, ad + (uint64_t)(k * 2), bd + (uint64_t)(k * 2), idesc, acc);
+                        acc = 1u;
+                    }
+                    tc5::commit2(&empty[st]);
+                    if (++st == kPrStages) { st = 0; ph ^= 1u; }
+                }
+                if (!dead) tc5::commit2(&acc_full[buf]);
+            }
+        }
+    } else if (warp >= 4) {                // ---- epilogue: this thread's TMEM lane = weight row of this CTA
+        const int q = warp & 3, row = q * 32 + lane;
+        uint32_t tl = 0;
+        int e = 0;
+        Y* y = reinterpret_cast<Y*>(a.y);
+        uint32_t xb = 0;
+        for (int i = first; i < items; i += step, ++tl) {
+            const GrItem it = pr_item<FW>(a, pre, i, FB, e);
+            const uint32_t buf = tl & 1u;
+            // all four warps must agree to go on: they meet at a block barrier in the loop below
+            int ok = *abort_flag ? 0 : (int)mbar_wait(&acc_full[buf], (tl >> 1) & 1u, kGrWaitLimit);
+            if (!ok) pr_timeout(abort_flag);
+            if (GU) {
+                asm volatile("{\n\t.reg .pred p, r;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred r, 1, 128, p;\n\tselp.u32 %0, 1, 0, r;\n\t}" : "=r"(ok) : "r"(ok) : "memory");
+            }
+            if (!ok) break;
+            tc5::fence_after();
+            const int f = it.f0 + fr + (GU ? (row & 63) : row);
+            const bool have = f < a.N;
+            for (int c0 = 0; c0 < it.cnt; c0 += 32) {
+                uint32_t v[32];
+                tc5::tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + buf * kPrNT + (uint32_t)c0, v);
+                // which of the 32 tokens exist
+                int r = c0 + lane < it.cnt ? 0 : -1;
+                if (GATHER && r == 0) r = __ldg(a.rows + it.p0 + c0 + lane);
+                const uint32_t live = __ballot_sync(0xffffffffu, r >= 0 && (!GATHER || r < a.n));
+                tc5::tmem_ld_wait();
+                Y* o = y + (int64_t)(it.p0 + c0) * a.N + f;
+                if (GU) {
+                    // warps 0, 1 hold gate rows, 2, 3 the up rows of the same features: each side keeps 16 of the
+                    // 32 columns and passes the other 16 on
+                    float* xs = s_xch + xb * 2048 + (q >> 1) * 1024 + (row & 63);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) xs[j * 64] = __uint_as_float(v[q < 2 ? 16 + j : j]);
+                    asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
+                    const float* xo = s_xch + xb * 2048 + ((q >> 1) ^ 1) * 1024 + (row & 63);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const int c = q < 2 ? j : 16 + j;
+                        const float mine = __uint_as_float(v[q < 2 ? j : 16 + j]), other = xo[j * 64];
+                        const float h = q < 2 ? __fmul_rn(silu_ref(mine), other) : __fmul_rn(silu_ref(other), mine);
+                        if (have && ((live >> c) & 1u)) o[(int64_t)c * a.N] = h_from_f<Y>(h);
+                    }
+                    xb ^= 1u;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (have && ((live >> j) & 1u)) o[(int64_t)j * a.N] = from_f<Y>(__uint_as_float(v[j]));
+                }
+            }
+            tc5::fence_before();
+            __syncwarp();
+            if (lane == 0) tc5::arrive_cluster(tc5::map_rank(smem_u32(&acc_empty[buf]), 0));
+        }
+    }
+    __syncwarp();
+    tc5::fence_before();
+    __syncthreads();
+    tc5::cluster_sync_all();               // the peer's MMAs and signals reach into this block's memory
+    if (warp == 2) { tc5::fence_after(); tc5::tmem_dealloc2(tmem, 512); }
+}
+
+template <typename T, typename Y, bool GU, bool GATHER>
+int run_pair(const GroupedArgs& a, cudaStream_t s) {
+    constexpr int FW = GU ? 128 : 256;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return GSB_ERR_CUDA;
+    const int sms = sm_count_of(dev);
+    if (sms < 2) return GSB_ERR_CUDA;
+    auto kernel = grouped_pair_kernel<T, Y, GU, GATHER>;
+    static std::atomic<uint64_t> ready{0};
+    if (dev >= 64 || !((ready.load() >> dev) & 1u)) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPrSmem) != cudaSuccess) return GSB_ERR_CUDA;
+        if (dev < 64) ready.fetch_or(1ull << dev);
+    }
+    const int64_t fbs = (a.N + FW - 1) / FW, items = ((a.E < a.P ? a.E : a.P) + a.P / kPrNT) * fbs;
+    if (items + sms >= (int64_t)1 << 31) return GSB_ERR_TOO_LARGE;
+    CUtensorMap tw, tw2, tx;
+    constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
+    if (!encode(&tw, a.w, bf, a.K, a.N, a.E, 64) || !encode(&tw2, GU ? a.w2 : a.w, bf, a.K, a.N, a.E, 64) ||
+        !encode(&tx, a.x, bf, a.K, a.n, 0, 32))
+        return GSB_ERR_CUDA;
+    const int64_t pairs = items < sms / 2 ? items : sms / 2;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(pairs * 2)); cfg.blockDim = dim3(kPrThreads); cfg.dynamicSmemBytes = kPrSmem; cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, a, tw, tw2, tx) == cudaSuccess ? GSB_OK : GSB_ERR_LAUNCH;
+}
+
+template <typename T>
+int run_pair_any(const GroupedArgs& a, int y_type, cudaStream_t s) {
+    if (a.w2) return run_pair<T, T, true, true>(a, s);
+    if (a.rows) return y_type == GSB_TYPE_F32 ? run_pair<T, float, false, true>(a, s) : run_pair<T, T, false, true>(a, s);
+    return y_type == GSB_TYPE_F32 ? run_pair<T, float, false, false>(a, s) : run_pair<T, T, false, false>(a, s);
+}
+
+}  // namespace
+
+int launch_grouped_pair(const GroupedArgs& a, int type, int y_type, cudaStream_t s) {
+    return type == GSB_TYPE_BF16 ? run_pair_any<__nv_bfloat16>(a, y_type, s) : run_pair_any<__half>(a, y_type, s);
+}
+
+int take_pair_status() {
+    int st = 0;
+    const int zero = 0;
+    if (cudaMemcpyFromSymbol(&st, g_pair_status, sizeof(int)) != cudaSuccess) return GSB_ERR_CUDA;
+    if (st && cudaMemcpyToSymbol(g_pair_status, &zero, sizeof(int)) != cudaSuccess) return GSB_ERR_CUDA;
+    return st;
+}
+
+}  // namespace gsb
