@@ -87,7 +87,7 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
     }
     if (warp == 2) { tc5::tmem_alloc(tmem_slot, Cfg::tmem_cols); tc5::tmem_relinquish(); }
     int descending = (smem_u32(smem) & 1023u) != 0;    // (the swizzled tiles need a 1 KiB boundary: as good as no list)
-    descending |= gr_scan<NT>(a, pre, reinterpret_cast<int*>(s_red));
+    descending |= seg_scan<NT>(a.offsets, a.E, a.P, pre, reinterpret_cast<int*>(s_red));
     tc5::fence_before();
     descending = __syncthreads_or(descending);
     tc5::fence_after();
@@ -357,7 +357,6 @@ Ffn16Ws carve16(int n, int topk, int H, int I, int E, void* base) {
     return ws;
 }
 
-inline bool misaligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a != 0; }
 inline bool is16(int type) { return type == GSB_TYPE_BF16 || type == GSB_TYPE_F16; }
 inline size_t type_bytes(int type) { return type == GSB_TYPE_F32 ? 4 : 2; }
 constexpr int64_t kMaxSlots = (int64_t)1 << 30;

@@ -76,7 +76,7 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
         fence_barrier_init();
     }
     int descending = (smem_u32(smem) & 1023u) != 0;
-    descending |= gr_scan<kPrNT>(a, pre, reinterpret_cast<int*>(s_xch));
+    descending |= seg_scan<kPrNT>(a.offsets, a.E, a.P, pre, reinterpret_cast<int*>(s_xch));
     descending = __syncthreads_or(descending);
     tc5::cluster_sync_all();
     if (warp == 2) { tc5::tmem_alloc2(tmem_slot, 512); tc5::tmem_relinquish2(); }
