@@ -61,8 +61,15 @@ def lib():
         L.gsb_comm_set_wait_cycles.argtypes = [C.c_void_p, C.c_longlong]
         L.gsb_comm_open_loopback.argtypes = [C.c_void_p]
         L.gsb_prefill_wait_profile.argtypes = [C.c_void_p]
-        L.gsb_moe_expert_ffn_w16_workspace_bytes.restype = C.c_size_t
-        L.gsb_lora_scratch_bytes.restype = C.c_size_t
+        # argument types given, so that plain integers do as pointers and sizes
+        V, I, Z = C.c_void_p, C.c_int, C.c_size_t
+        L.gsb_grouped_gemm.argtypes = [V, V, I, V, V, I, I, I, I, I, V, I, V]
+        L.gsb_moe_expert_ffn_w16_workspace_bytes.argtypes = [I] * 5
+        L.gsb_moe_expert_ffn_w16_workspace_bytes.restype = Z
+        L.gsb_moe_expert_ffn_w16.argtypes = [V] * 6 + [I] * 6 + [V, I, V, Z, V]
+        L.gsb_lora_scratch_bytes.argtypes = [I] * 3
+        L.gsb_lora_scratch_bytes.restype = Z
+        L.gsb_lora_add.argtypes = [V, V, V, I, V, V, V, V] + [I] * 6 + [V, I, V, Z, V]
         _lib = L
     return _lib
 

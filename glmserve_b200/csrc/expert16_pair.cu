@@ -291,7 +291,7 @@ int run_pair(const GroupedArgs& a, cudaStream_t s) {
     if (items + sms >= (int64_t)1 << 31) return GSB_ERR_TOO_LARGE;
     CUtensorMap tw, tw2, tx;
     constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
-    if (!encode(&tw, a.w, bf, a.K, a.N, a.E, 64) || !encode(&tw2, GU ? a.w2 : a.w, bf, a.K, a.N, a.E, 64) ||
+    if (!encode(&tw, a.w, bf, a.K, a.N, a.E, 64) || (GU && !encode(&tw2, a.w2, bf, a.K, a.N, a.E, 64)) ||
         !encode(&tx, a.x, bf, a.K, a.n, 0, 32))
         return GSB_ERR_CUDA;
     const int64_t pairs = items < sms / 2 ? items : sms / 2;
@@ -301,7 +301,7 @@ int run_pair(const GroupedArgs& a, cudaStream_t s) {
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, a, tw, tw2, tx) == cudaSuccess ? GSB_OK : GSB_ERR_LAUNCH;
+    return cudaLaunchKernelEx(&cfg, kernel, a, tw, GU ? tw2 : tw, tx) == cudaSuccess ? GSB_OK : GSB_ERR_LAUNCH;
 }
 
 template <typename T>

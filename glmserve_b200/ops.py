@@ -6,6 +6,7 @@ tensors used only as device buffers; every call runs on torch's current stream.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 
 import torch
@@ -104,15 +105,27 @@ def moe_expert_ffn(x, topk_ids, topk_w, gate_w, up_w, down_w):
 _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
+_HERE = contextlib.nullcontext()
+
+
+def _device_of(x):
+    """Context in which x's device is the current one (nothing to do where it is already)."""
+    return _HERE if x.get_device() == torch.cuda.current_device() else torch.cuda.device(x.device)
+
+
+def _raw_stream(x):
+    """Handle of torch's current stream on x's device; torch.cuda.current_stream() builds an object around it, which
+    takes longer than a small call's kernel launch."""
+    return torch._C._cuda_getCurrentRawStream(x.get_device())
+
+
 def _need16(x, *named):
-    """x: a bf16 or fp16 CUDA tensor; (t, dtype or None = x's, dims, name) the others, all on x's device."""
+    """x: a bf16 or fp16 CUDA tensor; (t, dtype, dims, name) the others, all on x's device."""
     if not x.is_cuda or x.dtype not in (torch.bfloat16, torch.float16) or not x.is_contiguous() or x.dim() != 2:
         raise ValueError("x: expected a contiguous 2-D CUDA tensor of torch.bfloat16 or torch.float16")
+    dev = x.get_device()
     for t, dtype, dims, name in named:
-        if t is None:
-            continue
-        dtype = dtype or x.dtype
-        if not t.is_cuda or t.device != x.device or t.dtype != dtype or not t.is_contiguous() or t.dim() != dims:
+        if t is not None and (t.dtype != dtype or t.dim() != dims or t.get_device() != dev or not t.is_contiguous()):
             raise ValueError(f"{name}: expected a contiguous {dims}-D tensor of {dtype} on {x.device}")
 
 
@@ -122,9 +135,9 @@ def _out16(out, shape, x, out_dtype, name="out"):
         if out_dtype not in (x.dtype, torch.float32):
             raise ValueError(f"out_dtype: expected {x.dtype} or torch.float32")
         return torch.empty(shape, dtype=out_dtype, device=x.device)
-    if not out.is_cuda or out.device != x.device or out.dtype not in (x.dtype, torch.float32) or \
-            not out.is_contiguous() or tuple(out.shape) != tuple(shape) or out_dtype not in (None, out.dtype):
-        raise ValueError(f"{name}: expected a contiguous tensor {tuple(shape)} of {x.dtype} or torch.float32 on {x.device}")
+    if out.dtype not in (x.dtype, torch.float32) or out.get_device() != x.get_device() or \
+            not out.is_contiguous() or tuple(out.shape) != shape or out_dtype not in (None, out.dtype):
+        raise ValueError(f"{name}: expected a contiguous tensor {shape} of {x.dtype} or torch.float32 on {x.device}")
     return out
 
 
@@ -134,16 +147,17 @@ def grouped_gemm(x, w, expert_offsets, rows=None, out=None, out_dtype=None):
     expert_offsets int32 [E+1] and rows int32 [P] as ``moe_dispatch`` returns them (offsets, sorted_token_ids);
     without ``rows`` row p is x[p].  Returns y [P,N] of x's type (or float32 with ``out_dtype`` / ``out``).  Rows
     that no segment covers are left as they were in ``out``; without ``out`` their contents are undefined."""
-    _need16(x, (w, None, 3, "w"), (expert_offsets, torch.int32, 1, "expert_offsets"), (rows, torch.int32, 1, "rows"))
+    _need16(x, (w, x.dtype, 3, "w"), (expert_offsets, torch.int32, 1, "expert_offsets"), (rows, torch.int32, 1, "rows"))
     n, K = x.shape
-    E, N = w.shape[:2]
-    if w.shape[2] != K or expert_offsets.shape[0] != E + 1:
+    E, N, Kw = w.shape
+    if Kw != K or expert_offsets.shape[0] != E + 1:
         raise ValueError("grouped_gemm: expected w [E,N,K] with x's K and expert_offsets [E+1]")
     P = n if rows is None else rows.shape[0]
     out = _out16(out, (P, N), x, out_dtype)
-    with torch.cuda.device(x.device):
-        check(lib().gsb_grouped_gemm(_p(x), _p(w), _TYPE[x.dtype], _p(expert_offsets), _p(rows), n, P, K, N, E,
-                                     _p(out), _TYPE[out.dtype], _stream()), "grouped_gemm")
+    with _device_of(x):
+        check(lib().gsb_grouped_gemm(x.data_ptr(), w.data_ptr(), _TYPE[x.dtype], expert_offsets.data_ptr(),
+                                     None if rows is None else rows.data_ptr(), n, P, K, N, E, out.data_ptr(),
+                                     _TYPE[out.dtype], _raw_stream(x)), "grouped_gemm")
     return out
 
 
@@ -151,21 +165,22 @@ def moe_expert_ffn_w16(x, topk_ids, topk_w, gate_w, up_w, down_w, out=None, out_
     """``moe_expert_ffn`` with bf16/fp16 activations and weights on the tensor cores: x [n,H], topk_ids int32 and
     topk_w float32 [n,topk], gate_w/up_w [E,I,H], down_w [E,H,I] -> out [n,H] of x's type (or float32).  A slot
     whose id is outside [0,E) adds nothing (padding, or an expert on another GPU)."""
-    _need16(x, (topk_ids, torch.int32, 2, "ids"), (topk_w, torch.float32, 2, "w"), (gate_w, None, 3, "gate_w"),
-            (up_w, None, 3, "up_w"), (down_w, None, 3, "down_w"))
+    _need16(x, (topk_ids, torch.int32, 2, "ids"), (topk_w, torch.float32, 2, "w"), (gate_w, x.dtype, 3, "gate_w"),
+            (up_w, x.dtype, 3, "up_w"), (down_w, x.dtype, 3, "down_w"))
     n, H = x.shape
-    E, I = gate_w.shape[:2]
+    E, I, _ = gate_w.shape
     topk = topk_ids.shape[1]
     if gate_w.shape != (E, I, H) or up_w.shape != (E, I, H) or down_w.shape != (E, H, I) or \
             topk_ids.shape != (n, topk) or topk_w.shape != (n, topk):
         raise ValueError("moe_expert_ffn_w16: expected gate_w, up_w [E,I,H], down_w [E,H,I], ids and w [n,topk]")
     out = _out16(out, (n, H), x, out_dtype)
-    nbytes = int(lib().gsb_moe_expert_ffn_w16_workspace_bytes(n, topk, H, I, E))
-    with torch.cuda.device(x.device):
+    nbytes = lib().gsb_moe_expert_ffn_w16_workspace_bytes(n, topk, H, I, E)
+    with _device_of(x):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        check(lib().gsb_moe_expert_ffn_w16(_p(x), _p(topk_ids), _p(topk_w), _p(gate_w), _p(up_w), _p(down_w),
-                                           _TYPE[x.dtype], n, topk, H, I, E, _p(out), _TYPE[out.dtype], _p(ws),
-                                           C.c_size_t(nbytes), _stream()), "moe_expert_ffn_w16")
+        check(lib().gsb_moe_expert_ffn_w16(x.data_ptr(), topk_ids.data_ptr(), topk_w.data_ptr(), gate_w.data_ptr(),
+                                           up_w.data_ptr(), down_w.data_ptr(), _TYPE[x.dtype], n, topk, H, I, E,
+                                           out.data_ptr(), _TYPE[out.dtype], ws.data_ptr(), nbytes, _raw_stream(x)),
+              "moe_expert_ffn_w16")
     return out
 
 
@@ -176,10 +191,10 @@ def lora_add(y, x, A, B, adapter_offsets, rows, ranks=None, scales=None):
     (columns of B and rows of A behind an adapter's rank are not used), scales float32 [nA].  The lists come from
     ``moe_dispatch(adapter_ids[:, None], nA)``, once per batch: offsets and sorted_token_ids; an id of -1 = no
     adapter.  ``rows`` may be longer than the segments: what lies behind the last one is ignored."""
-    _need16(x, (A, None, 3, "A"), (B, None, 3, "B"), (adapter_offsets, torch.int32, 1, "adapter_offsets"),
+    _need16(x, (A, x.dtype, 3, "A"), (B, x.dtype, 3, "B"), (adapter_offsets, torch.int32, 1, "adapter_offsets"),
             (rows, torch.int32, 1, "rows"), (ranks, torch.int32, 1, "ranks"), (scales, torch.float32, 1, "scales"))
     n, K = x.shape
-    nA, R = A.shape[:2]
+    nA, R, _ = A.shape
     N = B.shape[1]
     if A.shape != (nA, R, K) or B.shape != (nA, N, R) or adapter_offsets.shape[0] != nA + 1 or \
             (ranks is not None and ranks.shape[0] != nA) or (scales is not None and scales.shape[0] != nA):
@@ -188,12 +203,13 @@ def lora_add(y, x, A, B, adapter_offsets, rows, ranks=None, scales=None):
     if y is None:
         raise ValueError("y: expected the projection's result")
     _out16(y, (n, N), x, None, "y")
-    nbytes = int(lib().gsb_lora_scratch_bytes(P, R, nA))
-    with torch.cuda.device(x.device):
+    nbytes = lib().gsb_lora_scratch_bytes(P, R, nA)
+    with _device_of(x):
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        check(lib().gsb_lora_add(_p(x), _p(A), _p(B), _TYPE[x.dtype], _p(adapter_offsets), _p(rows), _p(ranks),
-                                 _p(scales), n, P, K, N, nA, R, _p(y), _TYPE[y.dtype], _p(scratch),
-                                 C.c_size_t(nbytes), _stream()), "lora_add")
+        check(lib().gsb_lora_add(x.data_ptr(), A.data_ptr(), B.data_ptr(), _TYPE[x.dtype], adapter_offsets.data_ptr(),
+                                 rows.data_ptr(), None if ranks is None else ranks.data_ptr(),
+                                 None if scales is None else scales.data_ptr(), n, P, K, N, nA, R, y.data_ptr(),
+                                 _TYPE[y.dtype], scratch.data_ptr(), nbytes, _raw_stream(x)), "lora_add")
     return y
 
 
