@@ -56,23 +56,16 @@ template <> __device__ __forceinline__ void mma_k16<__half>(float (&d)[4], uint3
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_tf32(float (&d)[4], float a0, float a1, float a2, float a3, float b0, float b1) {
-    asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-                 : "r"(__float_as_uint(a0)), "r"(__float_as_uint(a1)), "r"(__float_as_uint(a2)), "r"(__float_as_uint(a3)),
-                   "r"(__float_as_uint(b0)), "r"(__float_as_uint(b1)));
-}
-
 // ---- first launch: v ---------------------------------------------------------------------------
 // Block: up to 8 * NTK rows of one adapter x 16 * MT ranks, D[rank, row]; its eight warps and a.S blocks share the sum
 // over K (adjacent 32-column chunks go to adjacent warps).  The warps' tiles are added in shared memory in warp order,
 // the blocks' parts by the second launch in block order.
-template <typename T, int MT, int NTK>
+template <typename T, int MT>
 __global__ void __launch_bounds__(kShWarps * 32)
 lora_shrink_kernel(const LoraArgs a) {
     extern __shared__ float s_red[];                  // [warps][16 * MT ranks][8 * NTK rows]
     __shared__ int pre[kMaxE + 4], wsum[8];
-    constexpr int RT = 16 * MT, TT = 8 * NTK;
+    constexpr int RT = 16 * MT, TT = 8, NTK = 1;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     int descending = seg_scan<TT>(a.offsets, a.nA, a.P, pre, wsum);
     descending = __syncthreads_or(descending);
@@ -140,40 +133,163 @@ lora_shrink_kernel(const LoraArgs a) {
     }
 }
 
+// The same for adapters with many rows: 64 rows x 16 * MT ranks, D[row, rank], over K steps of 64 columns that 16-byte
+// asynchronous copies bring into a ring in shared memory (rows of 128 bytes, 16-byte piece c of row q at c ^ q % 8), so
+// that 48 KB a block stay in flight without a register: the direct kernel above, at 32 rows x 64 ranks a block, has room
+// for one step and measured 91 us for 8192 rows of 6144 at rank 64, this one WIDE_US.  Warps: four groups of 16 rows x two
+// halves of each K step.
+constexpr int kWdRows = 64, kWdStages = 4;
+template <int MT> constexpr int wd_stage_bytes() { return (kWdRows + 16 * MT) * 128; }
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+
+template <typename T, int MT>
+__global__ void __launch_bounds__(256, 2)
+lora_shrink_wide_kernel(const LoraArgs a) {
+    extern __shared__ __align__(128) uint8_t s_ring[];
+    __shared__ int pre[kMaxE + 4], wsum[8];
+    constexpr int RT = 16 * MT, SB = wd_stage_bytes<MT>();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    int descending = seg_scan<kWdRows>(a.offsets, a.nA, a.P, pre, wsum);
+    descending = __syncthreads_or(descending);
+    const LoraTile tile = lora_tile<kWdRows>(a, pre, blockIdx.x, descending);
+    if (tile.ad < 0) return;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int r0 = blockIdx.z * RT, rank = rank_of(a, tile.ad);
+    if (r0 >= rank) return;
+    const int steps = (a.K + 63) / 64, k_lo = steps * (int)blockIdx.y / a.S, k_hi = steps * ((int)blockIdx.y + 1) / a.S;
+    // copies: thread = 16-byte piece tid % 8 of rows tid / 8 + 32 i
+    const int piece = tid & 7, q0 = tid >> 3;
+    const T* xs[2];
+    bool xin[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int c = q0 + 32 * i, row = c < tile.cnt ? __ldg(a.rows + tile.p0 + c) : -1;
+        xin[i] = row >= 0 && row < a.n;
+        xs[i] = reinterpret_cast<const T*>(a.x) + (int64_t)(xin[i] ? row : 0) * a.K + piece * 8;
+    }
+    const T* A = reinterpret_cast<const T*>(a.A) + ((int64_t)tile.ad * a.R + r0) * a.K + piece * 8;
+    const uint32_t ring = smem_u32(s_ring), sw = (uint32_t)((piece ^ (q0 & 7)) << 4);
+    auto copy = [&](int step) {
+        if (step < k_hi) {
+            const uint32_t base = ring + (uint32_t)((step - k_lo) % kWdStages) * SB;
+            const bool in = step * 64 + piece * 8 < a.K;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                cp16(base + (uint32_t)((q0 + 32 * i) * 128) + sw, in && xin[i] ? xs[i] + step * 64 : xs[i], in && xin[i]);
+#pragma unroll
+            for (int i = 0; i < (RT + 31) / 32; ++i) {
+                const int r = q0 + 32 * i;
+                const bool have = in && r < RT && r0 + r < rank;    // what lies behind the adapter's rank counts as zero
+                if (r < RT) cp16(base + (uint32_t)((kWdRows + r) * 128) + sw, have ? A + (int64_t)r * a.K + step * 64 : A, have);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int i = 0; i < kWdStages - 1; ++i) copy(k_lo + i);
+    const int wr = (warp & 3) * 16, wk = warp >> 2;        // this warp's rows, and its half of the step
+    float acc[2 * MT][4] = {};
+    for (int step = k_lo; step < k_hi; ++step) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kWdStages - 2) : "memory");
+        __syncthreads();                                   // the step is there, and the stage copied into next is free
+        copy(step + kWdStages - 1);
+        const uint32_t base = ring + (uint32_t)((step - k_lo) % kWdStages) * SB;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+            const int c0 = wk * 4 + kk * 2;                // first 16-byte piece of these 16 columns
+            uint32_t fx[4], fa[4];
+            const int xr = wr + (lane & 15);
+            ldsm4(base + (uint32_t)(xr * 128 + (((c0 + (lane >> 4)) ^ (xr & 7)) << 4)), fx);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                // ranks m * 16 + 0..7 in fa[0], fa[1], ranks m * 16 + 8..15 in fa[2], fa[3]
+                const int ar = m * 16 + (lane & 7) + ((lane >> 4) << 3);
+                ldsm4(base + (uint32_t)((kWdRows + ar) * 128 + (((c0 + ((lane >> 3) & 1)) ^ (ar & 7)) << 4)), fa);
+                mma_k16<T>(acc[2 * m], fx[0], fx[1], fx[2], fx[3], fa[0], fa[1]);
+                mma_k16<T>(acc[2 * m + 1], fx[0], fx[1], fx[2], fx[3], fa[2], fa[3]);
+            }
+        }
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    // the second half's sums are added to the first's
+    float* red = reinterpret_cast<float*>(s_ring);
+    const int g = lane >> 2, t = lane & 3;
+    if (wk == 1)
+#pragma unroll
+        for (int j = 0; j < 2 * MT; ++j)
+#pragma unroll
+            for (int h = 0; h < 4; ++h) red[((warp & 3) * 8 * MT + j * 4 + h) * 32 + lane] = acc[j][h];
+    __syncthreads();
+    if (wk == 0)
+#pragma unroll
+        for (int j = 0; j < 2 * MT; ++j)
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+                const int c = wr + (h >> 1) * 8 + g, r = r0 + j * 8 + t * 2 + (h & 1);
+                if (c < tile.cnt && r < rank)
+                    a.part[((int64_t)blockIdx.y * a.P + tile.p0 + c) * a.R + r] = acc[j][h] + red[(warp * 8 * MT + j * 4 + h) * 32 + lane];
+            }
+}
+
 // ---- second launch: y += B v ---------------------------------------------------------------------
-// Block: up to 16 * MT rows of one adapter x a range of features, 32 features a warp at a time, D[row, feature].  v is
-// applied as the sum of two tf32 numbers (together 22 bits of it; B's 16-bit values are exact in tf32), so y's fp32 sums
-// keep fp32 accuracy.  n-tile j of a warp's chunk holds features 8 (c / 2) + 2 j + c % 2 in its columns c: lane t of a quad
-// then owns eight contiguous features of a row.
+// Block: up to 16 * MT rows of one adapter x a range of features, 32 features a warp at a time, D[row, feature].
+// v enters the 16-bit tensor cores as a sum of 16-bit numbers, so that y's fp32 sums keep (nearly) fp32 accuracy: three
+// bf16 numbers hold all 24 bits; two fp16 numbers hold 22, with each row of v scaled by a power of two to a largest
+// value in [2^14, 2^15) so that neither overflows or loses bits below fp16's normal range.  (tf32 would do it in two
+// for both types, but mma.sync runs tf32 at the rate of plain fp32 multiply-adds here: 192 us instead of EXP_US for 8192
+// rows of 6144 at rank 64.)  n-tile j of a warp's chunk holds features 8 (c / 2) + 2 j + c % 2 in its columns c: lane t
+// of a quad then owns eight contiguous features of a row.
 template <typename T> __device__ __forceinline__ float2 pair_f(uint32_t v);
 template <> __device__ __forceinline__ float2 pair_f<__nv_bfloat16>(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
 template <> __device__ __forceinline__ float2 pair_f<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
 
-__device__ __forceinline__ float tf32_of(float v) {
-    uint32_t r;
-    asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(r) : "f"(v));
-    return __uint_as_float(r);
+template <typename T> struct Split;      // v as the sum of N numbers of type T
+template <> struct Split<__nv_bfloat16> { static constexpr int N = 3; static constexpr bool scaled = false; };
+template <> struct Split<__half> { static constexpr int N = 2; static constexpr bool scaled = true; };
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(T a, T b) {
+    const unsigned short x = *reinterpret_cast<const unsigned short*>(&a), y = *reinterpret_cast<const unsigned short*>(&b);
+    return (uint32_t)x | ((uint32_t)y << 16);
 }
 
+// eight values of y as they lie in memory
+template <typename Y> struct Raw8 { uint4 q[sizeof(Y) / 2]; };
 template <typename Y>
-__device__ __forceinline__ void load8(const Y* p, int have, bool vec, float (&v)[8]) {
+__device__ __forceinline__ Raw8<Y> load8(const Y* p, int have, bool vec) {
+    Raw8<Y> v;
     if (vec && have == 8) {
-        if constexpr (sizeof(Y) == 4) {
-            const float4 q0 = *reinterpret_cast<const float4*>(p), q1 = *(reinterpret_cast<const float4*>(p) + 1);
-            v[0] = q0.x; v[1] = q0.y; v[2] = q0.z; v[3] = q0.w; v[4] = q1.x; v[5] = q1.y; v[6] = q1.z; v[7] = q1.w;
-        } else {
-            const uint4 q = *reinterpret_cast<const uint4*>(p);
-            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { const float2 f = pair_f<Y>(w[i]); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
+        for (int i = 0; i < (int)sizeof(Y) / 2; ++i) v.q[i] = *(reinterpret_cast<const uint4*>(p) + i);
+    } else {
+        uint32_t w[sizeof(Y) * 2];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if constexpr (sizeof(Y) == 4) w[i] = i < have ? __float_as_uint(p[i]) : 0u;
+            else {
+                const uint32_t h = i < have ? (uint32_t)reinterpret_cast<const unsigned short*>(p)[i] : 0u;
+                if (i & 1) w[i >> 1] |= h << 16; else w[i >> 1] = h;
+            }
         }
-        return;
-    }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < have ? to_f(p[i]) : 0.f;
+        for (int i = 0; i < (int)sizeof(Y) / 2; ++i) v.q[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    }
+    return v;
 }
 template <typename Y>
-__device__ __forceinline__ void store8(Y* p, int have, bool vec, const float (&v)[8]) {
+__device__ __forceinline__ void add_store8(Y* p, int have, bool vec, const Raw8<Y>& raw, const float (&d)[8]) {
+    float v[8];
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (sizeof(Y) == 4) v[i] = __uint_as_float(w[i]) + d[i];
+        else { const float2 f = pair_f<Y>(w[i >> 1]); v[i] = (i & 1 ? f.y : f.x) + d[i]; }
+    }
     if (vec && have == 8) {
         if constexpr (sizeof(Y) == 4) {
             *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
@@ -191,11 +307,14 @@ __device__ __forceinline__ void store8(Y* p, int have, bool vec, const float (&v
         if (i < have) p[i] = from_f<Y>(v[i]);
 }
 
-template <typename T, typename Y, int MT>
-__global__ void __launch_bounds__(256)
+// KG = 1: at most 16 ranks, whose B values are loaded ahead together with y (0: any number of ranks, B loaded in turn).
+template <typename T, typename Y, int MT, int KG>
+__global__ void __launch_bounds__(256, MT == 1 && KG == 1 ? 3 : 2)
 lora_expand_kernel(const LoraArgs a, int feats, int vec_b, int vec_y) {
-    extern __shared__ float4 s_v[];                   // [row tile of 16][16 ranks][hi g, hi g + 8, lo g, lo g + 8][lane]
-    __shared__ int pre[kMaxE + 4], wsum[8], srow[16 * MT];
+    constexpr int NS = Split<T>::N;
+    extern __shared__ uint4 s_v[];                    // [row tile of 16][16 ranks][part][lane]: A fragments
+    __shared__ int pre[kMaxE + 4], wsum[8];
+    __shared__ float s_scale[16 * MT];                // what a row's sums are multiplied by at the end
     int descending = seg_scan<16 * MT>(a.offsets, a.nA, a.P, pre, wsum);
     descending = __syncthreads_or(descending);
     const LoraTile tile = lora_tile<16 * MT>(a, pre, blockIdx.x, descending);
@@ -203,121 +322,165 @@ lora_expand_kernel(const LoraArgs a, int feats, int vec_b, int vec_y) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int rank = rank_of(a, tile.ad), kgs = (rank + 15) / 16;
     if (rank == 0) return;
-    if (threadIdx.x < 16 * MT) {
-        const int r = (int)threadIdx.x < tile.cnt ? __ldg(a.rows + tile.p0 + threadIdx.x) : -1;
-        srow[threadIdx.x] = r >= 0 && r < a.n ? r : -1;
+    int row[2 * MT];
+#pragma unroll
+    for (int m = 0; m < 2 * MT; ++m) {
+        const int c = m * 8 + g, r = c < tile.cnt ? __ldg(a.rows + tile.p0 + c) : -1;
+        row[m] = r < a.n ? r : -1;
     }
     const float sc = a.scales ? __ldg(a.scales + tile.ad) : 1.f;
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // v comes from the first launch
-    for (int i = threadIdx.x; i < MT * kgs * 64; i += 256) {
-        // (row tile, group of 16 ranks, half of the 16 rows, lane): four ranks of one row
-        const int l = i & 31, h = (i >> 5) & 1, kg = (i >> 6) % kgs, m = (i >> 6) / kgs;
-        const int c = m * 16 + h * 8 + (l >> 2), r = kg * 16 + (l & 3) * 4;
-        float v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float s = 0.f;
-            if (c < tile.cnt && r + j < rank)
-                for (int q = 0; q < a.S; ++q) s += a.part[((int64_t)q * a.P + tile.p0 + c) * a.R + r + j];
-            v[j] = sc * s;
-        }
-        float4* d = s_v + (int64_t)((m * kgs + kg) * 4) * 32 + l;
-        float4 hi = make_float4(tf32_of(v[0]), tf32_of(v[1]), tf32_of(v[2]), tf32_of(v[3]));
-        // what tf32 cannot hold of v; an infinite or NaN v has no rest
-        float4 lo = make_float4(v[0] - hi.x, v[1] - hi.y, v[2] - hi.z, v[3] - hi.w);
-        d[h * 32] = hi;
-        d[(2 + h) * 32] = make_float4(isfinite(v[0]) ? tf32_of(lo.x) : 0.f, isfinite(v[1]) ? tf32_of(lo.y) : 0.f,
-                                      isfinite(v[2]) ? tf32_of(lo.z) : 0.f, isfinite(v[3]) ? tf32_of(lo.w) : 0.f);
-    }
-    __syncthreads();
     const T* B = reinterpret_cast<const T*>(a.B) + (int64_t)tile.ad * a.N * a.R;
     Y* y = reinterpret_cast<Y*>(a.y);
-    const int f_end = min(a.N, (int)(blockIdx.y + 1) * feats), mts = (tile.cnt + 15) / 16;
-    for (int f0 = blockIdx.y * feats + warp * 32; f0 < f_end; f0 += 256) {
+    const int f_end = min(a.N, (int)(blockIdx.y + 1) * feats);
+
+    // four ranks of feature n of n-tile j, as two packed pairs
+    auto load_b = [&](int f0, int kg, int j) {
+        const int f = f0 + 8 * (g >> 1) + 2 * j + (g & 1), r = kg * 16 + t * 4;
+        uint2 w = make_uint2(0, 0);
+        if (f < a.N) {
+            const T* br = B + (int64_t)f * a.R + r;
+            if (vec_b && r + 4 <= rank) w = __ldg(reinterpret_cast<const uint2*>(br));
+            else {
+                const unsigned short* bs = reinterpret_cast<const unsigned short*>(br);
+                if (r < rank) w.x = bs[0];
+                if (r + 1 < rank) w.x |= (uint32_t)bs[1] << 16;
+                if (r + 2 < rank) w.y = bs[2];
+                if (r + 3 < rank) w.y |= (uint32_t)bs[3] << 16;
+            }
+        }
+        return w;
+    };
+    struct Ahead { Raw8<Y> y[2 * MT]; uint2 b[KG ? KG : 1][4]; };
+    auto load = [&](Ahead& q, int f0) {
+        if (f0 >= f_end) return;
+#pragma unroll
+        for (int kg = 0; kg < KG; ++kg)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) q.b[kg][j] = kg < kgs ? load_b(f0, kg, j) : make_uint2(0, 0);
+        const int f = f0 + 8 * t;
+#pragma unroll
+        for (int m = 0; m < 2 * MT; ++m)
+            if (row[m] >= 0 && f < a.N) q.y[m] = load8(y + (int64_t)row[m] * a.N + f, min(8, a.N - f), vec_y);
+    };
+    auto finish = [&](const Ahead& q, int f0) {
         float acc[MT][4][4] = {};
-        for (int kg = 0; kg < kgs; ++kg) {
-            const int r = kg * 16 + t * 4;
-            float2 b[4][2];
+        for (int kg = 0; kg < (KG ? KG : kgs); ++kg) {
+            if (kg >= kgs) break;
+            uint2 b[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[j] = KG ? q.b[kg][j] : load_b(f0, kg, j);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int u = NS - 1; u >= 0; --u) {    // small parts first
+                    const uint4 v = s_v[((m * kgs + kg) * NS + u) * 32 + lane];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) mma_k16<T>(acc[m][j], v.x, v.y, v.z, v.w, b[j].x, b[j].y);
+                }
+        }
+        const int f = f0 + 8 * t, have = min(8, a.N - f);
+#pragma unroll
+        for (int m = 0; m < 2 * MT; ++m) {
+            if (row[m] < 0 || have <= 0) continue;
+            float d[8];
+            const float back = Split<T>::scaled ? s_scale[m * 8 + g] : 1.f;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const int f = f0 + 8 * (g >> 1) + 2 * j + (g & 1);
-                uint32_t w0 = 0, w1 = 0;
-                if (f < a.N) {
-                    const T* br = B + (int64_t)f * a.R + r;
-                    if (vec_b && r + 4 <= rank) {
-                        const uint2 q = __ldg(reinterpret_cast<const uint2*>(br));
-                        w0 = q.x; w1 = q.y;
-                    } else {
-                        const unsigned short* bs = reinterpret_cast<const unsigned short*>(br);
-                        if (r < rank) w0 = bs[0];
-                        if (r + 1 < rank) w0 |= (uint32_t)bs[1] << 16;
-                        if (r + 2 < rank) w1 = bs[2];
-                        if (r + 3 < rank) w1 |= (uint32_t)bs[3] << 16;
-                    }
-                }
-                b[j][0] = pair_f<T>(w0);
-                b[j][1] = pair_f<T>(w1);
+                d[2 * j] = back * acc[m >> 1][j][2 * (m & 1)];
+                d[2 * j + 1] = back * acc[m >> 1][j][2 * (m & 1) + 1];
             }
+            add_store8(y + (int64_t)row[m] * a.N + f, have, vec_y, q.y[m], d);
+        }
+    };
+
+    int f0 = blockIdx.y * feats + warp * 32;
+    Ahead q0;
+    load(q0, f0);                                        // B and y do not wait for the first launch
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // v comes from it
+    // v of this tile: eight lanes a row, each every eighth run of two ranks
+    {
+        const int c = threadIdx.x >> 3, l8 = threadIdx.x & 7;
+        for (int c0 = 0; c0 < 16 * MT; c0 += 32) {
+            const int cr = c0 + c;
+            const bool live = cr < 16 * MT;
+            auto value = [&](int r) {
+                float s = 0.f;
+                if (live && cr < tile.cnt && r < rank)
+                    for (int q = 0; q < a.S; ++q) s += __ldcg(a.part + ((int64_t)q * a.P + tile.p0 + cr) * a.R + r);
+                return sc * s;
+            };
+            float up = 1.f;
+            if (Split<T>::scaled) {
+                float top = 0.f;
+                for (int r = l8 * 2; r < kgs * 16; r += 16) top = fmaxf(top, fmaxf(fabsf(value(r)), fabsf(value(r + 1))));
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                if (m >= mts) break;
-                const float4* d = s_v + (m * kgs + kg) * 128 + lane;
-                const float4 h0 = d[0], h1 = d[32], l0 = d[64], l1 = d[96];
+                for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                // 2^(14 - exponent), kept where both it and its inverse are normal; 1 for rows of zeros or infinities
+                int ex = 14 - ((int)((__float_as_uint(top) >> 23) & 0xff) - 127);
+                ex = top > 0.f && top < __int_as_float(0x7f800000) ? min(max(ex, -126), 126) : 0;
+                up = __int_as_float((ex + 127) << 23);
+                if (live && l8 == 0) s_scale[cr] = __int_as_float((127 - ex) << 23);
+            }
+            for (int r = l8 * 2; r < kgs * 16; r += 16) {
+                float v0 = up * value(r), v1 = up * value(r + 1);
+                if (!live) break;
+                // ranks 4 t' .. 4 t' + 3 of a group are lane t' of the quad: two in the first, two in the last register pair
+                const int kg = r >> 4, tq = (r >> 2) & 3, hi_pair = (r >> 1) & 1;
+                uint32_t* d = reinterpret_cast<uint32_t*>(s_v + (((cr >> 4) * kgs + kg) * NS) * 32 + (cr & 7) * 4 + tq) +
+                              hi_pair * 2 + ((cr >> 3) & 1);
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    mma_tf32(acc[m][j], l0.x, l1.x, l0.y, l1.y, b[j][0].x, b[j][0].y);
-                    mma_tf32(acc[m][j], l0.z, l1.z, l0.w, l1.w, b[j][1].x, b[j][1].y);
-                    mma_tf32(acc[m][j], h0.x, h1.x, h0.y, h1.y, b[j][0].x, b[j][0].y);
-                    mma_tf32(acc[m][j], h0.z, h1.z, h0.w, h1.w, b[j][1].x, b[j][1].y);
+                for (int u = 0; u < NS; ++u) {
+                    const T p0 = from_f<T>(v0), p1 = from_f<T>(v1);
+                    d[u * 128] = pack2(p0, p1);
+                    // the rest; infinity and NaN have none
+                    v0 = isfinite(v0) ? v0 - to_f(p0) : 0.f;
+                    v1 = isfinite(v1) ? v1 - to_f(p1) : 0.f;
                 }
             }
         }
-        const int f = f0 + 8 * t, have = min(8, a.N - f);
-        if (have <= 0) continue;
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const int row = srow[m * 16 + h * 8 + g];
-                if (row < 0) continue;
-                Y* p = y + (int64_t)row * a.N + f;
-                float v[8];
-                load8(p, have, vec_y, v);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    v[2 * j] += acc[m][j][2 * h];
-                    v[2 * j + 1] += acc[m][j][2 * h + 1];
-                }
-                store8(p, have, vec_y, v);
-            }
+    }
+    __syncthreads();
+    for (; f0 < f_end; f0 += 256) {
+        finish(q0, f0);
+        load(q0, f0 + 256);
     }
 }
 
 // How the first launch is cut: a rule on P and the number of adapters alone, because the scratch is sized by it.
-// Eight-row tiles (the least mma.sync multiplies) while an adapter has few rows, 32-row tiles above (each A is then
-// read once per 32 rows); the sum over K is spread until two blocks per SM have work.
+// Eight-row tiles (the least mma.sync multiplies) while an adapter has few rows, 64-row tiles above; the sum over K is
+// spread until two blocks per SM have work.
 inline bool lora_wide(int P, int nA) { return P > 8 * (int64_t)nA; }
 inline int lora_split(int P, int nA) {
-    const int64_t tiles = (nA < P ? nA : P) + P / (lora_wide(P, nA) ? 32 : 8);
+    const int64_t tiles = (nA < P ? nA : P) + P / (lora_wide(P, nA) ? kWdRows : 8);
     const int64_t s = 296 / tiles;
     return s < 1 ? 1 : s > 8 ? 8 : (int)s;
 }
 
-template <typename T, int MT, int NTK>
-int run_shrink(const LoraArgs& a, cudaStream_t s) {
-    constexpr size_t smem = (size_t)kShWarps * 16 * MT * 8 * NTK * 4;
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(lora_shrink_kernel<T, MT, NTK>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+template <typename T, int MT>
+int run_shrink_wide(const LoraArgs& a, cudaStream_t s) {
+    constexpr size_t smem = (size_t)kWdStages * wd_stage_bytes<MT>();
+    if (smem > 40 * 1024 && cudaFuncSetAttribute(lora_shrink_wide_kernel<T, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return GSB_ERR_CUDA;
-    const int tiles = (a.nA < a.P ? a.nA : a.P) + a.P / (8 * NTK);
-    lora_shrink_kernel<T, MT, NTK><<<dim3(tiles, a.S, (a.R + 16 * MT - 1) / (16 * MT)), kShWarps * 32, smem, s>>>(a);
+    const int tiles = (a.nA < a.P ? a.nA : a.P) + a.P / kWdRows;
+    lora_shrink_wide_kernel<T, MT><<<dim3(tiles, a.S, (a.R + 16 * MT - 1) / (16 * MT)), 256, smem, s>>>(a);
     return launch_status();
 }
 
-template <typename T, typename Y, int MT>
+template <typename T, int MT>
+int run_shrink(const LoraArgs& a, cudaStream_t s) {
+    constexpr size_t smem = (size_t)kShWarps * 16 * MT * 8 * 4;
+    if (smem > 40 * 1024 && cudaFuncSetAttribute(lora_shrink_kernel<T, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+        return GSB_ERR_CUDA;
+    const int tiles = (a.nA < a.P ? a.nA : a.P) + a.P / 8;
+    lora_shrink_kernel<T, MT><<<dim3(tiles, a.S, (a.R + 16 * MT - 1) / (16 * MT)), kShWarps * 32, smem, s>>>(a);
+    return launch_status();
+}
+
+template <typename T, typename Y, int MT, int KG>
 int run_expand(const LoraArgs& a, cudaStream_t s) {
-    const size_t smem = (size_t)MT * ((a.R + 15) / 16) * 128 * sizeof(float4);
-    auto kernel = lora_expand_kernel<T, Y, MT>;
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
+    const size_t smem = (size_t)MT * ((a.R + 15) / 16) * Split<T>::N * 32 * sizeof(uint4);
+    auto kernel = lora_expand_kernel<T, Y, MT, KG>;
+    if (smem > 40 * 1024 && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return GSB_ERR_CUDA;
     const int tiles = (a.nA < a.P ? a.nA : a.P) + a.P / (16 * MT);
     // features in ranges of whole passes of the block (256), until about four blocks per SM have work
@@ -339,10 +502,11 @@ template <typename T, typename Y>
 int run_lora(const LoraArgs& a, cudaStream_t s) {
     const bool wide = lora_wide(a.P, a.nA);
     int st;
-    if (wide) st = a.R <= 16 ? run_shrink<T, 1, 4>(a, s) : a.R <= 32 ? run_shrink<T, 2, 4>(a, s) : run_shrink<T, 4, 4>(a, s);
-    else st = a.R <= 16 ? run_shrink<T, 1, 1>(a, s) : a.R <= 32 ? run_shrink<T, 2, 1>(a, s) : run_shrink<T, 4, 1>(a, s);
+    if (wide) st = a.R <= 16 ? run_shrink_wide<T, 1>(a, s) : a.R <= 32 ? run_shrink_wide<T, 2>(a, s) : run_shrink_wide<T, 4>(a, s);
+    else st = a.R <= 16 ? run_shrink<T, 1>(a, s) : a.R <= 32 ? run_shrink<T, 2>(a, s) : run_shrink<T, 4>(a, s);
     if (st) return st;
-    return wide && a.R <= 64 ? run_expand<T, Y, 4>(a, s) : run_expand<T, Y, 1>(a, s);
+    if (wide) return a.R <= 16 ? run_expand<T, Y, 2, 1>(a, s) : run_expand<T, Y, 2, 0>(a, s);
+    return a.R <= 16 ? run_expand<T, Y, 1, 1>(a, s) : run_expand<T, Y, 1, 0>(a, s);
 }
 
 }  // namespace
