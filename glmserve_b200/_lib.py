@@ -63,7 +63,9 @@ def lib():
         L.gsb_prefill_wait_profile.argtypes = [C.c_void_p]
         # argument types given, so that plain integers do as pointers and sizes
         V, I, Z = C.c_void_p, C.c_int, C.c_size_t
-        L.gsb_grouped_gemm.argtypes = [V, V, I, V, V, I, I, I, I, I, V, I, V]
+        L.gsb_grouped_gemm_workspace_bytes.argtypes = [I] * 3
+        L.gsb_grouped_gemm_workspace_bytes.restype = Z
+        L.gsb_grouped_gemm.argtypes = [V, V, I, V, V, I, I, I, I, I, V, I, V, Z, V]
         L.gsb_moe_expert_ffn_w16_workspace_bytes.argtypes = [I] * 5
         L.gsb_moe_expert_ffn_w16_workspace_bytes.restype = Z
         L.gsb_moe_expert_ffn_w16.argtypes = [V] * 6 + [I] * 6 + [V, I, V, Z, V]

@@ -305,8 +305,10 @@ int run_grouped_any(const GroupedArgs& a, int y_type, cudaStream_t s) {
     return y_type == GSB_TYPE_F32 ? run_grouped<T, float, false>(a, s) : run_grouped<T, T, false>(a, s);
 }
 
-int launch_grouped(const GroupedArgs& a, int type, int y_type, cudaStream_t s) {
-    if (a.P / a.E > 64) return launch_grouped_pair(a, type, y_type, s);
+bool use_pair(int P, int E) { return P / E > 64; }
+
+int launch_grouped(const GroupedArgs& a, int type, int y_type, void* scratch, cudaStream_t s) {
+    if (use_pair(a.P, a.E)) return launch_grouped_pair(a, type, y_type, scratch, s);
     return type == GSB_TYPE_BF16 ? run_grouped_any<__nv_bfloat16>(a, y_type, s) : run_grouped_any<__half>(a, y_type, s);
 }
 
@@ -339,7 +341,7 @@ int run_combine16(const float* y, const int* ids, const int* slot_pos, const flo
 }
 
 // Scratch of the FFN; every buffer starts on a 256-byte boundary.
-struct Ffn16Ws { int *offsets, *tok, *row, *slot_pos, *disp; uint8_t* h; float* y; size_t total; };
+struct Ffn16Ws { int *offsets, *tok, *row, *slot_pos, *disp; uint8_t *h, *xs; float* y; size_t total; };
 Ffn16Ws carve16(int n, int topk, int H, int I, int E, void* base) {
     const size_t P = (size_t)n * topk;
     Ffn16Ws ws{};
@@ -352,7 +354,9 @@ Ffn16Ws carve16(int n, int topk, int H, int I, int E, void* base) {
     ws.slot_pos = reinterpret_cast<int*>(take(P * 4));
     ws.disp = reinterpret_cast<int*>(take(dispatch_scratch_bytes(n, topk, E)));
     ws.h = take(P * I * 2);
+    // the rows in expert order are done with when the per-slot rows are written
     ws.y = reinterpret_cast<float*>(take(P * H * 4));
+    ws.xs = reinterpret_cast<uint8_t*>(ws.y);
     ws.total = at;
     return ws;
 }
@@ -367,8 +371,13 @@ constexpr int64_t kMaxSlots = (int64_t)1 << 30;
 
 using namespace gsb;
 
+extern "C" size_t gsb_grouped_gemm_workspace_bytes(int P, int in, int E) {
+    return P > 0 && in > 0 && E > 0 && use_pair(P, E) ? grouped_pair_scratch_bytes(P, in) : 0;
+}
+
 extern "C" int gsb_grouped_gemm(const void* x, const void* w, int type, const int* expert_offsets, const int* rows,
-                                int n, int P, int in, int out, int E, void* y, int y_type, void* stream) {
+                                int n, int P, int in, int out, int E, void* y, int y_type, void* workspace,
+                                size_t workspace_bytes, void* stream) {
     if (!is16(type) || (y_type != type && y_type != GSB_TYPE_F32)) return GSB_ERR_INVALID_ARG;
     if (n < 0 || P < 0 || in <= 0 || out <= 0 || E <= 0 || (!rows && P > n)) return GSB_ERR_INVALID_ARG;
     if (P == 0 || n == 0) return GSB_OK;
@@ -377,10 +386,13 @@ extern "C" int gsb_grouped_gemm(const void* x, const void* w, int type, const in
         misaligned(y, type_bytes(y_type)))
         return GSB_ERR_INVALID_ARG;
     if (in % 8 || E > 1024 || P > kMaxSlots) return GSB_ERR_UNSUPPORTED;
+    const size_t need = rows ? gsb_grouped_gemm_workspace_bytes(P, in, E) : 0;
+    if (need && (!workspace || misaligned(workspace, 256))) return GSB_ERR_INVALID_ARG;
+    if (need > workspace_bytes) return GSB_ERR_WORKSPACE;
     GroupedArgs a{};
     a.x = x; a.w = w; a.offsets = expert_offsets; a.rows = rows;
     a.n = n; a.P = P; a.K = in; a.N = out; a.E = E; a.y = y;
-    return launch_grouped(a, type, y_type, reinterpret_cast<cudaStream_t>(stream));
+    return launch_grouped(a, type, y_type, workspace, reinterpret_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t gsb_moe_expert_ffn_w16_workspace_bytes(int n, int topk, int hidden, int moe_inter, int E) {
@@ -409,12 +421,12 @@ extern "C" int gsb_moe_expert_ffn_w16(const void* x, const int* topk_ids, const 
     GroupedArgs g{};
     g.x = x; g.w = gate_w; g.w2 = up_w; g.offsets = ws.offsets; g.rows = ws.tok;
     g.n = n; g.P = n * topk; g.K = hidden; g.N = moe_inter; g.E = E; g.y = ws.h;
-    st = launch_grouped(g, type, type, s);
+    st = launch_grouped(g, type, type, ws.xs, s);
     if (st) return st;
     GroupedArgs d{};
     d.x = ws.h; d.w = down_w; d.offsets = ws.offsets;
     d.n = d.P = n * topk; d.K = moe_inter; d.N = hidden; d.E = E; d.y = ws.y;
-    st = launch_grouped(d, type, GSB_TYPE_F32, s);
+    st = launch_grouped(d, type, GSB_TYPE_F32, nullptr, s);
     if (st) return st;
     if (out_type == GSB_TYPE_F32) return run_combine16<float>(ws.y, topk_ids, ws.slot_pos, topk_weights, n, topk, hidden, E, out, s);
     if (type == GSB_TYPE_BF16) return run_combine16<__nv_bfloat16>(ws.y, topk_ids, ws.slot_pos, topk_weights, n, topk, hidden, E, out, s);

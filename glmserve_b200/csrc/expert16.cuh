@@ -52,6 +52,8 @@ inline bool encode(CUtensorMap* m, const void* base, bool bf16, uint64_t d0, uin
 // The two kernels; types as in gsb_grouped_gemm (a.w2 given: SwiGLU of two products, y of x's type).
 int launch_grouped_split(const GroupedArgs& a, int type, int y_type, cudaStream_t s);
 int take_pair_status();      // status word of the pair kernel, cleared
-int launch_grouped_pair(const GroupedArgs& a, int type, int y_type, cudaStream_t s);
+// scratch (16-byte aligned, grouped_pair_scratch_bytes): a copy of the rows in expert order, used when a.rows is given
+size_t grouped_pair_scratch_bytes(int P, int K);
+int launch_grouped_pair(const GroupedArgs& a, int type, int y_type, void* scratch, cudaStream_t s);
 
 }  // namespace gsb

@@ -4,12 +4,14 @@
 // rows of one expert.  Each CTA stages its own 128 weight rows and half of the tokens; the tensor cores of both read
 // both halves, so a byte of shared memory feeds twice the products of a one-CTA tile - with a 128 x 256 tile per CTA the
 // operand reads plus the writes of the copies need 1.5 times the shared-memory bandwidth of an SM.
-// Weights come by TMA.  Token rows come by TMA as well when they lie in order (the down product); through a row list
-// eight warps gather them with 16-byte cp.async, writing the swizzled tile themselves: TMA's gather takes ~70 cycles per
-// four rows, 4.5 times the 512 cycles a 64-column k-block of this tile multiplies for (250 TFLOP/s with it), and a
-// sorted copy of the rows would cost an extra pass over them.
+// Both operands come by TMA, so the token rows lie in expert order: rows named by a list are copied into that order
+// first (one pass, GATHER_US for 16384 rows of 2048).  Gathering inside this kernel was slower: TMA's gather takes ~70
+// cycles per four rows, 4.5 times the 512 cycles a 64-column k-block multiplies for (250 TFLOP/s), and eight warps with
+// 16-byte cp.async deliver ~16 bytes a cycle where 32 are needed (1008 TFLOP/s against 1233 with rows in order).
 // SwiGLU: a CTA's 128 weight rows are 64 gate rows and their 64 up rows; the epilogue warps swap halves through shared
-// memory.  Two accumulators (2 x 256 TMEM columns), so the epilogue of a tile runs under the next one's main loop.
+// memory.  Two accumulators (2 x 256 TMEM columns), so the epilogue of a tile runs under the next one's main loop.  A
+// TMEM lane holds one feature of 32 tokens where memory wants a token's features side by side: 16-bit results are turned
+// round in shared memory and stored 16 bytes a lane (2-byte stores took as long as the main loop of K = 2048).
 #include "expert16.cuh"
 
 namespace gsb {
@@ -21,8 +23,9 @@ constexpr int kPrStages = 6;
 constexpr int kPrHalf = 128 * 128;         // 128 rows x 64 columns: weights, or this CTA's tokens
 constexpr int kPrStageBytes = 2 * kPrHalf;
 constexpr int kPrXch = 2 * 2 * 16 * 64 * 4; // two buffers of 2 x 16 columns x 64 rows fp32
-constexpr int kPrThreads = 512;            // warps: 0 weights, 1 MMA, 2 TMEM, 3 tokens (TMA), 4-7 epilogue, 8-15 gather
-constexpr size_t kPrSmem = (size_t)kPrStages * kPrStageBytes + kPrXch + (kMaxE + 4) * 4 + 256;
+constexpr int kPrTurn = 4 * 32 * 32 * 2;   // per epilogue warp: 32 tokens x 32 features, 16-bit
+constexpr int kPrThreads = 256;            // warps: 0 weights, 1 MMA, 2 TMEM, 3 tokens, 4-7 epilogue
+constexpr size_t kPrSmem = (size_t)kPrStages * kPrStageBytes + kPrXch + kPrTurn + (kMaxE + 4) * 4 + 256;
 static_assert(kPrSmem <= 227 * 1024, "stages exceed the shared memory of an SM");
 
 __device__ int g_pair_status;
@@ -49,14 +52,15 @@ __device__ __forceinline__ GrItem pr_item(const GroupedArgs& a, const int* pre, 
     return it;
 }
 
-template <typename T, typename Y, bool GU, bool GATHER>
+template <typename T, typename Y, bool GU>
 __global__ void __launch_bounds__(kPrThreads, 1)
 grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_w2,
-                    const __grid_constant__ CUtensorMap tm_x) {
+                    const __grid_constant__ CUtensorMap tm_x, int vec) {
     constexpr int FW = GU ? 128 : 256;     // output features of an item (both CTAs)
     extern __shared__ __align__(1024) uint8_t smem[];
     float* s_xch = reinterpret_cast<float*>(smem + kPrStages * kPrStageBytes);
-    int* pre = reinterpret_cast<int*>(smem + kPrStages * kPrStageBytes + kPrXch);
+    uint8_t* s_turn = smem + kPrStages * kPrStageBytes + kPrXch;
+    int* pre = reinterpret_cast<int*>(s_turn + kPrTurn);
     uint64_t* full = reinterpret_cast<uint64_t*>(pre + kMaxE + 4);     // the leader's are used, for both CTAs' data
     uint64_t* empty = full + kPrStages;
     uint64_t* acc_full = empty + kPrStages;
@@ -68,7 +72,7 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
     const int rank = (int)tc5::cluster_rank();
     if (tid == 0) {
         for (int i = 0; i < kPrStages; ++i) {
-            mbar_init(&full[i], GATHER ? 1 + 2 * 2 : 1);   // the weights' byte count, and two gather warps of each CTA
+            mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 2 * 4); }
@@ -100,7 +104,7 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
                 const int nb = ((it.cnt + 31) / 32 * 16 + 31) / 32;     // token boxes of 32 rows per CTA
                 for (int kb = 0; kb < nkb; ++kb) {
                     if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { pr_timeout(abort_flag); dead = true; break; }
-                    if (rank == 0) mbar_arrive_expect_tx(&full[st], 2u * (kPrHalf + (GATHER ? 0u : (uint32_t)nb * 4096u)));
+                    if (rank == 0) mbar_arrive_expect_tx(&full[st], 2u * (kPrHalf + (uint32_t)nb * 4096u));
                     const uint32_t bar = tc5::map_rank(smem_u32(&full[st]), 0);
                     uint8_t* dst = smem + st * kPrStageBytes;
                     tc5::tma2_load_3d(dst, &tm_w, kb * 64, it.f0 + fr, it.e, bar);
@@ -122,7 +126,7 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
                 }
         }
     } else if (warp == 3) {
-        if (!GATHER && lane == 0) {        // ---- this CTA's half of the token rows, in order
+        if (lane == 0) {                   // ---- this CTA's half of the token rows
             uint32_t st = 0, ph = 0;
             int e = 0;
             bool dead = false;
@@ -137,50 +141,6 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
                     if (++st == kPrStages) { st = 0; ph ^= 1u; }
                 }
             }
-        }
-    } else if (warp >= 8) {
-        if (GATHER) {                      // ---- this CTA's half of the token rows, through the list
-            // Two warps a k-block (64 rows each; eight lanes copy the 128 bytes of a row, four rows an instruction), four
-            // such groups in turn: a group waits for its own copies and fences them before it hands the k-block over, so
-            // what hides that latency is the other three groups' copies.
-            const int group = (warp - 8) >> 1, sub = (warp - 8) & 1, chunk = lane & 7;
-            const T* x = reinterpret_cast<const T*>(a.x) + chunk * 8;
-            uint32_t st = 0, ph = 0, cnt = 0;
-            int e = 0;
-            bool dead = false;
-            for (int i = first; i < items && !dead && !*abort_flag; i += step) {
-                const GrItem it = pr_item<FW>(a, pre, i, FB, e);
-                const int half = (it.cnt + 31) / 32 * 16;
-                int r[16];
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int p = rank * half + sub * 64 + j * 4 + (lane >> 3);
-                    // tokens behind the tile's last, and rows that do not exist, read row 0; neither is stored
-                    r[j] = p < it.cnt ? __ldg(a.rows + it.p0 + p) : 0;
-                    if (r[j] < 0 || r[j] >= a.n) r[j] = 0;
-                }
-                const int nj = max(0, (half - sub * 64 + 3) / 4);          // half is a multiple of 16
-                for (int kb = 0; kb < nkb; ++kb, ++cnt) {
-                    if ((int)(cnt & 3u) == group) {
-                        if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { pr_timeout(abort_flag); dead = true; break; }
-                        const uint32_t base = smem_u32(smem) + st * kPrStageBytes + kPrHalf + (uint32_t)((sub * 64 + (lane >> 3)) * 128);
-                        const bool in = kb * 64 + chunk * 8 < a.K;
-                        const T* xk = in ? x + kb * 64 : x;
-#pragma unroll
-                        for (int j = 0; j < 16; ++j)
-                            if (j < nj)     // 128-byte swizzle: 16-byte piece c of row q lies at c ^ (q % 8); sub * 64 is a multiple of 8
-                                tc5::cp_async16(base + (uint32_t)(j * 512 + ((chunk ^ ((j * 4 + (lane >> 3)) & 7)) << 4)), xk + (int64_t)r[j] * a.K, in);
-                        tc5::cp_async_commit();
-                        tc5::cp_async_wait<0>();
-                        fence_proxy_async();
-                        __syncwarp();
-                        if (lane == 0) tc5::arrive_cluster(tc5::map_rank(smem_u32(&full[st]), 0));
-                    }
-                    if (++st == kPrStages) { st = 0; ph ^= 1u; }
-                }
-                dead = __any_sync(0xffffffffu, dead);
-            }
-            tc5::cp_async_wait<0>();
         }
     } else if (warp == 1) {
         if (rank == 0 && lane == 0) {      // ---- MMA issue for the pair
@@ -236,30 +196,49 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
                 tc5::tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + buf * kPrNT + (uint32_t)c0, v);
                 // which of the 32 tokens exist
                 int r = c0 + lane < it.cnt ? 0 : -1;
-                if (GATHER && r == 0) r = __ldg(a.rows + it.p0 + c0 + lane);
-                const uint32_t live = __ballot_sync(0xffffffffu, r >= 0 && (!GATHER || r < a.n));
+                if (a.rows && r == 0) r = __ldg(a.rows + it.p0 + c0 + lane);
+                const uint32_t live = __ballot_sync(0xffffffffu, r >= 0 && r < a.n);
                 tc5::tmem_ld_wait();
                 Y* o = y + (int64_t)(it.p0 + c0) * a.N + f;
+                Y* turn = reinterpret_cast<Y*>(s_turn + q * 2048);
+                constexpr int NC = GU ? 16 : 32;       // columns this thread finishes, from column cb on
+                const int cb = GU && q >= 2 ? 16 : 0;
+                float d[NC];
                 if (GU) {
                     // warps 0, 1 hold gate rows, 2, 3 the up rows of the same features: each side keeps 16 of the
                     // 32 columns and passes the other 16 on
                     float* xs = s_xch + xb * 2048 + (q >> 1) * 1024 + (row & 63);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) xs[j * 64] = __uint_as_float(v[q < 2 ? 16 + j : j]);
+                    for (int j = 0; j < 16; ++j) xs[j * 64] = __uint_as_float(q < 2 ? v[16 + j] : v[j]);
                     asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
                     const float* xo = s_xch + xb * 2048 + ((q >> 1) ^ 1) * 1024 + (row & 63);
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        const int c = q < 2 ? j : 16 + j;
-                        const float mine = __uint_as_float(v[q < 2 ? j : 16 + j]), other = xo[j * 64];
-                        const float h = q < 2 ? __fmul_rn(silu_ref(mine), other) : __fmul_rn(silu_ref(other), mine);
-                        if (have && ((live >> c) & 1u)) o[(int64_t)c * a.N] = h_from_f<Y>(h);
+                        const float mine = __uint_as_float(q < 2 ? v[j] : v[16 + j]), other = xo[j * 64];
+                        d[j] = __fmul_rn(silu_ref(q < 2 ? mine : other), q < 2 ? other : mine);
                     }
                     xb ^= 1u;
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (have && ((live >> j) & 1u)) o[(int64_t)j * a.N] = from_f<Y>(__uint_as_float(v[j]));
+                    for (int j = 0; j < NC; ++j) d[j] = __uint_as_float(v[j]);
+                }
+                if (sizeof(Y) == 2 && vec) {
+#pragma unroll
+                    for (int j = 0; j < NC; ++j) turn[j * 32 + lane] = GU ? h_from_f<Y>(d[j]) : from_f<Y>(d[j]);
+                    __syncwarp();
+                    const int f8 = f - lane + (lane & 3) * 8;
+#pragma unroll
+                    for (int k = 0; k < NC / 8; ++k) {
+                        const int c = k * 8 + (lane >> 2);
+                        const uint4 w = *reinterpret_cast<const uint4*>(turn + c * 32 + (lane & 3) * 8);
+                        if (f8 < a.N && ((live >> (cb + c)) & 1u))
+                            *reinterpret_cast<uint4*>(y + (int64_t)(it.p0 + c0 + cb + c) * a.N + f8) = w;
+                    }
+                    __syncwarp();
+                } else {
+#pragma unroll
+                    for (int j = 0; j < NC; ++j)
+                        if (have && ((live >> (cb + j)) & 1u)) o[(int64_t)(cb + j) * a.N] = GU ? h_from_f<Y>(d[j]) : from_f<Y>(d[j]);
                 }
             }
             tc5::fence_before();
@@ -274,14 +253,36 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
     if (warp == 2) { tc5::fence_after(); tc5::tmem_dealloc2(tmem, 512); }
 }
 
-template <typename T, typename Y, bool GU, bool GATHER>
-int run_pair(const GroupedArgs& a, cudaStream_t s) {
+// Rows named by the list, in order: two rows a block.  Rows that do not exist are left out (their results are not stored).
+__global__ void __launch_bounds__(256)
+gather_rows_kernel(const uint4* __restrict__ x, const int* __restrict__ rows, const int* __restrict__ offsets, int n, int P, int K8,
+                   int E, uint4* __restrict__ out) {
+    const int end = seg_bound(offsets, E, P);
+    const int64_t p = (int64_t)blockIdx.x * 2 + (threadIdx.x >> 7);
+    if (p >= end) return;
+    const int r = __ldg(rows + p);
+    if (r < 0 || r >= n) return;
+    const uint4* src = x + (int64_t)r * K8;
+    uint4* dst = out + p * K8;
+    for (int c = threadIdx.x & 127; c < K8; c += 512) {
+        uint4 v[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (c + u * 128 < K8) v[u] = __ldg(src + c + u * 128);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+            if (c + u * 128 < K8) dst[c + u * 128] = v[u];
+    }
+}
+
+template <typename T, typename Y, bool GU>
+int run_pair(const GroupedArgs& a, void* scratch, cudaStream_t s) {
     constexpr int FW = GU ? 128 : 256;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return GSB_ERR_CUDA;
     const int sms = sm_count_of(dev);
     if (sms < 2) return GSB_ERR_CUDA;
-    auto kernel = grouped_pair_kernel<T, Y, GU, GATHER>;
+    auto kernel = grouped_pair_kernel<T, Y, GU>;
     static std::atomic<uint64_t> ready{0};
     if (dev >= 64 || !((ready.load() >> dev) & 1u)) {
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPrSmem) != cudaSuccess) return GSB_ERR_CUDA;
@@ -289,10 +290,16 @@ int run_pair(const GroupedArgs& a, cudaStream_t s) {
     }
     const int64_t fbs = (a.N + FW - 1) / FW, items = ((a.E < a.P ? a.E : a.P) + a.P / kPrNT) * fbs;
     if (items + sms >= (int64_t)1 << 31) return GSB_ERR_TOO_LARGE;
+    const void* sorted = a.x;
+    if (a.rows) {
+        gather_rows_kernel<<<(unsigned)((a.P + 1) / 2), 256, 0, s>>>(reinterpret_cast<const uint4*>(a.x), a.rows, a.offsets, a.n, a.P, a.K / 8, a.E,
+                                                      reinterpret_cast<uint4*>(scratch));
+        sorted = scratch;
+    }
     CUtensorMap tw, tw2, tx;
     constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
     if (!encode(&tw, a.w, bf, a.K, a.N, a.E, 64) || (GU && !encode(&tw2, a.w2, bf, a.K, a.N, a.E, 64)) ||
-        !encode(&tx, a.x, bf, a.K, a.n, 0, 32))
+        !encode(&tx, sorted, bf, a.K, a.rows ? a.P : a.n, 0, 32))
         return GSB_ERR_CUDA;
     const int64_t pairs = items < sms / 2 ? items : sms / 2;
     cudaLaunchConfig_t cfg{};
@@ -301,20 +308,21 @@ int run_pair(const GroupedArgs& a, cudaStream_t s) {
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, a, tw, GU ? tw2 : tw, tx) == cudaSuccess ? GSB_OK : GSB_ERR_LAUNCH;
+    return cudaLaunchKernelEx(&cfg, kernel, a, tw, GU ? tw2 : tw, tx, a.N % 8 == 0 && !misaligned(a.y, 16)) == cudaSuccess ? GSB_OK : GSB_ERR_LAUNCH;
 }
 
 template <typename T>
-int run_pair_any(const GroupedArgs& a, int y_type, cudaStream_t s) {
-    if (a.w2) return run_pair<T, T, true, true>(a, s);
-    if (a.rows) return y_type == GSB_TYPE_F32 ? run_pair<T, float, false, true>(a, s) : run_pair<T, T, false, true>(a, s);
-    return y_type == GSB_TYPE_F32 ? run_pair<T, float, false, false>(a, s) : run_pair<T, T, false, false>(a, s);
+int run_pair_any(const GroupedArgs& a, int y_type, void* scratch, cudaStream_t s) {
+    if (a.w2) return run_pair<T, T, true>(a, scratch, s);
+    return y_type == GSB_TYPE_F32 ? run_pair<T, float, false>(a, scratch, s) : run_pair<T, T, false>(a, scratch, s);
 }
 
 }  // namespace
 
-int launch_grouped_pair(const GroupedArgs& a, int type, int y_type, cudaStream_t s) {
-    return type == GSB_TYPE_BF16 ? run_pair_any<__nv_bfloat16>(a, y_type, s) : run_pair_any<__half>(a, y_type, s);
+size_t grouped_pair_scratch_bytes(int P, int K) { return (size_t)P * K * 2; }
+
+int launch_grouped_pair(const GroupedArgs& a, int type, int y_type, void* scratch, cudaStream_t s) {
+    return type == GSB_TYPE_BF16 ? run_pair_any<__nv_bfloat16>(a, y_type, scratch, s) : run_pair_any<__half>(a, y_type, scratch, s);
 }
 
 int take_pair_status() {

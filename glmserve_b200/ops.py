@@ -154,10 +154,13 @@ def grouped_gemm(x, w, expert_offsets, rows=None, out=None, out_dtype=None):
         raise ValueError("grouped_gemm: expected w [E,N,K] with x's K and expert_offsets [E+1]")
     P = n if rows is None else rows.shape[0]
     out = _out16(out, (P, N), x, out_dtype)
+    nbytes = 0 if rows is None else lib().gsb_grouped_gemm_workspace_bytes(P, K, E)
     with _device_of(x):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         check(lib().gsb_grouped_gemm(x.data_ptr(), w.data_ptr(), _TYPE[x.dtype], expert_offsets.data_ptr(),
                                      None if rows is None else rows.data_ptr(), n, P, K, N, E, out.data_ptr(),
-                                     _TYPE[out.dtype], _raw_stream(x)), "grouped_gemm")
+                                     _TYPE[out.dtype], None if ws is None else ws.data_ptr(), nbytes,
+                                     _raw_stream(x)), "grouped_gemm")
     return out
 
 

@@ -127,10 +127,13 @@ enum { GSB_TYPE_F32 = 0, GSB_TYPE_BF16 = 1, GSB_TYPE_F16 = 2 };
  * or F32).  Sums in fp32, one rounding at the end.  Rows of y that no segment covers, or whose rows[p] is outside
  * [0,n), are left as they were; an expert with an empty segment costs nothing.  Offsets are clamped to [0,P]; with
  * offsets that descend nothing is written.
- * in % 8 == 0, E <= 1024, P <= 2^30; x and w 16-byte aligned; y must not overlap the inputs. */
+ * in % 8 == 0, E <= 1024, P <= 2^30; x and w 16-byte aligned; y must not overlap the inputs.  workspace: with a row
+ * list gsb_grouped_gemm_workspace_bytes() bytes (0 for few rows per expert: then it may be NULL), 256-byte aligned, any
+ * contents; two calls that may overlap on the GPU need a workspace each. */
+GSB_API size_t gsb_grouped_gemm_workspace_bytes(int P, int in, int E);
 GSB_API int gsb_grouped_gemm(const void* x, const void* w, int type, const int* expert_offsets,
                              const int* rows, int n, int P, int in, int out, int E, void* y,
-                             int y_type, void* stream);
+                             int y_type, void* workspace, size_t workspace_bytes, void* stream);
 
 /* moe_expert_ffn with 16-bit weights and activations, tensor-core form of gsb_moe_expert_ffn:
  * out[t] = sum_k w[t,k] * down(silu(gate x) * up x), slots added in order.  x [n,hidden], gate_w/up_w

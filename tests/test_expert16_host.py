@@ -13,9 +13,9 @@ def _v(p):
     return C.c_void_p(p)
 
 
-def _grouped(x=P16, w=P16, type=1, offs=P16, rows=P16, n=4, P=4, inn=64, out=32, E=2, y=P16, yt=1):
+def _grouped(x=P16, w=P16, type=1, offs=P16, rows=P16, n=4, P=4, inn=64, out=32, E=2, y=P16, yt=1, ws=0, nb=0):
     from glmserve_b200._lib import lib
-    return lib().gsb_grouped_gemm(_v(x), _v(w), type, _v(offs), _v(rows), n, P, inn, out, E, _v(y), yt, None)
+    return lib().gsb_grouped_gemm(_v(x), _v(w), type, _v(offs), _v(rows), n, P, inn, out, E, _v(y), yt, _v(ws), C.c_size_t(nb), None)
 
 
 @pytest.mark.parametrize("kw,st", [
@@ -24,7 +24,8 @@ def _grouped(x=P16, w=P16, type=1, offs=P16, rows=P16, n=4, P=4, inn=64, out=32,
     (dict(E=0), INVALID), (dict(rows=0, P=5), INVALID), (dict(x=0), INVALID), (dict(w=0), INVALID),
     (dict(offs=0), INVALID), (dict(y=0), INVALID), (dict(x=P2), INVALID), (dict(w=P2), INVALID), (dict(y=ODD), INVALID),
     (dict(y=P2, yt=0), INVALID), (dict(offs=P2), INVALID), (dict(rows=P2), INVALID),
-    (dict(inn=60), UNSUPPORTED), (dict(E=1025), UNSUPPORTED), (dict(P=(1 << 30) + 1), UNSUPPORTED)])
+    (dict(inn=60), UNSUPPORTED), (dict(E=1025), UNSUPPORTED), (dict(P=(1 << 30) + 1), UNSUPPORTED),
+    (dict(P=2000), INVALID), (dict(P=2000, ws=P16 + 16, nb=1 << 30), INVALID), (dict(P=2000, ws=P16, nb=64), WORKSPACE)])
 def test_grouped_gemm_refusals(kw, st):
     assert _grouped(**kw) == st
 
@@ -70,6 +71,7 @@ def test_sizes():
     assert L.gsb_moe_expert_ffn_w16_workspace_bytes(0, 8, 64, 64, 4) == 0
     small, large = (L.gsb_moe_expert_ffn_w16_workspace_bytes(n, 8, 6144, 2048, 32) for n in (64, 8192))
     assert 64 * 8 * (2 * 2048 + 4 * 6144) <= small < large and large >= 8192 * 8 * (2 * 2048 + 4 * 6144)
+    assert L.gsb_grouped_gemm_workspace_bytes(8, 6144, 32) == 0 and L.gsb_grouped_gemm_workspace_bytes(8192, 6144, 8) == 8192 * 6144 * 2
     assert L.gsb_lora_scratch_bytes(0, 16, 4) == 0 and L.gsb_lora_scratch_bytes(8192, 64, 8) >= 8192 * 64 * 4
 
 
