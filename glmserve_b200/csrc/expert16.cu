@@ -10,43 +10,46 @@ namespace gsb {
 
 namespace {
 
-// ---- the tensor-core kernel -------------------------------------------------------------------
-// One item = 128 weight rows x up to NT token rows of one expert, as D[weight row, token] = sum_k W[row, k] X[token, k]
-// (M = 128 weight rows in the 128 TMEM lanes, N = tokens rounded up to 16): a decode batch pads tokens to 16, not to 128.
-// The 128 rows are two boxes of 64: consecutive rows of one matrix, or 64 gate rows and their 64 up rows, so that SwiGLU
-// pairs meet in the epilogue.  X rows are gathered by TMA (four rows an instruction), so no sorted copy is made.
-// A cluster of S CTAs works on one item, each on 1/S of K: the partial tiles are exchanged through distributed shared
-// memory, CTA r finishing the r-th part of the columns, and added in rank order - no atomics, the same bits every time.
-constexpr int kGrThreads = 256;            // warps: 0 weights, 1 MMA, 2 TMEM, 3 token rows, 4-7 epilogue
-constexpr int kCh = 16;                    // accumulator columns a pass of the epilogue exchanges
-constexpr int kABytes = 128 * 128;         // 128 weight rows x 64 columns
-
-template <int NT> struct GrCfg {
-    static constexpr int kps = NT <= 16 ? 2 : 1;                   // k-blocks of 64 columns per stage
-    static constexpr int stages = NT <= 16 ? 5 : NT <= 64 ? 8 : 4;
-    static constexpr int bbytes = NT * 128;
-    static constexpr int stage_bytes = kps * (kABytes + bbytes);
-    static constexpr int red_bytes = 2 * kCh * 128 * 4;
-    static constexpr int tmem_cols = 2 * NT < 32 ? 32 : 2 * NT;
-    static constexpr size_t smem = (size_t)stages * stage_bytes + red_bytes + (kMaxE + 4) * 4 + 256;
-    static_assert(smem <= 227 * 1024, "stages exceed the shared memory of an SM");
-};
+// ---- few rows per expert ----------------------------------------------------------------------
+// Bound by the weights, which are read once; everything is arranged around keeping that stream going.
+// One item = w weight rows (128, 64 or 32) x up to 16 token rows of one expert, as D[weight row, token] = sum_k W[row, k]
+// X[token, k]: the weights are tcgen05's M operand (128 TMEM lanes), so the tokens are padded to 16, not to 128.  For
+// SwiGLU w is made of gate rows followed by as many up rows.  The copies of the next items run while this one is
+// multiplied and stored (one ring over all items of a CTA).  Token rows are gathered by warps with 16-byte cp.async, only
+// as many as there are; through TMA's gather they would hold up the weights in the same queue (GATHER4 us instead of
+// FEW_US for 32 experts of 6144 x 2048 with two rows each).
+// w is chosen on the device, where the number of experts with rows is known: the widest that does not leave SMs idle in
+// the last round (512 items of 128 rows on 148 SMs take 4 rounds, 1024 of 64 rows 7 half as long: 135 us against 123 for
+// 32 experts of 6144 x 2048, SPLIT_US with the same items cut in two along K instead).
+constexpr int kGrThreads = 384;            // warps: 0 weights, 1 MMA, 2 TMEM, 4-7 epilogue, 8-11 token rows
+constexpr int kABytes = 128 * 128;         // at most 128 weight rows x 64 columns
+constexpr int kNT = 16;                    // token rows per item at most
+constexpr int kBBytes = kNT * 128;
+constexpr int kKps = 2;                    // k-blocks of 64 columns per stage
+constexpr int kTokWarps = 4;
+constexpr int kRing = 5 * kKps * (kABytes + kBBytes);   // five stages of 128 weight rows, 9 of 64, 15 of 32
+constexpr int kMaxStages = 15;
+constexpr int kXch = 2 * kNT * 128 * 4;    // SwiGLU: two buffers of 16 columns x 128 rows
+constexpr size_t kGrSmem = (size_t)kRing + kXch + (kMaxE + 4) * 4 + 256;
+// A token warp comes back to the ring kTokWarps stages later.  With fewer stages than that it could be two uses of a stage
+// ahead, where the parity it waits for is the one that an unfinished phase shows as well.
+static_assert(kRing / (kKps * (kABytes + kBBytes)) >= kTokWarps, "ring too short for the token warps");
+static_assert(kGrSmem <= 227 * 1024, "stages exceed the shared memory of an SM");
 
 __device__ int g_op16_status;
 
 // item i: experts in order; inside one, all token tiles of a feature block run next to each other (they read the
 // same weights, which the second one finds in L2).  `e` only moves forward.
-template <int NT, int FW>
-__device__ __forceinline__ GrItem gr_item(const GroupedArgs& a, const int* pre, int i, int fb_count, int& e) {
+__device__ __forceinline__ GrItem gr_item(const GroupedArgs& a, const int* pre, int i, int fb_count, int fw, int& e) {
     while (i >= pre[e + 1] * fb_count) ++e;
     const int nt = pre[e + 1] - pre[e], local = i - pre[e] * fb_count;
     const int fb = local / nt, tt = local - fb * nt;
     GrItem it;
     it.e = e;
-    it.f0 = fb * FW;
+    it.f0 = fb * fw;
     const int lo = seg_bound(a.offsets, e, a.P), hi = seg_bound(a.offsets, e + 1, a.P);
-    it.p0 = lo + tt * NT;
-    it.cnt = min(NT, hi - it.p0);
+    it.p0 = lo + tt * kNT;
+    it.cnt = min(kNT, hi - it.p0);
     return it;
 }
 
@@ -55,248 +58,229 @@ __device__ __forceinline__ void gr_timeout(volatile int* abort_flag) {
     atomicCAS(&g_op16_status, 0, GSB_ERR_TIMEOUT);
 }
 
-template <int NT, typename T, typename Y, bool GU>
+template <typename T, typename Y, bool GU>
 __global__ void __launch_bounds__(kGrThreads, 1)
-grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_w2,
-               const __grid_constant__ CUtensorMap tm_x) {
-    using Cfg = GrCfg<NT>;
-    constexpr int FW = GU ? 64 : 128;      // output features of an item
+grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_w2) {
     extern __shared__ __align__(1024) uint8_t smem[];
-    uint8_t* s_stage = smem;
-    float* s_red = reinterpret_cast<float*>(smem + Cfg::stages * Cfg::stage_bytes);
-    int* pre = reinterpret_cast<int*>(s_red + 2 * kCh * 128);               // [E + 1] token tiles before expert e
+    float* s_xch = reinterpret_cast<float*>(smem + kRing);
+    int* pre = reinterpret_cast<int*>(smem + kRing + kXch);   // [E + 1] token tiles before expert e
     uint64_t* full = reinterpret_cast<uint64_t*>(pre + kMaxE + 4);
-    uint64_t* empty = full + Cfg::stages;
-    uint64_t* acc_full = empty + Cfg::stages;
+    uint64_t* empty = full + kMaxStages;
+    uint64_t* acc_full = empty + kMaxStages;
     uint64_t* acc_empty = acc_full + 2;
-    uint64_t* red_full = acc_empty + 2;
-    uint64_t* red_free = red_full + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(red_free + 2);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int S = (int)tc5::cluster_size(), rank = (int)tc5::cluster_rank();
     if (tid == 0) {
-        for (int i = 0; i < Cfg::stages; ++i) { mbar_init(&full[i], 2); mbar_init(&empty[i], 1); }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 4);
-            mbar_init(&red_full[i], 4 * S); mbar_init(&red_free[i], 4 * S);
-        }
+        for (int i = 0; i < kMaxStages; ++i) { mbar_init(&full[i], 2); mbar_init(&empty[i], 1); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 4); }
         *abort_flag = 0;
         fence_barrier_init();
     }
-    if (warp == 2) { tc5::tmem_alloc(tmem_slot, Cfg::tmem_cols); tc5::tmem_relinquish(); }
+    if (warp == 2) { tc5::tmem_alloc(tmem_slot, 2 * kNT); tc5::tmem_relinquish(); }
     int descending = (smem_u32(smem) & 1023u) != 0;    // (the swizzled tiles need a 1 KiB boundary: as good as no list)
-    descending |= seg_scan<NT>(a.offsets, a.E, a.P, pre, reinterpret_cast<int*>(s_red));
+    descending |= seg_scan<kNT>(a.offsets, a.E, a.P, pre, reinterpret_cast<int*>(s_xch));
     tc5::fence_before();
     descending = __syncthreads_or(descending);
     tc5::fence_after();
-    if (S > 1) tc5::cluster_sync_all();    // the peers' barriers exist before anyone arrives on them
     const uint32_t tmem = *tmem_slot;
-    const int nkb = (a.K + 63) >> 6, kb0 = nkb * rank / S, kb1 = nkb * (rank + 1) / S;
-    const int FB = (a.N + FW - 1) / FW;
-    // at most (E + P / NT) * FB, which the host has checked to fit; a list that is not ascending is no list
-    const int items = descending ? 0 : pre[a.E] * FB;
-    const int first = blockIdx.x / S, step = gridDim.x / S;
+    const int nkb = (a.K + 63) >> 6;
+    // at most (E + P / 16) token tiles, and so many items as the host has checked to fit; a list that descends is no list
+    const int tiles = descending ? 0 : pre[a.E];
+    const int w = best_width(tiles, a.N * (GU ? 2 : 1), (int)gridDim.x, GU ? 64 : 32);   // weight rows of an item
+    const int fw = GU ? w / 2 : w;         // output features of an item
+    const int FB = (a.N + fw - 1) / fw;
+    const int items = tiles * FB;
+    // the ring's stages are as long as w rows need, so a narrow item has as many bytes on their way as a wide one (the
+    // MMA's unused rows read on into what follows; their lanes are not stored)
+    const int abytes = w * 128, stage_bytes = kKps * (abytes + kBBytes), stages = min(kMaxStages, kRing / stage_bytes);
+    const int first = blockIdx.x, step = gridDim.x;
 
-    if (warp == 0) {
-        if (lane == 0) {                   // ---- weights
-            uint32_t st = 0, ph = 0;
-            int e = 0;
-            bool dead = false;
-            for (int i = first; i < items && !dead && !*abort_flag; i += step) {
-                const GrItem it = gr_item<NT, FW>(a, pre, i, FB, e);
-                for (int kb = kb0; kb < kb1; kb += Cfg::kps) {
-                    if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
-                    const int nk = min(Cfg::kps, kb1 - kb);
-                    mbar_arrive_expect_tx(&full[st], (uint32_t)nk * kABytes);
-                    uint8_t* dst = s_stage + st * Cfg::stage_bytes;
-                    for (int j = 0; j < nk; ++j) {
-                        tc5::tma_load_3d(dst + j * kABytes, &tm_w, (kb + j) * 64, it.f0, it.e, &full[st]);
-                        tc5::tma_load_3d(dst + j * kABytes + kABytes / 2, GU ? &tm_w2 : &tm_w, (kb + j) * 64,
-                                         GU ? it.f0 : it.f0 + 64, it.e, &full[st]);
-                    }
-                    if (++st == Cfg::stages) { st = 0; ph ^= 1u; }
-                }
-            }
-            // after a time-out elsewhere: nothing may still be copying into this block's memory when it ends
-            if (*abort_flag)
-                for (int j = 0; j < Cfg::stages; ++j) {
-                    if (st == 0) { st = Cfg::stages; ph ^= 1u; }
-                    --st;
-                    mbar_wait(&full[st], ph, kGrWaitLimit / 16);
-                }
-        }
-    } else if (warp == 3) {                // ---- token rows
+    if (warp == 0) {                       // ---- weights
+        const bool leader = tc5::elect_one();
         uint32_t st = 0, ph = 0;
         int e = 0;
         bool dead = false;
-        constexpr int G = NT > 128 ? NT / 128 : 1;    // groups of four rows per lane
         for (int i = first; i < items && !dead && !*abort_flag; i += step) {
-            const GrItem it = gr_item<NT, FW>(a, pre, i, FB, e);
-            const int nr = (it.cnt + 15) & ~15;
-            int r[G][4];
-#pragma unroll
-            for (int g = 0; g < G; ++g)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int q = (g * 32 + lane) * 4 + j;
-                    // columns behind the tile's last row, and rows that do not exist, read row 0; neither is stored
-                    int v = 0;
-                    if (q < it.cnt) v = a.rows ? __ldg(a.rows + it.p0 + q) : it.p0 + q;
-                    r[g][j] = v >= 0 && v < a.n ? v : 0;
-                }
-            for (int kb = kb0; kb < kb1; kb += Cfg::kps) {
+            const GrItem it = gr_item(a, pre, i, FB, fw, e);
+            for (int kb = 0; kb < nkb; kb += kKps) {
                 if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
-                const int nk = min(Cfg::kps, kb1 - kb);
-                if (lane == 0) mbar_arrive_expect_tx(&full[st], (uint32_t)(nk * nr * 128));
-                __syncwarp();
-                uint8_t* dst = s_stage + st * Cfg::stage_bytes + Cfg::kps * kABytes;
-                for (int j = 0; j < nk; ++j)
-#pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        const int q = (g * 32 + lane) * 4;
-                        if (q < nr) tc5::tma_gather4(dst + j * Cfg::bbytes + q * 128, &tm_x, (kb + j) * 64, r[g][0], r[g][1], r[g][2], r[g][3], &full[st]);
-                    }
-                if (++st == Cfg::stages) { st = 0; ph ^= 1u; }
+                if (leader) {
+                    const int nk = min(kKps, nkb - kb);
+                    mbar_arrive_expect_tx(&full[st], (uint32_t)(nk * w * 128));
+                    uint8_t* dst = smem + st * stage_bytes;
+                    for (int j = 0; j < nk; ++j)
+                        for (int r = 0; r < fw; r += 32) {
+                            tc5::tma_load_3d(dst + j * abytes + r * 128, &tm_w, (kb + j) * 64, it.f0 + r, it.e, &full[st]);
+                            if (GU) tc5::tma_load_3d(dst + j * abytes + (fw + r) * 128, &tm_w2, (kb + j) * 64, it.f0 + r, it.e, &full[st]);
+                        }
+                }
+                if (++st == (uint32_t)stages) { st = 0; ph ^= 1u; }
             }
             dead = __any_sync(0xffffffffu, dead);
         }
-    } else if (warp == 1) {
-        if (lane == 0) {                   // ---- MMA issue
-            uint32_t st = 0, ph = 0, tl = 0;
-            int e = 0;
-            bool dead = false;
-            constexpr uint32_t ab = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
-            const uint64_t d0 = tc5::desc_sw128(smem_u32(s_stage));
-            for (int i = first; i < items && !dead && !*abort_flag; i += step, ++tl) {
-                const GrItem it = gr_item<NT, FW>(a, pre, i, FB, e);
-                const uint32_t buf = tl & 1u;
-                if (!mbar_wait(&acc_empty[buf], ((tl >> 1) & 1u) ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); break; }
-                tc5::fence_after();
-                const uint32_t idesc = tc5::idesc_f16(ab, 128, (uint32_t)((it.cnt + 15) & ~15));
-                uint32_t acc = 0;
-                for (int kb = kb0; kb < kb1; kb += Cfg::kps) {
-                    if (!mbar_wait(&full[st], ph, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
-                    tc5::fence_after();
-                    const int nk = min(Cfg::kps, kb1 - kb);
-                    const uint64_t ad = d0 + (uint64_t)(st * (uint32_t)(Cfg::stage_bytes >> 4));
-                    const uint64_t bd = ad + (uint64_t)(Cfg::kps * kABytes >> 4);
-                    for (int j = 0; j < nk; ++j)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            tc5::mma_f16_ss(tmem + buf * NT, ad + (uint64_t)(j * (kABytes >> 4) + k * 2),
-                                            bd + (uint64_t)(j * (Cfg::bbytes >> 4) + k * 2), idesc, acc);
-                            acc = 1u;
-                        }
-                    tc5::commit(&empty[st]);
-                    if (++st == Cfg::stages) { st = 0; ph ^= 1u; }
-                }
-                if (!dead) tc5::commit(&acc_full[buf]);
+        // the signals of the last MMAs have arrived before the block ends
+        for (int j = 0; j < stages && !*abort_flag; ++j) {
+            mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit);
+            if (++st == (uint32_t)stages) { st = 0; ph ^= 1u; }
+        }
+        // after a time-out: nothing may still be copying into this block's memory when it ends
+        if (*abort_flag)
+            for (int j = 0; j < stages; ++j) {
+                if (st == 0) { st = (uint32_t)stages; ph ^= 1u; }
+                --st;
+                mbar_wait(&full[st], ph, kGrWaitLimit / 16);
             }
+    } else if (warp >= 8) {                // ---- token rows: the four warps take stages in turn
+        // eight lanes copy the 128 bytes of a row's k-block; a warp fences its copies before it hands the stage over, and
+        // the other three's are on their way meanwhile
+        const int group = warp - 8, piece = lane & 7;
+        const T* x = reinterpret_cast<const T*>(a.x) + piece * 8;
+        uint32_t st = 0, ph = 0, cnt = 0;
+        int e = 0;
+        bool dead = false;
+        for (int i = first; i < items && !dead && !*abort_flag; i += step) {
+            const GrItem it = gr_item(a, pre, i, FB, fw, e);
+            int r[kNT / 4];
+#pragma unroll
+            for (int j = 0; j < kNT / 4; ++j) {
+                // rows that do not exist read row 0 and are not stored; what lies in the place of the columns behind the
+                // tile's last reaches only those columns
+                const int q = j * 4 + (lane >> 3);
+                r[j] = -1;
+                if (q < it.cnt) {
+                    const int v = a.rows ? __ldg(a.rows + it.p0 + q) : it.p0 + q;
+                    r[j] = v >= 0 && v < a.n ? v : 0;
+                }
+            }
+            for (int kb = 0; kb < nkb; kb += kKps, ++cnt) {
+                if ((int)(cnt % kTokWarps) == group) {
+                    if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
+                    const uint32_t base = smem_u32(smem) + st * stage_bytes + kKps * abytes + (uint32_t)((lane >> 3) * 128);
+#pragma unroll
+                    for (int u = 0; u < kKps; ++u) {
+                        const bool in = (kb + u) * 64 + piece * 8 < a.K;
+                        const T* xk = in ? x + (kb + u) * 64 : x;
+#pragma unroll
+                        for (int j = 0; j < kNT / 4; ++j)     // 128-byte swizzle: piece c of row q lies at c ^ q % 8
+                            if (r[j] >= 0 && kb + u < nkb)
+                                tc5::cp_async16(base + (uint32_t)(u * kBBytes + j * 512 + ((piece ^ ((j * 4 + (lane >> 3)) & 7)) << 4)),
+                                                xk + (int64_t)r[j] * a.K, in);
+                    }
+                    tc5::cp_async_commit();
+                    tc5::cp_async_wait<0>();
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&full[st]);
+                }
+                if (++st == (uint32_t)stages) { st = 0; ph ^= 1u; }
+            }
+            dead = __any_sync(0xffffffffu, dead);
+        }
+        tc5::cp_async_wait<0>();
+    } else if (warp == 1) {                // ---- MMA issue
+        const bool leader = tc5::elect_one();
+        uint32_t st = 0, ph = 0, tl = 0;
+        bool dead = false;
+        constexpr uint32_t idesc_ab = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+        const uint32_t idesc = tc5::idesc_f16(idesc_ab, 128, kNT);
+        const uint64_t d0 = tc5::desc_sw128(smem_u32(smem));
+        for (int i = first; i < items && !dead && !*abort_flag; i += step, ++tl) {
+            const uint32_t buf = tl & 1u;
+            if (!mbar_wait(&acc_empty[buf], ((tl >> 1) & 1u) ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); break; }
+            tc5::fence_after();
+            uint32_t acc = 0;
+            for (int kb = 0; kb < nkb; kb += kKps) {
+                if (!mbar_wait(&full[st], ph, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
+                tc5::fence_after();
+                if (leader) {
+                    const uint64_t ad = d0 + (uint64_t)(st * (uint32_t)(stage_bytes >> 4));
+                    const uint64_t bd = ad + (uint64_t)(kKps * abytes >> 4);
+#pragma unroll
+                    for (int j = 0; j < kKps; ++j)
+                        if (kb + j < nkb)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k)
+                                tc5::mma_f16_ss(tmem + buf * kNT, ad + (uint64_t)(j * (abytes >> 4) + k * 2),
+                                                bd + (uint64_t)(j * (kBBytes >> 4) + k * 2), idesc, j + k ? 1u : acc);
+                    tc5::commit(&empty[st]);
+                }
+                acc = 1u;
+                if (++st == (uint32_t)stages) { st = 0; ph ^= 1u; }
+            }
+            dead = __any_sync(0xffffffffu, dead);
+            if (!dead && leader) tc5::commit(&acc_full[buf]);
         }
     } else if (warp >= 4) {                // ---- epilogue: this thread's TMEM lane = weight row
         const int q = warp & 3, row = q * 32 + lane;
-        const int lsh = S == 4 ? 2 : S == 2 ? 1 : 0, per = kCh >> lsh;     // columns of a pass that one CTA finishes
-        const uint32_t red0 = smem_u32(s_red);
-        uint32_t tl = 0, cc = 0;
+        uint32_t tl = 0;
         int e = 0;
-        bool dead = false;
         Y* y = reinterpret_cast<Y*>(a.y);
-        for (int i = first; i < items && !dead; i += step, ++tl) {
-            const GrItem it = gr_item<NT, FW>(a, pre, i, FB, e);
+        for (int i = first; i < items; i += step, ++tl) {
+            const GrItem it = gr_item(a, pre, i, FB, fw, e);
             const uint32_t buf = tl & 1u;
-            if (*abort_flag || !mbar_wait(&acc_full[buf], (tl >> 1) & 1u, kGrWaitLimit)) {
-                if (!*abort_flag) gr_timeout(abort_flag);
-                break;
-            }
+            int ok = *abort_flag ? 0 : (int)mbar_wait(&acc_full[buf], (tl >> 1) & 1u, kGrWaitLimit);
+            if (!ok) gr_timeout(abort_flag);
+            // all four warps must agree to go on: they meet at a barrier below
+            if (GU) ok = epilogue_agree(ok);
+            if (!ok) break;
             tc5::fence_after();
-            for (int c0 = 0; c0 < it.cnt; c0 += kCh, ++cc) {
-                const uint32_t rb = cc & 1u, rph = (cc >> 1) & 1u;
-                uint32_t v[kCh];
-                tc5::tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + buf * NT + (uint32_t)c0, v);
-                tc5::tmem_ld_wait();
-                if (!tc5::wait_cluster(&red_free[rb], rph ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
-#pragma unroll
-                for (int j = 0; j < kCh; ++j) {
-                    const int owner = j >> (4 - lsh), jl = j & (per - 1);
-                    tc5::st_cluster(tc5::map_rank(red0 + (uint32_t)(((rb * kCh + rank * per + jl) * 128 + row) * 4), (uint32_t)owner),
-                                    __uint_as_float(v[j]));
-                }
-                __syncwarp();
-                if (lane < S) tc5::arrive_cluster(tc5::map_rank(smem_u32(&red_full[rb]), (uint32_t)lane));
-                if (!tc5::wait_cluster(&red_full[rb], rph, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
-                const float* red = s_red + rb * kCh * 128;
-                const int f = it.f0 + (GU ? (row & 63) : row);
-                for (int jl = GU ? row >> 6 : 0; jl < per; jl += GU ? 2 : 1) {
-                    const int c = c0 + rank * per + jl;
-                    if (c >= it.cnt || f >= a.N) continue;
-                    const int p = it.p0 + c;
-                    if (a.rows) { const int r = __ldg(a.rows + p); if (r < 0 || r >= a.n) continue; }
-                    float s0 = 0.f, s1 = 0.f;
-                    for (int src = 0; src < S; ++src) {
-                        s0 += red[(src * per + jl) * 128 + (GU ? (row & 63) : row)];
-                        if (GU) s1 += red[(src * per + jl) * 128 + (row & 63) + 64];
-                    }
-                    y[(int64_t)p * a.N + f] = GU ? h_from_f<Y>(__fmul_rn(silu_ref(s0), s1)) : from_f<Y>(s0);
-                }
-                __syncwarp();
-                if (lane < S) tc5::arrive_cluster(tc5::map_rank(smem_u32(&red_free[rb]), (uint32_t)lane));
-            }
+            uint32_t u[kNT];
+            tc5::tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + buf * kNT, u);
+            // which of the tokens exist
+            int r = lane < it.cnt ? 0 : -1;
+            if (a.rows && r == 0) r = __ldg(a.rows + it.p0 + lane);
+            const uint32_t live = __ballot_sync(0xffffffffu, r >= 0 && r < a.n);
+            tc5::tmem_ld_wait();
             tc5::fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&acc_empty[buf]);
+            if (GU) {
+                // rows [0, fw) are gate, [fw, 2 fw) the up rows of the same features
+                float* xs = s_xch + buf * kNT * 128;
+#pragma unroll
+                for (int j = 0; j < kNT; ++j) xs[j * 128 + row] = __uint_as_float(u[j]);
+                asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
+                const int fl = row & (fw - 1), f = it.f0 + fl, groups = 128 / fw;     // fw is 64 or 32
+                for (int c = row / fw; c < it.cnt; c += groups)
+                    if (f < a.N && ((live >> c) & 1u))
+                        y[(int64_t)(it.p0 + c) * a.N + f] = h_from_f<Y>(__fmul_rn(silu_ref(xs[c * 128 + fl]), xs[c * 128 + fw + fl]));
+            } else {
+                const int f = it.f0 + row;
+                if (row < w && f < a.N)
+#pragma unroll
+                    for (int j = 0; j < kNT; ++j)
+                        if ((live >> j) & 1u) y[(int64_t)(it.p0 + j) * a.N + f] = from_f<Y>(__uint_as_float(u[j]));
+            }
         }
     }
     __syncwarp();
     tc5::fence_before();
     __syncthreads();
-    if (S > 1) tc5::cluster_sync_all();    // peers may still read or signal this block's memory
-    if (warp == 2) { tc5::fence_after(); tc5::tmem_dealloc(tmem, Cfg::tmem_cols); }
-}
-
-template <int NT, typename T, typename Y, bool GU>
-int run_grouped_nt(const GroupedArgs& a, int S, cudaStream_t s) {
-    using Cfg = GrCfg<NT>;
-    constexpr int FW = GU ? 64 : 128;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return GSB_ERR_CUDA;
-    const int sms = sm_count_of(dev);
-    if (!sms) return GSB_ERR_CUDA;
-    auto kernel = grouped_kernel<NT, T, Y, GU>;
-    static std::atomic<uint64_t> ready{0};     // devices on which the shared-memory size was raised
-    if (dev >= 64 || !((ready.load() >> dev) & 1u)) {
-        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Cfg::smem) != cudaSuccess) return GSB_ERR_CUDA;
-        if (dev < 64) ready.fetch_or(1ull << dev);
-    }
-    const int64_t fbs = (a.N + FW - 1) / FW, tiles = (a.E < a.P ? a.E : a.P) + a.P / NT;
-    const int64_t items = tiles * fbs;
-    if (items + sms >= (int64_t)1 << 31) return GSB_ERR_TOO_LARGE;
-    CUtensorMap tw, tw2, tx;
-    constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
-    if (!encode(&tw, a.w, bf, a.K, a.N, a.E, 64) || (GU && !encode(&tw2, a.w2, bf, a.K, a.N, a.E, 64)) ||
-        !encode(&tx, a.x, bf, a.K, a.n, 0, 1))
-        return GSB_ERR_CUDA;
-    const int64_t groups = items < sms / S ? items : sms / S;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(groups * S)); cfg.blockDim = dim3(kGrThreads); cfg.dynamicSmemBytes = Cfg::smem; cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = (unsigned)S; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-    cfg.attrs = at; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, a, tw, GU ? tw2 : tw, tx) == cudaSuccess ? GSB_OK : GSB_ERR_LAUNCH;
+    if (warp == 2) { tc5::fence_after(); tc5::tmem_dealloc(tmem, 2 * kNT); }
 }
 
 template <typename T, typename Y, bool GU>
 int run_grouped(const GroupedArgs& a, cudaStream_t s) {
-    const int64_t per_expert = a.P / a.E, nkb = (a.K + 63) / 64;
-    const int nt = per_expert <= 16 ? 16 : per_expert <= 64 ? 64 : 256;
-    const int64_t fbs = (a.N + (GU ? 63 : 127)) / (GU ? 64 : 128), items = ((a.E < a.P ? a.E : a.P) + a.P / nt) * fbs;
-    int S = items >= 1184 ? 1 : items >= 592 ? 2 : 4;
-    while (S > nkb) S >>= 1;
-    if (nt == 16) return run_grouped_nt<16, T, Y, GU>(a, S, s);
-    if (nt == 64) return run_grouped_nt<64, T, Y, GU>(a, S, s);
-    return run_grouped_nt<256, T, Y, GU>(a, S, s);
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return GSB_ERR_CUDA;
+    const int sms = sm_count_of(dev);
+    if (!sms) return GSB_ERR_CUDA;
+    auto kernel = grouped_kernel<T, Y, GU>;
+    static std::atomic<uint64_t> ready{0};     // devices on which the shared-memory size was raised
+    if (dev >= 64 || !((ready.load() >> dev) & 1u)) {
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGrSmem) != cudaSuccess) return GSB_ERR_CUDA;
+        if (dev < 64) ready.fetch_or(1ull << dev);
+    }
+    const int64_t fbs = (a.N + 31) / 32, tiles = (a.E < a.P ? a.E : a.P) + a.P / kNT, items = tiles * fbs;
+    if (items + sms >= (int64_t)1 << 31) return GSB_ERR_TOO_LARGE;
+    CUtensorMap tw, tw2;
+    constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
+    if (!encode(&tw, a.w, bf, a.K, a.N, a.E, 32) || (GU && !encode(&tw2, a.w2, bf, a.K, a.N, a.E, 32))) return GSB_ERR_CUDA;
+    const int grid = (int)(items < sms ? items : sms);
+    kernel<<<grid, kGrThreads, kGrSmem, s>>>(a, tw, GU ? tw2 : tw);
+    return launch_status();
 }
 
 template <typename T>
@@ -305,7 +289,7 @@ int run_grouped_any(const GroupedArgs& a, int y_type, cudaStream_t s) {
     return y_type == GSB_TYPE_F32 ? run_grouped<T, float, false>(a, s) : run_grouped<T, T, false>(a, s);
 }
 
-bool use_pair(int P, int E) { return P / E > 64; }
+bool use_pair(int P, int E) { return P / E > 16; }
 
 int launch_grouped(const GroupedArgs& a, int type, int y_type, void* scratch, cudaStream_t s) {
     if (use_pair(a.P, a.E)) return launch_grouped_pair(a, type, y_type, scratch, s);

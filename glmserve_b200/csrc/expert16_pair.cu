@@ -37,8 +37,7 @@ __device__ __forceinline__ void pr_timeout(volatile int* abort_flag) {
 
 // Item i: experts in order, inside one the token tiles of a feature block next to each other (same weights).  An
 // expert's rows are cut into equal tiles (multiples of 32 rows) instead of full ones and a rest.
-template <int FW>
-__device__ __forceinline__ GrItem pr_item(const GroupedArgs& a, const int* pre, int i, int fb_count, int& e) {
+__device__ __forceinline__ GrItem pr_item(const GroupedArgs& a, const int* pre, int i, int fb_count, int fw, int& e) {
     while (i >= pre[e + 1] * fb_count) ++e;
     const int nt = pre[e + 1] - pre[e], local = i - pre[e] * fb_count;
     const int fb = local / nt, tt = local - fb * nt;
@@ -46,7 +45,7 @@ __device__ __forceinline__ GrItem pr_item(const GroupedArgs& a, const int* pre, 
     const int rows = ((hi - lo + nt - 1) / nt + 31) & ~31;
     GrItem it;
     it.e = e;
-    it.f0 = fb * FW;
+    it.f0 = fb * fw;
     it.p0 = lo + tt * rows;
     it.cnt = min(rows, hi - it.p0);
     return it;
@@ -56,7 +55,6 @@ template <typename T, typename Y, bool GU>
 __global__ void __launch_bounds__(kPrThreads, 1)
 grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_w2,
                     const __grid_constant__ CUtensorMap tm_x, int vec) {
-    constexpr int FW = GU ? 128 : 256;     // output features of an item (both CTAs)
     extern __shared__ __align__(1024) uint8_t smem[];
     float* s_xch = reinterpret_cast<float*>(smem + kPrStages * kPrStageBytes);
     uint8_t* s_turn = smem + kPrStages * kPrStageBytes + kPrXch;
@@ -89,68 +87,75 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
     tc5::fence_after();
     const uint32_t tmem = *tmem_slot;
     const int nkb = (a.K + 63) >> 6;
-    const int FB = (a.N + FW - 1) / FW;
-    const int items = descending ? 0 : pre[a.E] * FB;
+    const int tiles = descending ? 0 : pre[a.E];
+    constexpr int fc = GU ? 64 : 128, fw = 2 * fc;     // output features of this CTA, and of an item (both CTAs)
+    const int FB = (a.N + fw - 1) / fw;
+    const int items = tiles * FB;
     const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
-    const int fr = rank * (FW / 2);        // this CTA's features start here inside an item
+    const int fr = rank * fc;              // this CTA's features start here inside an item
 
-    if (warp == 0) {
-        if (lane == 0) {                   // ---- weights of this CTA; bytes are counted on the leader's barrier
-            uint32_t st = 0, ph = 0;
-            int e = 0;
-            bool dead = false;
-            for (int i = first; i < items && !dead && !*abort_flag; i += step) {
-                const GrItem it = pr_item<FW>(a, pre, i, FB, e);
-                const int nb = ((it.cnt + 31) / 32 * 16 + 31) / 32;     // token boxes of 32 rows per CTA
-                for (int kb = 0; kb < nkb; ++kb) {
-                    if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { pr_timeout(abort_flag); dead = true; break; }
+    if (warp == 0) {                       // ---- weights of this CTA; bytes are counted on the leader's barrier
+        const bool leader = tc5::elect_one();
+        uint32_t st = 0, ph = 0;
+        int e = 0;
+        bool dead = false;
+        for (int i = first; i < items && !dead && !*abort_flag; i += step) {
+            const GrItem it = pr_item(a, pre, i, FB, fw, e);
+            const int nb = ((it.cnt + 31) / 32 * 16 + 31) / 32;         // token boxes of 32 rows per CTA
+            for (int kb = 0; kb < nkb; ++kb) {
+                if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { pr_timeout(abort_flag); dead = true; break; }
+                if (leader) {
                     if (rank == 0) mbar_arrive_expect_tx(&full[st], 2u * (kPrHalf + (uint32_t)nb * 4096u));
                     const uint32_t bar = tc5::map_rank(smem_u32(&full[st]), 0);
                     uint8_t* dst = smem + st * kPrStageBytes;
                     tc5::tma2_load_3d(dst, &tm_w, kb * 64, it.f0 + fr, it.e, bar);
-                    tc5::tma2_load_3d(dst + kPrHalf / 2, GU ? &tm_w2 : &tm_w, kb * 64, GU ? it.f0 + fr : it.f0 + fr + 64, it.e, bar);
-                    if (++st == kPrStages) { st = 0; ph ^= 1u; }
+                    if (GU) tc5::tma2_load_3d(dst + kPrHalf / 2, &tm_w2, kb * 64, it.f0 + fr, it.e, bar);
                 }
-            }
-            // the signals of the last MMAs have arrived before the block ends
-            for (int j = 0; j < kPrStages && !*abort_flag; ++j) {
-                mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit);
                 if (++st == kPrStages) { st = 0; ph ^= 1u; }
             }
-            // after a time-out: nothing may still be copying into this block's memory when it ends
-            if (*abort_flag && rank == 0)
-                for (int j = 0; j < kPrStages; ++j) {
-                    if (st == 0) { st = kPrStages; ph ^= 1u; }
-                    --st;
-                    mbar_wait(&full[st], ph, kGrWaitLimit / 16);
-                }
+            dead = __any_sync(0xffffffffu, dead);
         }
-    } else if (warp == 3) {
-        if (lane == 0) {                   // ---- this CTA's half of the token rows
-            uint32_t st = 0, ph = 0;
-            int e = 0;
-            bool dead = false;
-            for (int i = first; i < items && !dead && !*abort_flag; i += step) {
-                const GrItem it = pr_item<FW>(a, pre, i, FB, e);
-                const int half = (it.cnt + 31) / 32 * 16, nb = (half + 31) / 32;
-                for (int kb = 0; kb < nkb; ++kb) {
-                    if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { pr_timeout(abort_flag); dead = true; break; }
+        // the signals of the last MMAs have arrived before the block ends
+        for (int j = 0; j < kPrStages && !*abort_flag; ++j) {
+            mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit);
+            if (++st == kPrStages) { st = 0; ph ^= 1u; }
+        }
+        // after a time-out: nothing may still be copying into this block's memory when it ends
+        if (*abort_flag && rank == 0)
+            for (int j = 0; j < kPrStages; ++j) {
+                if (st == 0) { st = kPrStages; ph ^= 1u; }
+                --st;
+                mbar_wait(&full[st], ph, kGrWaitLimit / 16);
+            }
+    } else if (warp == 3) {                // ---- this CTA's half of the token rows
+        const bool leader = tc5::elect_one();
+        uint32_t st = 0, ph = 0;
+        int e = 0;
+        bool dead = false;
+        for (int i = first; i < items && !dead && !*abort_flag; i += step) {
+            const GrItem it = pr_item(a, pre, i, FB, fw, e);
+            const int half = (it.cnt + 31) / 32 * 16, nb = (half + 31) / 32;
+            for (int kb = 0; kb < nkb; ++kb) {
+                if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { pr_timeout(abort_flag); dead = true; break; }
+                if (leader) {
                     const uint32_t bar = tc5::map_rank(smem_u32(&full[st]), 0);
                     for (int b = 0; b < nb; ++b)
                         tc5::tma2_load_2d(smem + st * kPrStageBytes + kPrHalf + b * 4096, &tm_x, kb * 64, it.p0 + rank * half + b * 32, bar);
-                    if (++st == kPrStages) { st = 0; ph ^= 1u; }
                 }
+                if (++st == kPrStages) { st = 0; ph ^= 1u; }
             }
+            dead = __any_sync(0xffffffffu, dead);
         }
-    } else if (warp == 1) {
-        if (rank == 0 && lane == 0) {      // ---- MMA issue for the pair
+    } else if (warp == 1) {                // ---- MMA issue for the pair
+        if (rank == 0) {
+            const bool leader = tc5::elect_one();
             uint32_t st = 0, ph = 0, tl = 0;
             int e = 0;
             bool dead = false;
             constexpr uint32_t ab = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
             const uint64_t d0 = tc5::desc_sw128(smem_u32(smem));
             for (int i = first; i < items && !dead && !*abort_flag; i += step, ++tl) {
-                const GrItem it = pr_item<FW>(a, pre, i, FB, e);
+                const GrItem it = pr_item(a, pre, i, FB, fw, e);
                 const uint32_t buf = tl & 1u;
                 if (!tc5::wait_cluster(&acc_empty[buf], ((tl >> 1) & 1u) ^ 1u, kGrWaitLimit)) { pr_timeout(abort_flag); break; }
                 tc5::fence_after();
@@ -159,17 +164,19 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
                 for (int kb = 0; kb < nkb; ++kb) {
                     if (!tc5::wait_cluster(&full[st], ph, kGrWaitLimit)) { pr_timeout(abort_flag); dead = true; break; }
                     tc5::fence_after();
-                    const uint64_t ad = d0 + (uint64_t)(st * (uint32_t)(kPrStageBytes >> 4));
-                    const uint64_t bd = ad + (uint64_t)(kPrHalf >> 4);
+                    if (leader) {
+                        const uint64_t ad = d0 + (uint64_t)(st * (uint32_t)(kPrStageBytes >> 4));
+                        const uint64_t bd = ad + (uint64_t)(kPrHalf >> 4);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        tc5::mma2_f16_ss(tmem + buf * kPrNT, ad + (uint64_t)(k * 2), bd + (uint64_t)(k * 2), idesc, acc);
-                        acc = 1u;
+                        for (int k = 0; k < 4; ++k)
+                            tc5::mma2_f16_ss(tmem + buf * kPrNT, ad + (uint64_t)(k * 2), bd + (uint64_t)(k * 2), idesc, k ? 1u : acc);
+                        tc5::commit2(&empty[st]);
                     }
-                    tc5::commit2(&empty[st]);
+                    acc = 1u;
                     if (++st == kPrStages) { st = 0; ph ^= 1u; }
                 }
-                if (!dead) tc5::commit2(&acc_full[buf]);
+                dead = __any_sync(0xffffffffu, dead);
+                if (!dead && leader) tc5::commit2(&acc_full[buf]);
             }
         }
     } else if (warp >= 4) {                // ---- epilogue: this thread's TMEM lane = weight row of this CTA
@@ -179,18 +186,15 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
         Y* y = reinterpret_cast<Y*>(a.y);
         uint32_t xb = 0;
         for (int i = first; i < items; i += step, ++tl) {
-            const GrItem it = pr_item<FW>(a, pre, i, FB, e);
+            const GrItem it = pr_item(a, pre, i, FB, fw, e);
             const uint32_t buf = tl & 1u;
             // all four warps must agree to go on: they meet at a block barrier in the loop below
             int ok = *abort_flag ? 0 : (int)mbar_wait(&acc_full[buf], (tl >> 1) & 1u, kGrWaitLimit);
             if (!ok) pr_timeout(abort_flag);
-            if (GU) {
-                asm volatile("{\n\t.reg .pred p, r;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred r, 1, 128, p;\n\tselp.u32 %0, 1, 0, r;\n\t}" : "=r"(ok) : "r"(ok) : "memory");
-            }
+            if (GU) ok = epilogue_agree(ok);
             if (!ok) break;
             tc5::fence_after();
-            const int f = it.f0 + fr + (GU ? (row & 63) : row);
-            const bool have = f < a.N;
+            const int f = it.f0 + fr + (GU ? row & 63 : row);
             for (int c0 = 0; c0 < it.cnt; c0 += 32) {
                 uint32_t v[32];
                 tc5::tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + buf * kPrNT + (uint32_t)c0, v);
@@ -230,15 +234,15 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
 #pragma unroll
                     for (int k = 0; k < NC / 8; ++k) {
                         const int c = k * 8 + (lane >> 2);
-                        const uint4 w = *reinterpret_cast<const uint4*>(turn + c * 32 + (lane & 3) * 8);
+                        const uint4 o8 = *reinterpret_cast<const uint4*>(turn + c * 32 + (lane & 3) * 8);
                         if (f8 < a.N && ((live >> (cb + c)) & 1u))
-                            *reinterpret_cast<uint4*>(y + (int64_t)(it.p0 + c0 + cb + c) * a.N + f8) = w;
+                            *reinterpret_cast<uint4*>(y + (int64_t)(it.p0 + c0 + cb + c) * a.N + f8) = o8;
                     }
                     __syncwarp();
                 } else {
 #pragma unroll
                     for (int j = 0; j < NC; ++j)
-                        if (have && ((live >> (cb + j)) & 1u)) o[(int64_t)(cb + j) * a.N] = GU ? h_from_f<Y>(d[j]) : from_f<Y>(d[j]);
+                        if (f < a.N && ((live >> (cb + j)) & 1u)) o[(int64_t)(cb + j) * a.N] = GU ? h_from_f<Y>(d[j]) : from_f<Y>(d[j]);
                 }
             }
             tc5::fence_before();
@@ -298,7 +302,7 @@ int run_pair(const GroupedArgs& a, void* scratch, cudaStream_t s) {
     }
     CUtensorMap tw, tw2, tx;
     constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
-    if (!encode(&tw, a.w, bf, a.K, a.N, a.E, 64) || (GU && !encode(&tw2, a.w2, bf, a.K, a.N, a.E, 64)) ||
+    if (!encode(&tw, a.w, bf, a.K, a.N, a.E, GU ? 64 : 128) || (GU && !encode(&tw2, a.w2, bf, a.K, a.N, a.E, 64)) ||
         !encode(&tx, sorted, bf, a.K, a.rows ? a.P : a.n, 0, 32))
         return GSB_ERR_CUDA;
     const int64_t pairs = items < sms / 2 ? items : sms / 2;

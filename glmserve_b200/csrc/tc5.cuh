@@ -7,6 +7,15 @@
 namespace gsb {
 namespace tc5 {
 
+// One lane of the (converged) warp, the same one every time.  The roles that issue TMA copies and MMAs run with all 32
+// lanes and let this one issue: descriptors and addresses then are the same in every lane and stay in uniform registers.
+// With one lane running the loop alone each instruction first moves its operands there (110 cycles an MMA).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t pred;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(pred));
+    return pred != 0;
+}
+
 __device__ __forceinline__ void tmem_alloc(uint32_t* smem_dst, uint32_t ncols) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(smem_dst)), "r"(ncols) : "memory");
 }
