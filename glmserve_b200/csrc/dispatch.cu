@@ -18,6 +18,8 @@ __global__ void __launch_bounds__(kDispWarps * 32)
 dispatch_kernel(const int* __restrict__ topk_ids, int P, int topk, int E,
                 int* __restrict__ expert_offsets, int* __restrict__ sorted_token_ids,
                 int* __restrict__ sorted_row, int* __restrict__ slot_pos) {
+    // (a no-op unless the next launch asks for programmatic serialization)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ int smem[];
     dispatch_block(topk_ids, P, topk, E, expert_offsets, sorted_token_ids, sorted_row, slot_pos, smem);
 }
@@ -62,6 +64,8 @@ __global__ void __launch_bounds__(kDispWarps * 32)
 dispatch_scatter_kernel(const int* __restrict__ topk_ids, int P, int topk, int E, const int* __restrict__ blk,
                         int* __restrict__ sorted_token_ids, int* __restrict__ sorted_row,
                         int* __restrict__ slot_pos) {
+    // (a no-op unless the next launch asks for programmatic serialization)
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     extern __shared__ int smem[];
     const int b0 = blockIdx.x * kDispBlockSlots, b1 = min(P, b0 + kDispBlockSlots);
     dispatch_hist(topk_ids, b0, b1, E, smem);

@@ -78,7 +78,10 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
         *abort_flag = 0;
         fence_barrier_init();
     }
+    if (warp == 0 && lane == 0) { tc5::prefetch_map(&tm_w); if (GU) tc5::prefetch_map(&tm_w2); }
     if (warp == 2) { tc5::tmem_alloc(tmem_slot, 2 * kNT); tc5::tmem_relinquish(); }
+    pdl_trigger();
+    pdl_wait();
     int descending = (smem_u32(smem) & 1023u) != 0;    // (the swizzled tiles need a 1 KiB boundary: as good as no list)
     descending |= seg_scan<kNT>(a.offsets, a.E, a.P, pre, reinterpret_cast<int*>(s_xch));
     tc5::fence_before();
@@ -279,8 +282,7 @@ int run_grouped(const GroupedArgs& a, cudaStream_t s) {
     constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
     if (!encode(&tw, a.w, bf, a.K, a.N, a.E, 32) || (GU && !encode(&tw2, a.w2, bf, a.K, a.N, a.E, 32))) return GSB_ERR_CUDA;
     const int grid = (int)(items < sms ? items : sms);
-    kernel<<<grid, kGrThreads, kGrSmem, s>>>(a, tw, GU ? tw2 : tw);
-    return launch_status();
+    return launch_after(kernel, dim3(grid), kGrThreads, kGrSmem, 1, s, a, tw, GU ? tw2 : tw);
 }
 
 template <typename T>
@@ -302,6 +304,8 @@ __global__ void __launch_bounds__(256)
 combine16_kernel(const float* __restrict__ y, const int* __restrict__ ids, const int* __restrict__ slot_pos,
                  const float* __restrict__ w, int topk, int H, int E, O* __restrict__ out) {
     const int64_t t = blockIdx.x;
+    pdl_trigger();
+    pdl_wait();
     for (int c = (blockIdx.y * 256 + threadIdx.x) * 4; c < H; c += gridDim.y * 1024) {   // H is a multiple of 8
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
         for (int k = 0; k < topk; ++k) {
@@ -320,8 +324,7 @@ combine16_kernel(const float* __restrict__ y, const int* __restrict__ ids, const
 template <typename O>
 int run_combine16(const float* y, const int* ids, const int* slot_pos, const float* w, int n, int topk, int H, int E,
                   void* out, cudaStream_t s) {
-    combine16_kernel<O><<<dim3(n, (H + 1023) / 1024), 256, 0, s>>>(y, ids, slot_pos, w, topk, H, E, reinterpret_cast<O*>(out));
-    return launch_status();
+    return launch_after(combine16_kernel<O>, dim3(n, (H + 1023) / 1024), 256, 0, 1, s, y, ids, slot_pos, w, topk, H, E, reinterpret_cast<O*>(out));
 }
 
 // Scratch of the FFN; every buffer starts on a 256-byte boundary.

@@ -77,6 +77,9 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
         *abort_flag = 0;
         fence_barrier_init();
     }
+    if (warp == 0 && lane == 0) { tc5::prefetch_map(&tm_w); tc5::prefetch_map(&tm_x); if (GU) tc5::prefetch_map(&tm_w2); }
+    pdl_trigger();
+    pdl_wait();
     int descending = (smem_u32(smem) & 1023u) != 0;
     descending |= seg_scan<kPrNT>(a.offsets, a.E, a.P, pre, reinterpret_cast<int*>(s_xch));
     descending = __syncthreads_or(descending);
@@ -261,6 +264,8 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
 __global__ void __launch_bounds__(256)
 gather_rows_kernel(const uint4* __restrict__ x, const int* __restrict__ rows, const int* __restrict__ offsets, int n, int P, int K8,
                    int E, uint4* __restrict__ out) {
+    pdl_trigger();
+    pdl_wait();
     const int end = seg_bound(offsets, E, P);
     const int64_t p = (int64_t)blockIdx.x * 2 + (threadIdx.x >> 7);
     if (p >= end) return;
@@ -296,8 +301,9 @@ int run_pair(const GroupedArgs& a, void* scratch, cudaStream_t s) {
     if (items + sms >= (int64_t)1 << 31) return GSB_ERR_TOO_LARGE;
     const void* sorted = a.x;
     if (a.rows) {
-        gather_rows_kernel<<<(unsigned)((a.P + 1) / 2), 256, 0, s>>>(reinterpret_cast<const uint4*>(a.x), a.rows, a.offsets, a.n, a.P, a.K / 8, a.E,
-                                                      reinterpret_cast<uint4*>(scratch));
+        const int st = launch_after(gather_rows_kernel, dim3((unsigned)((a.P + 1) / 2)), 256, 0, 1, s, reinterpret_cast<const uint4*>(a.x),
+                                    a.rows, a.offsets, a.n, a.P, a.K / 8, a.E, reinterpret_cast<uint4*>(scratch));
+        if (st) return st;
         sorted = scratch;
     }
     CUtensorMap tw, tw2, tx;
@@ -306,13 +312,7 @@ int run_pair(const GroupedArgs& a, void* scratch, cudaStream_t s) {
         !encode(&tx, sorted, bf, a.K, a.rows ? a.P : a.n, 0, 32))
         return GSB_ERR_CUDA;
     const int64_t pairs = items < sms / 2 ? items : sms / 2;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)(pairs * 2)); cfg.blockDim = dim3(kPrThreads); cfg.dynamicSmemBytes = kPrSmem; cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = 2; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-    cfg.attrs = at; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, a, tw, GU ? tw2 : tw, tx, a.N % 8 == 0 && !misaligned(a.y, 16)) == cudaSuccess ? GSB_OK : GSB_ERR_LAUNCH;
+    return launch_after(kernel, dim3((unsigned)(pairs * 2)), kPrThreads, kPrSmem, 2, s, a, tw, GU ? tw2 : tw, tx, (int)(a.N % 8 == 0 && !misaligned(a.y, 16)));
 }
 
 template <typename T>

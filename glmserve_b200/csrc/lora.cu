@@ -66,7 +66,7 @@ lora_shrink_kernel(const LoraArgs a) {
     extern __shared__ float s_red[];                  // [warps][16 * MT ranks][8 * NTK rows]
     __shared__ int pre[kMaxE + 4], wsum[8];
     constexpr int RT = 16 * MT, TT = 8, NTK = 1;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    pdl_trigger();    // (an ordinary launch: what the kernels ahead wrote is there, for the second launch too)
     int descending = seg_scan<TT>(a.offsets, a.nA, a.P, pre, wsum);
     descending = __syncthreads_or(descending);
     const LoraTile tile = lora_tile<TT>(a, pre, blockIdx.x, descending);
@@ -154,7 +154,7 @@ lora_shrink_wide_kernel(const LoraArgs a) {
     extern __shared__ __align__(128) uint8_t s_ring[];
     __shared__ int pre[kMaxE + 4], wsum[8];
     constexpr int RT = 16 * MT, SB = wd_stage_bytes<MT>();
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    pdl_trigger();    // (an ordinary launch: what the kernels ahead wrote is there, for the second launch too)
     int descending = seg_scan<kWdRows>(a.offsets, a.nA, a.P, pre, wsum);
     descending = __syncthreads_or(descending);
     const LoraTile tile = lora_tile<kWdRows>(a, pre, blockIdx.x, descending);
@@ -396,7 +396,7 @@ lora_expand_kernel(const LoraArgs a, int feats, int vec_b, int vec_y) {
     int f0 = blockIdx.y * feats + warp * 32;
     Ahead q0;
     load(q0, f0);                                        // B and y do not wait for the first launch
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // v comes from it
+    pdl_wait();                                          // v comes from it
     // v of this tile: eight lanes a row, each every eighth run of two ranks
     {
         const int c = threadIdx.x >> 3, l8 = threadIdx.x & 7;
@@ -489,13 +489,7 @@ int run_expand(const LoraArgs& a, cudaStream_t s) {
     per = per < 1 ? 1 : per > passes ? passes : per;
     const int vec_b = a.R % 4 == 0 && !misaligned(a.B, 8);
     const int vec_y = a.N % (16 / (int)sizeof(Y)) == 0 && !misaligned(a.y, 16);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(tiles, (passes + per - 1) / per); cfg.blockDim = dim3(256); cfg.dynamicSmemBytes = smem; cfg.stream = s;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at; cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, a, per * 256, vec_b, vec_y) == cudaSuccess ? GSB_OK : GSB_ERR_LAUNCH;
+    return launch_after(kernel, dim3(tiles, (passes + per - 1) / per), 256, smem, 1, s, a, per * 256, vec_b, vec_y);
 }
 
 template <typename T, typename Y>

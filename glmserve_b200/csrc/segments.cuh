@@ -71,6 +71,26 @@ inline int sm_count_of(int dev) {
     return v;
 }
 
+// Programmatic dependent launch: a kernel started with launch_after() may begin before the one ahead of it in the stream
+// has ended, once all of that one's blocks have called pdl_trigger(); it touches nothing that another kernel writes, or
+// still reads, before pdl_wait(), which returns when the kernel ahead is complete.  Every kernel here waits, so what a
+// kernel two places ahead wrote is there as well.
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename K, typename... A>
+inline int launch_after(K kernel, dim3 grid, int threads, size_t smem, int cluster, cudaStream_t s, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid; cfg.blockDim = dim3((unsigned)threads); cfg.dynamicSmemBytes = smem; cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)cluster; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    cfg.attrs = at; cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? GSB_OK : GSB_ERR_LAUNCH;
+}
+
 inline bool misaligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a != 0; }
 
 }  // namespace gsb
