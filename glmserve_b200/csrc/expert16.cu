@@ -425,6 +425,6 @@ extern "C" int gsb_operators16_status(void) {
     const int zero = 0;
     if (cudaDeviceSynchronize() != cudaSuccess || cudaMemcpyFromSymbol(&st, g_op16_status, sizeof(int)) != cudaSuccess) return GSB_ERR_CUDA;
     if (st && cudaMemcpyToSymbol(g_op16_status, &zero, sizeof(int)) != cudaSuccess) return GSB_ERR_CUDA;
-    const int pair = take_pair_status();
-    return st ? st : pair;
+    const int pair = take_pair_status(), lora = take_lora_status();
+    return st ? st : pair ? pair : lora;
 }

@@ -44,35 +44,11 @@ __device__ __forceinline__ int epilogue_agree(int ok) {
     return all;
 }
 
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-inline EncodeTiledFn encode_fn() {
-    static const EncodeTiledFn fn = [] {
-        void* p = nullptr;
-        cudaDriverEntryPointQueryResult q;
-        const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-                        q == cudaDriverEntryPointSuccess;
-        return ok ? reinterpret_cast<EncodeTiledFn>(p) : nullptr;
-    }();
-    return fn;
-}
-
-// [d2, d1, d0] row-major 16-bit tensor (d2 = 0: two dims), boxes of 64 columns x box_rows rows, 128-byte swizzle.
-inline bool encode(CUtensorMap* m, const void* base, bool bf16, uint64_t d0, uint64_t d1, uint64_t d2, uint32_t box_rows) {
-    EncodeTiledFn fn = encode_fn();
-    if (!fn) return false;
-    const cuuint64_t dims[3] = {d0, d1, d2}, strides[2] = {d0 * 2, d0 * d1 * 2};
-    const cuuint32_t box[3] = {64, box_rows, 1}, estr[3] = {1, 1, 1};
-    return fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, d2 ? 3 : 2, const_cast<void*>(base),
-              dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 // The two kernels; types as in gsb_grouped_gemm (a.w2 given: SwiGLU of two products, y of x's type).
 int launch_grouped_split(const GroupedArgs& a, int type, int y_type, cudaStream_t s);
-int take_pair_status();      // status word of the pair kernel, cleared
+// status words of the kernels in the other files, cleared
+int take_pair_status();
+int take_lora_status();
 // scratch (16-byte aligned, grouped_pair_scratch_bytes): a copy of the rows in expert order, used when a.rows is given
 size_t grouped_pair_scratch_bytes(int P, int K);
 int launch_grouped_pair(const GroupedArgs& a, int type, int y_type, void* scratch, cudaStream_t s);

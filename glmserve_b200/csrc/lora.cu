@@ -5,8 +5,11 @@
 // Both are bound by those bytes; the tensor cores only keep the arithmetic out of the way, so mma.sync fed straight from
 // global memory does: every lane loads 16 (B: 8) contiguous bytes of a row and takes them as its k positions in the
 // fragments of BOTH operands - a sum does not care in which order k runs.
+#include <type_traits>
+
 #include "launchers.cuh"
 #include "segments.cuh"
+#include "tc5.cuh"
 
 namespace gsb {
 
@@ -27,6 +30,8 @@ constexpr int kShWarps = 8;
 __device__ __forceinline__ int rank_of(const LoraArgs& a, int ad) {
     return a.ranks ? min(max(__ldg(a.ranks + ad), 0), a.R) : a.R;
 }
+
+constexpr int kMaxRank = 256, kMaxSplit = 8;
 
 struct LoraTile { int ad, p0, cnt; };
 
@@ -253,6 +258,12 @@ template <typename T> struct Split;      // v as the sum of N numbers of type T
 template <> struct Split<__nv_bfloat16> { static constexpr int N = 3; static constexpr bool scaled = false; };
 template <> struct Split<__half> { static constexpr int N = 2; static constexpr bool scaled = true; };
 
+// The power of two that lifts `top` into [2^14, 2^15), kept where it and its inverse are normal; 0 for zero and infinity.
+__device__ __forceinline__ int row_exponent(float top) {
+    const int ex = 14 - ((int)((__float_as_uint(top) >> 23) & 0xff) - 127);
+    return top > 0.f && top < __int_as_float(0x7f800000) ? min(max(ex, -126), 126) : 0;
+}
+
 template <typename T> __device__ __forceinline__ uint32_t pack2(T a, T b) {
     const unsigned short x = *reinterpret_cast<const unsigned short*>(&a), y = *reinterpret_cast<const unsigned short*>(&b);
     return (uint32_t)x | ((uint32_t)y << 16);
@@ -305,6 +316,65 @@ __device__ __forceinline__ void add_store8(Y* p, int have, bool vec, const Raw8<
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         if (i < have) p[i] = from_f<Y>(v[i]);
+}
+
+// The parts of v[p, r] added in order, all loads in flight at once.
+__device__ __forceinline__ float sum_parts(const LoraArgs& a, int p, int r) {
+    const float* q0 = a.part + (int64_t)p * a.R + r;
+    const int64_t step = (int64_t)a.P * a.R;
+    float v[kMaxSplit], s = 0.f;
+#pragma unroll
+    for (int q = 0; q < kMaxSplit; ++q) v[q] = q < a.S ? __ldcg(q0 + q * step) : 0.f;
+#pragma unroll
+    for (int q = 0; q < kMaxSplit; ++q) s += v[q];
+    return s;
+}
+
+// v of a tile into shared memory as A fragments ([row tile of 16][16 ranks][part][lane]), eight lanes a row, each every
+// eighth run of two ranks; up to 16 * KG ranks (0: any number, read twice where a row is scaled).
+template <typename T, int MT, int KG>
+__device__ __forceinline__ void stage_v(const LoraArgs& a, const LoraTile& tile, int rank, float sc, uint4* s_v, float* s_scale) {
+    constexpr int NS = Split<T>::N;
+    const int kgs = (rank + 15) / 16, l8 = threadIdx.x & 7, cr = threadIdx.x >> 3;
+    if (cr >= 16 * MT) return;                           // (whole warps: 16 rows are four)
+    auto value = [&](int r) { return cr < tile.cnt && r < rank ? sc * sum_parts(a, tile.p0 + cr, r) : 0.f; };
+    float v[KG ? 2 * KG : 2], up = 1.f;
+    if (KG) {
+#pragma unroll
+        for (int i = 0; i < KG; ++i) { v[2 * i] = value(i * 16 + l8 * 2); v[2 * i + 1] = value(i * 16 + l8 * 2 + 1); }
+    }
+    if (Split<T>::scaled) {
+        float top = 0.f;
+        if (KG) {
+#pragma unroll
+            for (int i = 0; i < 2 * KG; ++i) top = fmaxf(top, fabsf(v[i]));
+        } else {
+            for (int r = l8 * 2; r < kgs * 16; r += 16) top = fmaxf(top, fmaxf(fabsf(value(r)), fabsf(value(r + 1))));
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int ex = row_exponent(top);
+        up = __int_as_float((ex + 127) << 23);
+        if (l8 == 0) s_scale[cr] = __int_as_float((127 - ex) << 23);
+    }
+#pragma unroll
+    for (int kg = 0; kg < (KG ? KG : kMaxRank / 16); ++kg) {
+        if (kg >= kgs) break;
+        const int r = kg * 16 + l8 * 2;
+        float v0 = up * (KG ? v[KG ? 2 * kg : 0] : value(r)), v1 = up * (KG ? v[KG ? 2 * kg + 1 : 0] : value(r + 1));
+        // ranks 4 t' .. 4 t' + 3 of a group are lane t' of the quad: two in the first, two in the last register pair
+        const int tq = l8 >> 1, hi_pair = l8 & 1;
+        uint32_t* d = reinterpret_cast<uint32_t*>(s_v + (((cr >> 4) * kgs + kg) * NS) * 32 + (cr & 7) * 4 + tq) +
+                      hi_pair * 2 + ((cr >> 3) & 1);
+#pragma unroll
+        for (int u = 0; u < NS; ++u) {
+            const T p0 = from_f<T>(v0), p1 = from_f<T>(v1);
+            d[u * 128] = pack2(p0, p1);
+            // the rest; infinity and NaN have none
+            v0 = isfinite(v0) ? v0 - to_f(p0) : 0.f;
+            v1 = isfinite(v1) ? v1 - to_f(p1) : 0.f;
+        }
+    }
 }
 
 // KG = 1: at most 16 ranks, whose B values are loaded ahead together with y (0: any number of ranks, B loaded in turn).
@@ -397,53 +467,282 @@ lora_expand_kernel(const LoraArgs a, int feats, int vec_b, int vec_y) {
     Ahead q0;
     load(q0, f0);                                        // B and y do not wait for the first launch
     pdl_wait();                                          // v comes from it
-    // v of this tile: eight lanes a row, each every eighth run of two ranks
-    {
-        const int c = threadIdx.x >> 3, l8 = threadIdx.x & 7;
-        for (int c0 = 0; c0 < 16 * MT; c0 += 32) {
-            const int cr = c0 + c;
-            const bool live = cr < 16 * MT;
-            auto value = [&](int r) {
-                float s = 0.f;
-                if (live && cr < tile.cnt && r < rank)
-                    for (int q = 0; q < a.S; ++q) s += __ldcg(a.part + ((int64_t)q * a.P + tile.p0 + cr) * a.R + r);
-                return sc * s;
-            };
-            float up = 1.f;
-            if (Split<T>::scaled) {
-                float top = 0.f;
-                for (int r = l8 * 2; r < kgs * 16; r += 16) top = fmaxf(top, fmaxf(fabsf(value(r)), fabsf(value(r + 1))));
-#pragma unroll
-                for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-                // 2^(14 - exponent), kept where both it and its inverse are normal; 1 for rows of zeros or infinities
-                int ex = 14 - ((int)((__float_as_uint(top) >> 23) & 0xff) - 127);
-                ex = top > 0.f && top < __int_as_float(0x7f800000) ? min(max(ex, -126), 126) : 0;
-                up = __int_as_float((ex + 127) << 23);
-                if (live && l8 == 0) s_scale[cr] = __int_as_float((127 - ex) << 23);
-            }
-            for (int r = l8 * 2; r < kgs * 16; r += 16) {
-                float v0 = up * value(r), v1 = up * value(r + 1);
-                if (!live) break;
-                // ranks 4 t' .. 4 t' + 3 of a group are lane t' of the quad: two in the first, two in the last register pair
-                const int kg = r >> 4, tq = (r >> 2) & 3, hi_pair = (r >> 1) & 1;
-                uint32_t* d = reinterpret_cast<uint32_t*>(s_v + (((cr >> 4) * kgs + kg) * NS) * 32 + (cr & 7) * 4 + tq) +
-                              hi_pair * 2 + ((cr >> 3) & 1);
-#pragma unroll
-                for (int u = 0; u < NS; ++u) {
-                    const T p0 = from_f<T>(v0), p1 = from_f<T>(v1);
-                    d[u * 128] = pack2(p0, p1);
-                    // the rest; infinity and NaN have none
-                    v0 = isfinite(v0) ? v0 - to_f(p0) : 0.f;
-                    v1 = isfinite(v1) ? v1 - to_f(p1) : 0.f;
-                }
-            }
-        }
-    }
+    stage_v<T, MT, KG>(a, tile, rank, sc, s_v, s_scale);
     __syncthreads();
     for (; f0 < f_end; f0 += 256) {
         finish(q0, f0);
         load(q0, f0 + 256);
     }
+}
+
+// The same on tcgen05, for ranks up to 64: D[feature, row] = sum over v's parts of B[feature, :] v_part[row, :], 128
+// features (TMEM lanes) x up to 64 rows of one adapter a unit, the CTAs taking equal runs of the sequence (tile, its
+// feature blocks).  The product is nothing; what this buys is the way y is met: a lane holds one feature of every row, so
+// a warp reads and writes whole 128-byte lines straight from registers, one load, one add and one store a value, with the
+// loads of 32 rows on their way before the product is waited for.  (mma.sync's fragments are 8-byte pieces of eight rows:
+// the kernel above took 121 us for 8192 rows of 6144 at rank 64, bound by its instructions, this one EXPT_US.)
+// B comes by TMA as 128-byte rows of 64 ranks, zeros behind R; columns between an adapter's rank and the next multiple of
+// 16 are zeroed in shared memory, since v's zeros would not hide a NaN there.  Needs R % 8 == 0 and B 16-byte aligned.
+constexpr int kTcNT = 64;                  // rows per tile at most
+constexpr int kTcStages = 4;               // ring of B tiles
+constexpr int kTcABytes = 128 * 128;
+constexpr int kTcVBytes = kTcNT * 128;     // one part of v: 64 rows x 64 ranks
+constexpr int kTcGroups = 4;               // of four epilogue warps, units in turn; accumulator slots
+constexpr int kTcThreads = 128 + kTcGroups * 128;   // warps: 0 B, 1 MMA, 2 zeroes, 3 TMEM, 4-19 epilogue
+constexpr long long kTcWaitLimit = 2000000000LL;
+template <typename T> constexpr size_t tc_smem() { return (size_t)kTcStages * kTcABytes + (size_t)Split<T>::N * kTcVBytes + (kMaxE + 4) * 4 + 1280; }
+
+__device__ int g_lora_status;
+
+__device__ __forceinline__ void lora_timeout(volatile int* abort_flag) {
+    *abort_flag = 1;
+    atomicCAS(&g_lora_status, 0, GSB_ERR_TIMEOUT);
+}
+
+// v of a tile as 128-byte swizzled rows of 64 ranks, a copy per part, for 512 threads: eight a row, eight ranks each.
+template <typename T>
+__device__ __forceinline__ void stage_v_rows(const LoraArgs& a, const LoraTile& tile, int rank, int e, uint8_t* s_vp, int64_t* s_off, float* s_back) {
+    constexpr int NS = Split<T>::N;
+    const int c = e >> 3, p8 = e & 7;
+    const bool in = c < tile.cnt;
+    if (p8 == 0) {
+        const int r = in ? __ldg(a.rows + tile.p0 + c) : -1;
+        s_off[c] = r >= 0 && r < a.n ? (int64_t)r * a.N : -1;
+    }
+    const float sc = a.scales ? __ldg(a.scales + tile.ad) : 1.f;
+    float v[8], top = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int r = p8 * 8 + j;
+        v[j] = in && r < rank ? sc * sum_parts(a, tile.p0 + c, r) : 0.f;
+        top = fmaxf(top, fabsf(v[j]));
+    }
+    if (Split<T>::scaled) {
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int ex = row_exponent(top);
+        const float up = __int_as_float((ex + 127) << 23);
+        if (p8 == 0) s_back[c] = __int_as_float((127 - ex) << 23);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= up;
+    }
+#pragma unroll
+    for (int u = 0; u < NS; ++u) {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const T h0 = from_f<T>(v[2 * j]), h1 = from_f<T>(v[2 * j + 1]);
+            w[j] = pack2(h0, h1);
+            v[2 * j] = isfinite(v[2 * j]) ? v[2 * j] - to_f(h0) : 0.f;       // the rest; infinity and NaN have none
+            v[2 * j + 1] = isfinite(v[2 * j + 1]) ? v[2 * j + 1] - to_f(h1) : 0.f;
+        }
+        *reinterpret_cast<uint4*>(s_vp + u * kTcNT * 128 + c * 128 + ((p8 ^ (c & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+template <typename T, typename Y>
+__global__ void __launch_bounds__(kTcThreads, 1)
+lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b) {
+    constexpr int NS = Split<T>::N;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    uint8_t* s_vp = smem + kTcStages * kTcABytes;                       // parts of v, 128-byte swizzled rows
+    int* pre = reinterpret_cast<int*>(s_vp + NS * kTcVBytes);
+    uint64_t* b_full = reinterpret_cast<uint64_t*>(pre + kMaxE + 4);    // TMA -> zeroing warp
+    uint64_t* b_ready = b_full + kTcStages;                            // zeroing warp -> MMA
+    uint64_t* b_empty = b_ready + kTcStages;                           // MMA -> TMA
+    uint64_t* acc_full = b_empty + kTcStages;                          // MMA -> epilogue group
+    uint64_t* acc_empty = acc_full + kTcGroups;
+    uint64_t* v_full = acc_empty + kTcGroups;                          // epilogue warps -> MMA: v of the next tile is there
+    int64_t* s_off = reinterpret_cast<int64_t*>(v_full + 1);           // [64] where a row of y begins (elements), -1: no such row
+    float* s_back = reinterpret_cast<float*>(s_off + kTcNT);           // [64] what a row's sums are multiplied by
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_back + kTcNT);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* wsum = reinterpret_cast<int*>(tmem_slot + 2);                 // [8]
+
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (tid == 0) {
+        for (int i = 0; i < kTcStages; ++i) { mbar_init(&b_full[i], 1); mbar_init(&b_ready[i], 1); mbar_init(&b_empty[i], 1); }
+        for (int i = 0; i < kTcGroups; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 4); }
+        mbar_init(v_full, 4 * kTcGroups);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 3) { tc5::tmem_alloc(tmem_slot, kTcGroups * kTcNT); tc5::tmem_relinquish(); }
+    int descending = (smem_u32(smem) & 1023u) != 0;
+    descending |= seg_scan<kTcNT>(a.offsets, a.nA, a.P, pre, wsum);
+    tc5::fence_before();
+    descending = __syncthreads_or(descending);
+    tc5::fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int FB = (a.N + 127) / 128;
+    const int units = descending ? 0 : pre[a.nA] * FB;                  // (checked to fit by the host)
+    const int u_beg = (int)((int64_t)units * blockIdx.x / gridDim.x), u_end = (int)((int64_t)units * (blockIdx.x + 1) / gridDim.x);
+
+    if (warp == 0) {                       // ---- B tiles
+        const bool leader = tc5::elect_one();
+        uint32_t st = 0, ph = 0;
+        for (int u = u_beg, ti = -1; u < u_end && !*abort_flag; ++u) {
+            ti = u / FB;
+            const LoraTile tile = lora_tile<kTcNT>(a, pre, ti, 0);
+            if (!mbar_wait(&b_empty[st], ph ^ 1u, kTcWaitLimit)) { lora_timeout(abort_flag); break; }
+            if (leader) {
+                mbar_arrive_expect_tx(&b_full[st], kTcABytes);
+                tc5::tma_load_3d(smem + st * kTcABytes, &tm_b, 0, (u - ti * FB) * 128, tile.ad, &b_full[st]);
+            }
+            if (++st == kTcStages) { st = 0; ph ^= 1u; }
+        }
+        for (int j = 0; j < kTcStages && !*abort_flag; ++j) {           // the last MMAs' signals have arrived
+            mbar_wait(&b_empty[st], ph ^ 1u, kTcWaitLimit);
+            if (++st == kTcStages) { st = 0; ph ^= 1u; }
+        }
+        if (*abort_flag)                   // after a time-out: nothing may still be copying when the block ends
+            for (int j = 0; j < kTcStages; ++j) {
+                if (st == 0) { st = kTcStages; ph ^= 1u; }
+                --st;
+                mbar_wait(&b_full[st], ph, kTcWaitLimit / 16);
+            }
+    } else if (warp == 2) {                // ---- zeroes between an adapter's rank and the next multiple of 16
+        uint32_t st = 0, ph = 0;
+        for (int u = u_beg; u < u_end && !*abort_flag; ++u) {
+            const int rank = rank_of(a, lora_tile<kTcNT>(a, pre, u / FB, 0).ad);
+            if (!mbar_wait(&b_full[st], ph, kTcWaitLimit)) { lora_timeout(abort_flag); break; }
+            if (rank & 15) {
+                for (int f = lane; f < 128; f += 32)
+                    for (int r = rank; r < ((rank + 15) & ~15); ++r)    // piece c of row f lies at c ^ f % 8
+                        *reinterpret_cast<unsigned short*>(smem + st * kTcABytes + f * 128 + (((r >> 3) ^ (f & 7)) << 4) + (r & 7) * 2) = 0;
+                fence_proxy_async();
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&b_ready[st]);
+            if (++st == kTcStages) { st = 0; ph ^= 1u; }
+        }
+    } else if (warp == 1) {                // ---- MMA issue
+        const bool leader = tc5::elect_one();
+        uint32_t st = 0, ph = 0, n = 0, vph = 0;
+        constexpr uint32_t ab = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+        const uint64_t b0 = tc5::desc_sw128(smem_u32(smem)), v0 = tc5::desc_sw128(smem_u32(s_vp));
+        LoraTile tile{-1, 0, 0};
+        int kgs = 0;
+        for (int u = u_beg; u < u_end && !*abort_flag; ++u, ++n) {
+            if (u == u_beg || u % FB == 0) {
+                tile = lora_tile<kTcNT>(a, pre, u / FB, 0);
+                kgs = (rank_of(a, tile.ad) + 15) / 16;
+                if (!mbar_wait(v_full, vph, kTcWaitLimit)) { lora_timeout(abort_flag); break; }
+                vph ^= 1u;
+            }
+            const uint32_t slot = n % kTcGroups;
+            if (!mbar_wait(&b_ready[st], ph, kTcWaitLimit) || !mbar_wait(&acc_empty[slot], ((n / kTcGroups) & 1u) ^ 1u, kTcWaitLimit)) {
+                lora_timeout(abort_flag);
+                break;
+            }
+            tc5::fence_after();
+            if (leader) {
+                const uint32_t idesc = tc5::idesc_f16(ab, 128, (uint32_t)((tile.cnt + 15) & ~15));
+                const uint64_t bd = b0 + (uint64_t)(st * (uint32_t)(kTcABytes >> 4));
+                uint32_t acc = 0;
+                for (int p = NS - 1; p >= 0; --p)          // small parts first
+                    for (int k = 0; k < kgs; ++k) {
+                        tc5::mma_f16_ss(tmem + slot * kTcNT, bd + (uint64_t)(k * 2), v0 + (uint64_t)(p * (kTcVBytes >> 4) + k * 2), idesc, acc);
+                        acc = 1u;
+                    }
+                tc5::commit(&b_empty[st]);
+                tc5::commit(&acc_full[slot]);
+            }
+            if (++st == kTcStages) { st = 0; ph ^= 1u; }
+        }
+    } else if (warp >= 4) {                // ---- v of a tile, then y of this group's units
+        const int e = tid - 128, group = (warp - 4) >> 2, q = warp & 3;
+        for (int us = u_beg; us < u_end;) {                // units of one tile
+            const int ti = us / FB, ue = min(u_end, (ti + 1) * FB);
+            const LoraTile tile = lora_tile<kTcNT>(a, pre, ti, 0);
+            const int rank = rank_of(a, tile.ad);
+            if (us == u_beg) pdl_wait();
+            // every group is done with the units of the tile before, hence the MMAs with its v
+            asm volatile("barrier.cta.sync 1, %0;" ::"n"(kTcGroups * 128) : "memory");
+            stage_v_rows<T>(a, tile, rank, e, s_vp, s_off, s_back);
+            fence_proxy_async();
+            asm volatile("barrier.cta.sync 1, %0;" ::"n"(kTcGroups * 128) : "memory");
+            if (lane == 0) mbar_arrive(v_full);
+
+            // this group's units of the tile, 16 rows at a time, the next 16 rows' loads ahead of the sums of the last
+            const int chunks = (tile.cnt + 15) / 16, u0 = us + ((group - (us - u_beg)) & (kTcGroups - 1));
+            const int total = u0 < ue ? ((ue - 1 - u0) / kTcGroups + 1) * chunks : 0;
+            // rows without a gap from the first on: the common case needs no test per row
+            const uint32_t l0 = __ballot_sync(0xffffffffu, s_off[lane] >= 0), l1 = __ballot_sync(0xffffffffu, s_off[32 + lane] >= 0);
+            const int s_live = ~l0 ? __ffs(~l0) - 1 : 32 + (~l1 ? __ffs(~l1) - 1 : 32);
+            struct At { int u, c0; };
+            At next{u0, 0};
+            auto load = [&](float (&v)[16]) {
+                const int f = (next.u - ti * FB) * 128 + q * 32 + lane;
+                const Y* yf = reinterpret_cast<const Y*>(a.y) + f;
+                const bool have = f < a.N && rank > 0;
+                if (__all_sync(0xffffffffu, have) && next.c0 + 16 <= s_live) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] = to_f(__ldcs(yf + s_off[next.c0 + j]));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const int64_t o = s_off[next.c0 + j];
+                        v[j] = have && o >= 0 ? to_f(__ldcs(yf + o)) : 0.f;
+                    }
+                }
+                next.c0 += 16;
+                if (next.c0 >= tile.cnt) { next.c0 = 0; next.u += kTcGroups; }
+            };
+            At now{u0, 0};
+            auto finish = [&](const float (&v)[16]) {
+                const int n = now.u - u_beg;
+                if (now.c0 == 0) {
+                    if (*abort_flag || !mbar_wait(&acc_full[group], (n / kTcGroups) & 1u, kTcWaitLimit)) {
+                        if (!*abort_flag) lora_timeout(abort_flag);
+                    }
+                    tc5::fence_after();
+                }
+                uint32_t d[16];
+                tc5::tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(group * kTcNT + now.c0), d);
+                tc5::tmem_ld_wait();
+                const int f = (now.u - ti * FB) * 128 + q * 32 + lane;
+                Y* yf = reinterpret_cast<Y*>(a.y) + f;
+                const bool have = f < a.N && rank > 0 && !*abort_flag;
+                float s[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    s[j] = v[j] + (Split<T>::scaled ? s_back[now.c0 + j] * __uint_as_float(d[j]) : __uint_as_float(d[j]));
+                if (__all_sync(0xffffffffu, have) && now.c0 + 16 <= s_live) {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) __stcs(yf + s_off[now.c0 + j], from_f<Y>(s[j]));
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const int64_t o = s_off[now.c0 + j];
+                        if (have && o >= 0) __stcs(yf + o, from_f<Y>(s[j]));
+                    }
+                }
+                now.c0 += 16;
+                if (now.c0 >= tile.cnt) {
+                    now.c0 = 0;
+                    now.u += kTcGroups;
+                    tc5::fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&acc_empty[group]);
+                }
+            };
+            float v0[16], v1[16];
+            if (total) load(v0);
+            for (int k = 0; k < total; k += 2) {
+                if (k + 1 < total) load(v1);
+                finish(v0);
+                if (k + 1 >= total) break;
+                if (k + 2 < total) load(v0);
+                finish(v1);
+            }
+            us = ue;
+        }
+    }
+    __syncwarp();
+    tc5::fence_before();
+    __syncthreads();
+    if (warp == 3) { tc5::fence_after(); tc5::tmem_dealloc(tmem, kTcGroups * kTcNT); }
 }
 
 // How the first launch is cut: a rule on P and the number of adapters alone, because the scratch is sized by it.
@@ -453,7 +752,12 @@ inline bool lora_wide(int P, int nA) { return P > 8 * (int64_t)nA; }
 inline int lora_split(int P, int nA) {
     const int64_t tiles = (nA < P ? nA : P) + P / (lora_wide(P, nA) ? kWdRows : 8);
     const int64_t s = 296 / tiles;
-    return s < 1 ? 1 : s > 8 ? 8 : (int)s;
+    return s < 1 ? 1 : s > kMaxSplit ? kMaxSplit : (int)s;
+}
+// ... and no more than leave a warp (a block of the pipelined form) four 64-column steps.
+inline int lora_split_used(int P, int nA, int K) {
+    const int most = lora_wide(P, nA) ? K / 256 : K / 1024, s = lora_split(P, nA);
+    return most < 1 ? 1 : s < most ? s : most;
 }
 
 template <typename T, int MT>
@@ -493,17 +797,46 @@ int run_expand(const LoraArgs& a, cudaStream_t s) {
 }
 
 template <typename T, typename Y>
+int run_expand_tc(const LoraArgs& a, cudaStream_t s) {
+    auto kernel = lora_expand_tc_kernel<T, Y>;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return GSB_ERR_CUDA;
+    const int sms = sm_count_of(dev);
+    if (!sms || cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tc_smem<T>()) != cudaSuccess) return GSB_ERR_CUDA;
+    const int64_t units = ((int64_t)(a.nA < a.P ? a.nA : a.P) + a.P / kTcNT) * ((a.N + 127) / 128);
+    if (units >= (int64_t)1 << 31) return GSB_ERR_TOO_LARGE;
+    CUtensorMap tb;
+    if (!encode(&tb, a.B, std::is_same<T, __nv_bfloat16>::value, a.R, a.N, a.nA, 128)) return GSB_ERR_CUDA;
+    return launch_after(kernel, dim3((unsigned)(units < sms ? units : sms)), kTcThreads, tc_smem<T>(), 1, s, a, tb);
+}
+
+template <typename T, typename Y>
 int run_lora(const LoraArgs& a, cudaStream_t s) {
     const bool wide = lora_wide(a.P, a.nA);
     int st;
     if (wide) st = a.R <= 16 ? run_shrink_wide<T, 1>(a, s) : a.R <= 32 ? run_shrink_wide<T, 2>(a, s) : run_shrink_wide<T, 4>(a, s);
     else st = a.R <= 16 ? run_shrink<T, 1>(a, s) : a.R <= 32 ? run_shrink<T, 2>(a, s) : run_shrink<T, 4>(a, s);
     if (st) return st;
-    if (wide) return a.R <= 16 ? run_expand<T, Y, 2, 1>(a, s) : run_expand<T, Y, 2, 0>(a, s);
-    return a.R <= 16 ? run_expand<T, Y, 1, 1>(a, s) : run_expand<T, Y, 1, 0>(a, s);
+    // Measured over 16 .. 8192 rows, 1024 and 6144 features, 2 .. 32 adapters.  16-row tiles with B loaded ahead while
+    // there are few rows (rank 64, 256 rows of 1024: 11 us against 13 for 32-row tiles and 16 for tcgen05); 32-row tiles
+    // halve the reads of B above (rank 16, 8192 rows of 6144: 111 us against 135 and 120); tcgen05 where rank and output
+    // are large (rank 64, 8192 rows of 6144: 125 us against 166 and 182; rank 32: 121, 127, 136).
+    const int64_t outputs = (int64_t)a.P * a.N;
+    if (a.R > 16 && a.R <= 64 && a.R % 8 == 0 && !misaligned(a.B, 16) && outputs >= (a.R > 32 ? 6 << 20 : 24 << 20)) return run_expand_tc<T, Y>(a, s);
+    if (a.R > 64) return run_expand<T, Y, 1, 0>(a, s);
+    if (wide && a.P >= 1024) return a.R <= 16 ? run_expand<T, Y, 2, 1>(a, s) : run_expand<T, Y, 2, 0>(a, s);
+    return a.R <= 16 ? run_expand<T, Y, 1, 1>(a, s) : a.R <= 32 ? run_expand<T, Y, 1, 2>(a, s) : run_expand<T, Y, 1, 4>(a, s);
 }
 
 }  // namespace
+
+int take_lora_status() {
+    int st = 0;
+    const int zero = 0;
+    if (cudaMemcpyFromSymbol(&st, g_lora_status, sizeof(int)) != cudaSuccess) return GSB_ERR_CUDA;
+    if (st && cudaMemcpyToSymbol(g_lora_status, &zero, sizeof(int)) != cudaSuccess) return GSB_ERR_CUDA;
+    return st;
+}
 
 }  // namespace gsb
 
@@ -525,13 +858,13 @@ extern "C" int gsb_lora_add(const void* x, const void* A, const void* B, int typ
     if (misaligned(x, 16) || misaligned(A, 16) || misaligned(B, 2) || misaligned(y, y_type == GSB_TYPE_F32 ? 4 : 2) ||
         misaligned(adapter_offsets, 4) || misaligned(rows, 4) || misaligned(ranks, 4) || misaligned(scales, 4))
         return GSB_ERR_INVALID_ARG;
-    if (in % 8 || max_rank > 256 || n_adapters > 1024) return GSB_ERR_UNSUPPORTED;
+    if (in % 8 || max_rank > kMaxRank || n_adapters > 1024) return GSB_ERR_UNSUPPORTED;
     if (!scratch || misaligned(scratch, 256)) return GSB_ERR_INVALID_ARG;
     if (scratch_bytes < gsb_lora_scratch_bytes(P, max_rank, n_adapters)) return GSB_ERR_WORKSPACE;
     LoraArgs a{};
     a.x = x; a.A = A; a.B = B; a.offsets = adapter_offsets; a.rows = rows; a.ranks = ranks; a.scales = scales;
     a.n = n; a.P = P; a.K = in; a.N = out; a.nA = n_adapters; a.R = max_rank;
-    a.S = lora_split(P, n_adapters); a.part = reinterpret_cast<float*>(scratch); a.y = y;
+    a.S = lora_split_used(P, n_adapters, in); a.part = reinterpret_cast<float*>(scratch); a.y = y;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if (type == GSB_TYPE_BF16)
         return y_type == GSB_TYPE_F32 ? run_lora<__nv_bfloat16, float>(a, s) : run_lora<__nv_bfloat16, __nv_bfloat16>(a, s);
