@@ -103,30 +103,31 @@ def moe_expert_ffn(x, topk_ids, topk_w, gate_w, up_w, down_w):
 
 
 _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_16BIT = (torch.bfloat16, torch.float16)
 
 
 _HERE = contextlib.nullcontext()
 
 
-def _device_of(x):
-    """Context in which x's device is the current one (nothing to do where it is already)."""
-    return _HERE if x.get_device() == torch.cuda.current_device() else torch.cuda.device(x.device)
+def _device(dev):
+    """Context in which device `dev` is the current one (nothing to do where it is already)."""
+    return _HERE if dev == torch.cuda.current_device() else torch.cuda.device(dev)
 
 
-def _raw_stream(x):
-    """Handle of torch's current stream on x's device; torch.cuda.current_stream() builds an object around it, which
+def _raw_stream(dev):
+    """Handle of torch's current stream on device `dev`; torch.cuda.current_stream() builds an object around it, which
     takes longer than a small call's kernel launch."""
-    return torch._C._cuda_getCurrentRawStream(x.get_device())
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
-def _need16(x, *named):
-    """x: a bf16 or fp16 CUDA tensor; (t, dtype, dims, name) the others, all on x's device."""
-    if not x.is_cuda or x.dtype not in (torch.bfloat16, torch.float16) or not x.is_contiguous() or x.dim() != 2:
-        raise ValueError("x: expected a contiguous 2-D CUDA tensor of torch.bfloat16 or torch.float16")
-    dev = x.get_device()
-    for t, dtype, dims, name in named:
-        if t is not None and (t.dtype != dtype or t.dim() != dims or t.get_device() != dev or not t.is_contiguous()):
-            raise ValueError(f"{name}: expected a contiguous {dims}-D tensor of {dtype} on {x.device}")
+def _is16(x, dev, *named):
+    """Whether x is a contiguous 2-D bf16/fp16 CUDA tensor and every (t, dtype, dims) lies likewise on its device."""
+    if dev < 0 or x.dim() != 2 or not x.is_contiguous() or x.dtype not in _16BIT:
+        return False
+    for t, dtype, dims in named:
+        if t is not None and (t.dtype is not dtype or t.dim() != dims or t.get_device() != dev or not t.is_contiguous()):
+            return False
+    return True
 
 
 def _out16(out, shape, x, out_dtype, name="out"):
@@ -147,7 +148,10 @@ def grouped_gemm(x, w, expert_offsets, rows=None, out=None, out_dtype=None):
     expert_offsets int32 [E+1] and rows int32 [P] as ``moe_dispatch`` returns them (offsets, sorted_token_ids);
     without ``rows`` row p is x[p].  Returns y [P,N] of x's type (or float32 with ``out_dtype`` / ``out``).  Rows
     that no segment covers are left as they were in ``out``; without ``out`` their contents are undefined."""
-    _need16(x, (w, x.dtype, 3, "w"), (expert_offsets, torch.int32, 1, "expert_offsets"), (rows, torch.int32, 1, "rows"))
+    dev, dtype = x.get_device(), x.dtype
+    if not _is16(x, dev, (w, dtype, 3), (expert_offsets, torch.int32, 1), (rows, torch.int32, 1)):
+        raise ValueError("grouped_gemm: expected contiguous tensors on one CUDA device: x [n,K] and w [E,N,K] of "
+                         "torch.bfloat16 or both of torch.float16, expert_offsets [E+1] and rows [P] of torch.int32")
     n, K = x.shape
     E, N, Kw = w.shape
     if Kw != K or expert_offsets.shape[0] != E + 1:
@@ -155,12 +159,12 @@ def grouped_gemm(x, w, expert_offsets, rows=None, out=None, out_dtype=None):
     P = n if rows is None else rows.shape[0]
     out = _out16(out, (P, N), x, out_dtype)
     nbytes = 0 if rows is None else lib().gsb_grouped_gemm_workspace_bytes(P, K, E)
-    with _device_of(x):
+    with _device(dev):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-        check(lib().gsb_grouped_gemm(x.data_ptr(), w.data_ptr(), _TYPE[x.dtype], expert_offsets.data_ptr(),
+        check(lib().gsb_grouped_gemm(x.data_ptr(), w.data_ptr(), _TYPE[dtype], expert_offsets.data_ptr(),
                                      None if rows is None else rows.data_ptr(), n, P, K, N, E, out.data_ptr(),
                                      _TYPE[out.dtype], None if ws is None else ws.data_ptr(), nbytes,
-                                     _raw_stream(x)), "grouped_gemm")
+                                     _raw_stream(dev)), "grouped_gemm")
     return out
 
 
@@ -168,8 +172,11 @@ def moe_expert_ffn_w16(x, topk_ids, topk_w, gate_w, up_w, down_w, out=None, out_
     """``moe_expert_ffn`` with bf16/fp16 activations and weights on the tensor cores: x [n,H], topk_ids int32 and
     topk_w float32 [n,topk], gate_w/up_w [E,I,H], down_w [E,H,I] -> out [n,H] of x's type (or float32).  A slot
     whose id is outside [0,E) adds nothing (padding, or an expert on another GPU)."""
-    _need16(x, (topk_ids, torch.int32, 2, "ids"), (topk_w, torch.float32, 2, "w"), (gate_w, x.dtype, 3, "gate_w"),
-            (up_w, x.dtype, 3, "up_w"), (down_w, x.dtype, 3, "down_w"))
+    dev, dtype = x.get_device(), x.dtype
+    if not _is16(x, dev, (topk_ids, torch.int32, 2), (topk_w, torch.float32, 2), (gate_w, dtype, 3), (up_w, dtype, 3),
+                 (down_w, dtype, 3)):
+        raise ValueError("moe_expert_ffn_w16: expected contiguous tensors on one CUDA device: x, gate_w, up_w and down_w "
+                         "of torch.bfloat16 or all of torch.float16, ids of torch.int32, w of torch.float32")
     n, H = x.shape
     E, I, _ = gate_w.shape
     topk = topk_ids.shape[1]
@@ -178,11 +185,11 @@ def moe_expert_ffn_w16(x, topk_ids, topk_w, gate_w, up_w, down_w, out=None, out_
         raise ValueError("moe_expert_ffn_w16: expected gate_w, up_w [E,I,H], down_w [E,H,I], ids and w [n,topk]")
     out = _out16(out, (n, H), x, out_dtype)
     nbytes = lib().gsb_moe_expert_ffn_w16_workspace_bytes(n, topk, H, I, E)
-    with _device_of(x):
+    with _device(dev):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
         check(lib().gsb_moe_expert_ffn_w16(x.data_ptr(), topk_ids.data_ptr(), topk_w.data_ptr(), gate_w.data_ptr(),
-                                           up_w.data_ptr(), down_w.data_ptr(), _TYPE[x.dtype], n, topk, H, I, E,
-                                           out.data_ptr(), _TYPE[out.dtype], ws.data_ptr(), nbytes, _raw_stream(x)),
+                                           up_w.data_ptr(), down_w.data_ptr(), _TYPE[dtype], n, topk, H, I, E,
+                                           out.data_ptr(), _TYPE[out.dtype], ws.data_ptr(), nbytes, _raw_stream(dev)),
               "moe_expert_ffn_w16")
     return out
 
@@ -194,8 +201,11 @@ def lora_add(y, x, A, B, adapter_offsets, rows, ranks=None, scales=None):
     (columns of B and rows of A behind an adapter's rank are not used), scales float32 [nA].  The lists come from
     ``moe_dispatch(adapter_ids[:, None], nA)``, once per batch: offsets and sorted_token_ids; an id of -1 = no
     adapter.  ``rows`` may be longer than the segments: what lies behind the last one is ignored."""
-    _need16(x, (A, x.dtype, 3, "A"), (B, x.dtype, 3, "B"), (adapter_offsets, torch.int32, 1, "adapter_offsets"),
-            (rows, torch.int32, 1, "rows"), (ranks, torch.int32, 1, "ranks"), (scales, torch.float32, 1, "scales"))
+    dev, dtype = x.get_device(), x.dtype
+    if not _is16(x, dev, (A, dtype, 3), (B, dtype, 3), (adapter_offsets, torch.int32, 1), (rows, torch.int32, 1),
+                 (ranks, torch.int32, 1), (scales, torch.float32, 1)):
+        raise ValueError("lora_add: expected contiguous tensors on one CUDA device: x, A and B of torch.bfloat16 or all of "
+                         "torch.float16, adapter_offsets, rows and ranks of torch.int32, scales of torch.float32")
     n, K = x.shape
     nA, R, _ = A.shape
     N = B.shape[1]
@@ -207,12 +217,12 @@ def lora_add(y, x, A, B, adapter_offsets, rows, ranks=None, scales=None):
         raise ValueError("y: expected the projection's result")
     _out16(y, (n, N), x, None, "y")
     nbytes = lib().gsb_lora_scratch_bytes(P, R, nA)
-    with _device_of(x):
+    with _device(dev):
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        check(lib().gsb_lora_add(x.data_ptr(), A.data_ptr(), B.data_ptr(), _TYPE[x.dtype], adapter_offsets.data_ptr(),
+        check(lib().gsb_lora_add(x.data_ptr(), A.data_ptr(), B.data_ptr(), _TYPE[dtype], adapter_offsets.data_ptr(),
                                  rows.data_ptr(), None if ranks is None else ranks.data_ptr(),
                                  None if scales is None else scales.data_ptr(), n, P, K, N, nA, R, y.data_ptr(),
-                                 _TYPE[y.dtype], scratch.data_ptr(), nbytes, _raw_stream(x)), "lora_add")
+                                 _TYPE[y.dtype], scratch.data_ptr(), nbytes, _raw_stream(dev)), "lora_add")
     return y
 
 
