@@ -23,7 +23,7 @@ namespace {
 // 32 experts of 6144 x 2048, SPLIT_US with the same items cut in two along K instead).
 constexpr int kGrThreads = 384;            // warps: 0 weights, 1 MMA, 2 TMEM, 4-7 epilogue, 8-11 token rows
 constexpr int kABytes = 128 * 128;         // at most 128 weight rows x 64 columns
-constexpr int kNT = 16;                    // token rows per item at most
+constexpr int kNT = 16;                    // token rows per item at most (seg_scan is given its logarithm, 4)
 constexpr int kBBytes = kNT * 128;
 constexpr int kKps = 2;                    // k-blocks of 64 columns per stage
 constexpr int kTokWarps = 4;
@@ -83,7 +83,7 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
     pdl_trigger();
     pdl_wait();
     int descending = (smem_u32(smem) & 1023u) != 0;    // (the swizzled tiles need a 1 KiB boundary: as good as no list)
-    descending |= seg_scan<kNT>(a.offsets, a.E, a.P, pre, reinterpret_cast<int*>(s_xch));
+    descending |= seg_scan(a.offsets, a.E, a.P, 4, pre, reinterpret_cast<int*>(s_xch));
     tc5::fence_before();
     descending = __syncthreads_or(descending);
     tc5::fence_after();
@@ -298,33 +298,110 @@ int launch_grouped(const GroupedArgs& a, int type, int y_type, void* scratch, cu
     return type == GSB_TYPE_BF16 ? run_grouped_any<__nv_bfloat16>(a, y_type, s) : run_grouped_any<__half>(a, y_type, s);
 }
 
-// out[t] = sum over k, in order, of w[t, k] * y[slot_pos[t, k]]; slots whose id is outside [0, E) add nothing.
-template <typename O>
+// Dispatch of a few slots (P <= 256): the same lists as dispatch_kernel, by counting instead of sorting - thread i finds
+// slot i's place as the slots of smaller ids plus the earlier ones of its own, thread e expert e's start.
+constexpr int kFewSlots = 256;
+__global__ void __launch_bounds__(1024)
+dispatch_few_kernel(const int* __restrict__ ids, int P, int topk, int E, int* __restrict__ offsets, int* __restrict__ tok,
+                    int* __restrict__ slot_pos) {
+    __shared__ __align__(16) int s_id[kFewSlots];
+    const int i = threadIdx.x;
+    pdl_trigger();
+    if (i < kFewSlots) {
+        const int id = i < P ? __ldg(ids + i) : -1;
+        s_id[i] = id >= 0 && id < E ? id : E;               // what is nobody's sorts behind the last expert
+    }
+    __syncthreads();
+    const int mine = i < kFewSlots ? s_id[i] : 0;
+    int below = 0, before = 0, start = 0;
+    for (int j = 0; j < P; j += 4) {
+        const int4 v = *reinterpret_cast<const int4*>(s_id + j);
+        const int w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            below += w[u] < mine;
+            before += w[u] == mine && j + u < i;
+            start += w[u] < i;
+        }
+    }
+    if (i < P && mine < E) {
+        tok[below + before] = i / topk;
+        slot_pos[i] = below + before;
+    }
+    if (i <= E) offsets[i] = start;
+    if (i == 1023 && E == 1024) {
+        int all = 0;
+        for (int j = 0; j < P; ++j) all += s_id[j] < E;
+        offsets[E] = all;
+    }
+}
+
+// out[t] = sum over k, in order, of w[t, k] * y[slot_pos[t, k]]; slots whose id is outside [0, E) add nothing.  A block
+// takes 1024 * U features of a token: where the slots' rows lie is read once, then every thread has the loads of J
+// slots on their way, U each of 16 bytes: four of one slot (16384 rows of 4096 in 50 us, the rate of a copy), or one of
+// eight slots, which spreads a few tokens over more blocks.
+template <typename O, int U>
 __global__ void __launch_bounds__(256)
 combine16_kernel(const float* __restrict__ y, const int* __restrict__ ids, const int* __restrict__ slot_pos,
                  const float* __restrict__ w, int topk, int H, int E, O* __restrict__ out) {
     const int64_t t = blockIdx.x;
+    __shared__ int s_pos[256];
+    __shared__ float s_w[256];
     pdl_trigger();
     pdl_wait();
-    for (int c = (blockIdx.y * 256 + threadIdx.x) * 4; c < H; c += gridDim.y * 1024) {   // H is a multiple of 8
-        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int k = 0; k < topk; ++k) {
-            const int id = __ldg(ids + t * topk + k);
-            if (id < 0 || id >= E) continue;
-            const float4 v = __ldg(reinterpret_cast<const float4*>(y + (int64_t)__ldg(slot_pos + t * topk + k) * H + c));
-            const float wk = __ldg(w + t * topk + k);
-            acc.x = fmaf(wk, v.x, acc.x); acc.y = fmaf(wk, v.y, acc.y);
-            acc.z = fmaf(wk, v.z, acc.z); acc.w = fmaf(wk, v.w, acc.w);
+    constexpr int J = U == 1 ? 8 : 1;
+    float4 acc[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int c0 = blockIdx.y * 1024 * U + threadIdx.x * 4;             // H is a multiple of 8
+    for (int k0 = 0; k0 < topk; k0 += 256) {
+        __syncthreads();
+        if (k0 + (int)threadIdx.x < topk) {
+            const int64_t i = t * topk + k0 + threadIdx.x;
+            const int id = __ldg(ids + i);
+            const bool have = id >= 0 && id < E;
+            s_pos[threadIdx.x] = have ? __ldg(slot_pos + i) : -1;
+            s_w[threadIdx.x] = have ? __ldg(w + i) : 0.f;
         }
-        O* o = out + t * H + c;
-        o[0] = from_f<O>(acc.x); o[1] = from_f<O>(acc.y); o[2] = from_f<O>(acc.z); o[3] = from_f<O>(acc.w);
+        __syncthreads();
+        const int kn = min(256, topk - k0);
+        for (int k = 0; k < kn; k += J) {
+            float4 v[J][U];
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const int pos = k + j < kn ? s_pos[k + j] : -1;
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+                    v[j][u] = pos >= 0 && c0 + u * 1024 < H ? __ldcs(reinterpret_cast<const float4*>(y + (int64_t)pos * H + c0 + u * 1024))
+                                                            : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                const float wk = k + j < kn ? s_w[k + j] : 0.f;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    acc[u].x = fmaf(wk, v[j][u].x, acc[u].x); acc[u].y = fmaf(wk, v[j][u].y, acc[u].y);
+                    acc[u].z = fmaf(wk, v[j][u].z, acc[u].z); acc[u].w = fmaf(wk, v[j][u].w, acc[u].w);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (c0 + u * 1024 >= H) continue;
+        __align__(16) O o[4] = {from_f<O>(acc[u].x), from_f<O>(acc[u].y), from_f<O>(acc[u].z), from_f<O>(acc[u].w)};
+        O* dst = out + t * H + c0 + u * 1024;
+        if constexpr (sizeof(O) == 4) *reinterpret_cast<float4*>(dst) = *reinterpret_cast<const float4*>(o);
+        else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(o);
     }
 }
 
 template <typename O>
 int run_combine16(const float* y, const int* ids, const int* slot_pos, const float* w, int n, int topk, int H, int E,
                   void* out, cudaStream_t s) {
-    return launch_after(combine16_kernel<O>, dim3(n, (H + 1023) / 1024), 256, 0, 1, s, y, ids, slot_pos, w, topk, H, E, reinterpret_cast<O*>(out));
+    O* o = reinterpret_cast<O*>(out);
+    if (n < 256) return launch_after(combine16_kernel<O, 1>, dim3(n, (H + 1023) / 1024), 256, 0, 1, s, y, ids, slot_pos, w, topk, H, E, o);
+    return launch_after(combine16_kernel<O, 4>, dim3(n, (H + 4095) / 4096), 256, 0, 1, s, y, ids, slot_pos, w, topk, H, E, o);
 }
 
 // Scratch of the FFN; every buffer starts on a 256-byte boundary.
@@ -403,7 +480,13 @@ extern "C" int gsb_moe_expert_ffn_w16(const void* x, const int* topk_ids, const 
     const Ffn16Ws ws = carve16(n, topk, hidden, moe_inter, E, workspace);
     if (workspace_bytes < ws.total) return GSB_ERR_WORKSPACE;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    int st = launch_dispatch(topk_ids, n, topk, E, ws.offsets, ws.tok, ws.row, ws.slot_pos, s, ws.disp);
+    int st;
+    if (n * topk <= kFewSlots) {
+        dispatch_few_kernel<<<1, 1024, 0, s>>>(topk_ids, n * topk, topk, E, ws.offsets, ws.tok, ws.slot_pos);
+        st = launch_status();
+    } else {
+        st = launch_dispatch(topk_ids, n, topk, E, ws.offsets, ws.tok, ws.row, ws.slot_pos, s, ws.disp);
+    }
     if (st) return st;
     GroupedArgs g{};
     g.x = x; g.w = gate_w; g.w2 = up_w; g.offsets = ws.offsets; g.rows = ws.tok;

@@ -54,7 +54,7 @@ __device__ __forceinline__ GrItem pr_item(const GroupedArgs& a, const int* pre, 
 template <typename T, typename Y, bool GU>
 __global__ void __launch_bounds__(kPrThreads, 1)
 grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_w2,
-                    const __grid_constant__ CUtensorMap tm_x, int vec) {
+                    const __grid_constant__ CUtensorMap tm_x, int vec, int lg) {
     extern __shared__ __align__(1024) uint8_t smem[];
     float* s_xch = reinterpret_cast<float*>(smem + kPrStages * kPrStageBytes);
     uint8_t* s_turn = smem + kPrStages * kPrStageBytes + kPrXch;
@@ -81,7 +81,7 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
     pdl_trigger();
     pdl_wait();
     int descending = (smem_u32(smem) & 1023u) != 0;
-    descending |= seg_scan<kPrNT>(a.offsets, a.E, a.P, pre, reinterpret_cast<int*>(s_xch));
+    descending |= seg_scan(a.offsets, a.E, a.P, lg, pre, reinterpret_cast<int*>(s_xch));
     descending = __syncthreads_or(descending);
     tc5::cluster_sync_all();
     if (warp == 2) { tc5::tmem_alloc2(tmem_slot, 512); tc5::tmem_relinquish2(); }
@@ -242,6 +242,10 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
                             *reinterpret_cast<uint4*>(y + (int64_t)(it.p0 + c0 + cb + c) * a.N + f8) = o8;
                     }
                     __syncwarp();
+                } else if (live == 0xffffffffu && f - lane + 32 <= a.N) {
+                    Y* oj = o + (int64_t)cb * a.N;
+#pragma unroll
+                    for (int j = 0; j < NC; ++j, oj += a.N) *oj = GU ? h_from_f<Y>(d[j]) : from_f<Y>(d[j]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < NC; ++j)
@@ -260,27 +264,28 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
     if (warp == 2) { tc5::fence_after(); tc5::tmem_dealloc2(tmem, 512); }
 }
 
-// Rows named by the list, in order: two rows a block.  Rows that do not exist are left out (their results are not stored).
+// Rows named by the list, in order: a warp takes a row, eight 16-byte loads a lane on their way.  Rows that do not exist
+// are left out (their results are not stored).
 __global__ void __launch_bounds__(256)
 gather_rows_kernel(const uint4* __restrict__ x, const int* __restrict__ rows, const int* __restrict__ offsets, int n, int P, int K8,
                    int E, uint4* __restrict__ out) {
     pdl_trigger();
     pdl_wait();
     const int end = seg_bound(offsets, E, P);
-    const int64_t p = (int64_t)blockIdx.x * 2 + (threadIdx.x >> 7);
+    const int64_t p = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (p >= end) return;
     const int r = __ldg(rows + p);
     if (r < 0 || r >= n) return;
     const uint4* src = x + (int64_t)r * K8;
     uint4* dst = out + p * K8;
-    for (int c = threadIdx.x & 127; c < K8; c += 512) {
-        uint4 v[4];
+    for (int c = threadIdx.x & 31; c < K8; c += 256) {
+        uint4 v[8];
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (c + u * 128 < K8) v[u] = __ldg(src + c + u * 128);
+        for (int u = 0; u < 8; ++u)
+            if (c + u * 32 < K8) v[u] = __ldg(src + c + u * 32);
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-            if (c + u * 128 < K8) dst[c + u * 128] = v[u];
+        for (int u = 0; u < 8; ++u)
+            if (c + u * 32 < K8) dst[c + u * 32] = v[u];
     }
 }
 
@@ -297,11 +302,17 @@ int run_pair(const GroupedArgs& a, void* scratch, cudaStream_t s) {
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPrSmem) != cudaSuccess) return GSB_ERR_CUDA;
         if (dev < 64) ready.fetch_or(1ull << dev);
     }
-    const int64_t fbs = (a.N + FW - 1) / FW, items = ((a.E < a.P ? a.E : a.P) + a.P / kPrNT) * fbs;
+    // Tiles of 256 rows, or of fewer (down to 32) where all of them still run at once: a small problem is then spread over
+    // more SMs and its epilogues are shorter (256 rows for each of 4 experts, 1024 x 1024: 12 us with 256 rows a tile, 8 with
+    // 64, 11 with 32, which take two rounds).
+    const int64_t fbs = (a.N + FW - 1) / FW, hit = a.E < a.P ? a.E : a.P;
+    int lg = 8;
+    while (lg > 5 && (hit > (a.P >> (lg - 1)) ? hit : a.P >> (lg - 1)) * fbs <= sms / 2) --lg;
+    const int64_t items = (hit + (a.P >> lg)) * fbs;
     if (items + sms >= (int64_t)1 << 31) return GSB_ERR_TOO_LARGE;
     const void* sorted = a.x;
     if (a.rows) {
-        const int st = launch_after(gather_rows_kernel, dim3((unsigned)((a.P + 1) / 2)), 256, 0, 1, s, reinterpret_cast<const uint4*>(a.x),
+        const int st = launch_after(gather_rows_kernel, dim3((unsigned)((a.P + 7) / 8)), 256, 0, 1, s, reinterpret_cast<const uint4*>(a.x),
                                     a.rows, a.offsets, a.n, a.P, a.K / 8, a.E, reinterpret_cast<uint4*>(scratch));
         if (st) return st;
         sorted = scratch;
@@ -312,7 +323,7 @@ int run_pair(const GroupedArgs& a, void* scratch, cudaStream_t s) {
         !encode(&tx, sorted, bf, a.K, a.rows ? a.P : a.n, 0, 32))
         return GSB_ERR_CUDA;
     const int64_t pairs = items < sms / 2 ? items : sms / 2;
-    return launch_after(kernel, dim3((unsigned)(pairs * 2)), kPrThreads, kPrSmem, 2, s, a, tw, GU ? tw2 : tw, tx, (int)(a.N % 8 == 0 && !misaligned(a.y, 16)));
+    return launch_after(kernel, dim3((unsigned)(pairs * 2)), kPrThreads, kPrSmem, 2, s, a, tw, GU ? tw2 : tw, tx, (int)(a.N % 8 == 0 && !misaligned(a.y, 16)), lg);
 }
 
 template <typename T>

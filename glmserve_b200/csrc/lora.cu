@@ -72,7 +72,7 @@ lora_shrink_kernel(const LoraArgs a) {
     __shared__ int pre[kMaxE + 4], wsum[8];
     constexpr int RT = 16 * MT, TT = 8, NTK = 1;
     pdl_trigger();    // (an ordinary launch: what the kernels ahead wrote is there, for the second launch too)
-    int descending = seg_scan<TT>(a.offsets, a.nA, a.P, pre, wsum);
+    int descending = seg_scan(a.offsets, a.nA, a.P, 3, pre, wsum);
     descending = __syncthreads_or(descending);
     const LoraTile tile = lora_tile<TT>(a, pre, blockIdx.x, descending);
     if (tile.ad < 0) return;
@@ -160,7 +160,7 @@ lora_shrink_wide_kernel(const LoraArgs a) {
     __shared__ int pre[kMaxE + 4], wsum[8];
     constexpr int RT = 16 * MT, SB = wd_stage_bytes<MT>();
     pdl_trigger();    // (an ordinary launch: what the kernels ahead wrote is there, for the second launch too)
-    int descending = seg_scan<kWdRows>(a.offsets, a.nA, a.P, pre, wsum);
+    int descending = seg_scan(a.offsets, a.nA, a.P, 6, pre, wsum);
     descending = __syncthreads_or(descending);
     const LoraTile tile = lora_tile<kWdRows>(a, pre, blockIdx.x, descending);
     if (tile.ad < 0) return;
@@ -385,7 +385,7 @@ lora_expand_kernel(const LoraArgs a, int feats, int vec_b, int vec_y) {
     extern __shared__ uint4 s_v[];                    // [row tile of 16][16 ranks][part][lane]: A fragments
     __shared__ int pre[kMaxE + 4], wsum[8];
     __shared__ float s_scale[16 * MT];                // what a row's sums are multiplied by at the end
-    int descending = seg_scan<16 * MT>(a.offsets, a.nA, a.P, pre, wsum);
+    int descending = seg_scan(a.offsets, a.nA, a.P, MT == 1 ? 4 : 5, pre, wsum);
     descending = __syncthreads_or(descending);
     const LoraTile tile = lora_tile<16 * MT>(a, pre, blockIdx.x, descending);
     if (tile.ad < 0) return;
@@ -569,7 +569,7 @@ lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b
     }
     if (warp == 3) { tc5::tmem_alloc(tmem_slot, kTcGroups * kTcNT); tc5::tmem_relinquish(); }
     int descending = (smem_u32(smem) & 1023u) != 0;
-    descending |= seg_scan<kTcNT>(a.offsets, a.nA, a.P, pre, wsum);
+    descending |= seg_scan(a.offsets, a.nA, a.P, 6, pre, wsum);
     tc5::fence_before();
     descending = __syncthreads_or(descending);
     tc5::fence_after();

@@ -24,10 +24,9 @@ __device__ __forceinline__ int seg_bound(const int* offsets, int e, int P) { ret
 
 constexpr int kMaxE = 1024;     // segments at most
 
-// pre[e] = tiles of at most NT rows before segment e, e = 0..E (E <= kMaxE); the first 256 threads work, all call.
+// pre[e] = tiles of at most 2^lg rows before segment e, e = 0..E (E <= kMaxE); the first 256 threads work, all call.
 // Returns non-zero in a thread that saw the list descend.  `wsum`: shared scratch of 8 ints.
-template <int NT>
-__device__ __forceinline__ int seg_scan(const int* offsets, int E, int P, int* pre, int* wsum) {
+__device__ __forceinline__ int seg_scan(const int* offsets, int E, int P, int lg, int* pre, int* wsum) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     int c[4], sum = 0, incl = 0, descending = 0;
     if (tid < 256) {
@@ -37,7 +36,7 @@ __device__ __forceinline__ int seg_scan(const int* offsets, int E, int P, int* p
             c[j] = sum;
             if (e < E) {
                 const int lo = seg_bound(offsets, e, P), hi = seg_bound(offsets, e + 1, P);
-                sum += hi > lo ? (hi - lo + NT - 1) / NT : 0;
+                sum += hi > lo ? (hi - lo + (1 << lg) - 1) >> lg : 0;
                 descending |= hi < lo;
             }
         }
