@@ -62,80 +62,83 @@ template <> __device__ __forceinline__ void mma_k16<__half>(float (&d)[4], uint3
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // ---- first launch: v ---------------------------------------------------------------------------
-// Block: up to 8 * NTK rows of one adapter x 16 * MT ranks, D[rank, row]; its eight warps and a.S blocks share the sum
-// over K (adjacent 32-column chunks go to adjacent warps).  The warps' tiles are added in shared memory in warp order,
-// the blocks' parts by the second launch in block order.
+// This warp's share of D[rank, row] for eight rows of one adapter and 16 * MT ranks from r0 on: the 32-column chunks
+// c0, c0 + stride, ... of the sum over K.
 template <typename T, int MT>
-__global__ void __launch_bounds__(kShWarps * 32)
-lora_shrink_kernel(const LoraArgs a) {
-    extern __shared__ float s_red[];                  // [warps][16 * MT ranks][8 * NTK rows]
-    __shared__ int pre[kMaxE + 4], wsum[8];
-    constexpr int RT = 16 * MT, TT = 8, NTK = 1;
-    pdl_trigger();    // (an ordinary launch: what the kernels ahead wrote is there, for the second launch too)
-    int descending = seg_scan(a.offsets, a.nA, a.P, 3, pre, wsum);
-    descending = __syncthreads_or(descending);
-    const LoraTile tile = lora_tile<TT>(a, pre, blockIdx.x, descending);
-    if (tile.ad < 0) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int r0 = blockIdx.z * RT, rank = rank_of(a, tile.ad);
-    if (r0 >= rank) return;
+__device__ __forceinline__ void shrink_sum(const LoraArgs& a, const LoraTile& tile, int rank, int r0, int c0, int stride, float (&acc)[MT][4]) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const T* A = reinterpret_cast<const T*>(a.A) + ((int64_t)tile.ad * a.R + r0) * a.K + t * 8;
-    const T* xr[NTK];
-    bool xin[NTK];
-#pragma unroll
-    for (int j = 0; j < NTK; ++j) {
-        const int c = j * 8 + g;
-        const int row = c < tile.cnt ? __ldg(a.rows + tile.p0 + c) : -1;
-        xin[j] = row >= 0 && row < a.n;
-        xr[j] = reinterpret_cast<const T*>(a.x) + (int64_t)(xin[j] ? row : 0) * a.K + t * 8;
-    }
-    float acc[MT][NTK][4] = {};
+    const int row = g < tile.cnt ? __ldg(a.rows + tile.p0 + g) : -1;
+    const bool xin = row >= 0 && row < a.n;
+    const T* xr = reinterpret_cast<const T*>(a.x) + (int64_t)(xin ? row : 0) * a.K + t * 8;
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    const int chunks = (a.K + 31) / 32, stride = kShWarps * a.S;
-    constexpr int U = MT * NTK >= 8 ? 1 : MT * NTK >= 4 ? 2 : 4;      // chunks in flight
-    for (int c0 = blockIdx.y * kShWarps + warp; c0 < chunks; c0 += stride * U) {
-        uint4 fa[U][MT][2], fx[U][NTK];
+    const int chunks = (a.K + 31) / 32;
+    constexpr int U = MT >= 4 ? 2 : 4;                 // chunks in flight
+    for (; c0 < chunks; c0 += stride * U) {
+        uint4 fa[U][MT][2], fx[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int k = (c0 + u * stride) * 32;
             const bool in = k + t * 8 < a.K;
-#pragma unroll
-            for (int j = 0; j < NTK; ++j) fx[u][j] = in && xin[j] ? __ldg(reinterpret_cast<const uint4*>(xr[j] + k)) : zero;
+            fx[u] = in && xin ? __ldg(reinterpret_cast<const uint4*>(xr + k)) : zero;
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int r = m * 16 + h * 8 + g;          // what lies behind the adapter's rank counts as zero
+                    const int r = m * 16 + h * 8 + g;  // what lies behind the adapter's rank counts as zero
                     fa[u][m][h] = in && r0 + r < rank ? __ldg(reinterpret_cast<const uint4*>(A + (int64_t)r * a.K + k)) : zero;
                 }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int j = 0; j < NTK; ++j) {
-                    mma_k16<T>(acc[m][j], fa[u][m][0].x, fa[u][m][1].x, fa[u][m][0].y, fa[u][m][1].y, fx[u][j].x, fx[u][j].y);
-                    mma_k16<T>(acc[m][j], fa[u][m][0].z, fa[u][m][1].z, fa[u][m][0].w, fa[u][m][1].w, fx[u][j].z, fx[u][j].w);
-                }
+            for (int m = 0; m < MT; ++m) {
+                mma_k16<T>(acc[m], fa[u][m][0].x, fa[u][m][1].x, fa[u][m][0].y, fa[u][m][1].y, fx[u].x, fx[u].y);
+                mma_k16<T>(acc[m], fa[u][m][0].z, fa[u][m][1].z, fa[u][m][0].w, fa[u][m][1].w, fx[u].z, fx[u].w);
+            }
     }
-    float* mine = s_red + warp * RT * TT;
+}
+
+// The warps' shares through shared memory ([warp][rank][row]), then put(row, rank, sum over the warps in order).
+template <int MT, typename F>
+__device__ __forceinline__ void shrink_add(const float (&acc)[MT][4], float* s_red, F put) {
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    constexpr int RT = 16 * MT;
+    float* mine = s_red + (threadIdx.x >> 5) * RT * 8;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int j = 0; j < NTK; ++j)
-#pragma unroll
-            for (int h = 0; h < 4; ++h)
-                mine[(m * 16 + (h >> 1) * 8 + g) * TT + j * 8 + t * 2 + (h & 1)] = acc[m][j][h];
+        for (int h = 0; h < 4; ++h) mine[(m * 16 + (h >> 1) * 8 + g) * 8 + t * 2 + (h & 1)] = acc[m][h];
     __syncthreads();
-    for (int i = threadIdx.x; i < RT * TT; i += kShWarps * 32) {
+    for (int i = threadIdx.x; i < RT * 8; i += kShWarps * 32) {
         const int c = i / RT, r = i - c * RT;
-        if (c >= tile.cnt || r0 + r >= rank) continue;
         float s = 0.f;
 #pragma unroll
-        for (int w = 0; w < kShWarps; ++w) s += s_red[(w * RT + r) * TT + c];
-        a.part[((int64_t)blockIdx.y * a.P + tile.p0 + c) * a.R + r0 + r] = s;
+        for (int w = 0; w < kShWarps; ++w) s += s_red[(w * RT + r) * 8 + c];
+        put(c, r, s);
     }
+}
+
+// Block: up to eight rows of one adapter x 16 * MT ranks; its eight warps and a.S blocks share the sum over K (adjacent
+// chunks go to adjacent warps).  The warps' tiles are added in shared memory in warp order, the blocks' parts by the
+// second launch in block order.
+template <typename T, int MT>
+__global__ void __launch_bounds__(kShWarps * 32)
+lora_shrink_kernel(const LoraArgs a) {
+    extern __shared__ float s_red[];
+    __shared__ int pre[kMaxE + 4], wsum[8];
+    pdl_trigger();    // (an ordinary launch: what the kernels ahead wrote is there, for the second launch too)
+    int descending = seg_scan(a.offsets, a.nA, a.P, 3, pre, wsum);
+    descending = __syncthreads_or(descending);
+    const LoraTile tile = lora_tile<8>(a, pre, blockIdx.x, descending);
+    if (tile.ad < 0) return;
+    const int r0 = blockIdx.z * 16 * MT, rank = rank_of(a, tile.ad);
+    if (r0 >= rank) return;
+    float acc[MT][4] = {};
+    shrink_sum<T, MT>(a, tile, rank, r0, blockIdx.y * kShWarps + (threadIdx.x >> 5), kShWarps * a.S, acc);
+    shrink_add<MT>(acc, s_red, [&](int c, int r, float s) {
+        if (c < tile.cnt && r0 + r < rank) a.part[((int64_t)blockIdx.y * a.P + tile.p0 + c) * a.R + r0 + r] = s;
+    });
 }
 
 // The same for adapters with many rows: 64 rows x 16 * MT ranks, D[row, rank], over K steps of 64 columns that 16-byte
@@ -331,13 +334,13 @@ __device__ __forceinline__ float sum_parts(const LoraArgs& a, int p, int r) {
 }
 
 // v of a tile into shared memory as A fragments ([row tile of 16][16 ranks][part][lane]), eight lanes a row, each every
-// eighth run of two ranks; up to 16 * KG ranks (0: any number, read twice where a row is scaled).
-template <typename T, int MT, int KG>
-__device__ __forceinline__ void stage_v(const LoraArgs& a, const LoraTile& tile, int rank, float sc, uint4* s_v, float* s_scale) {
+// eighth run of two ranks; up to 16 * KG ranks (0: any number, read twice where a row is scaled).  of(row, rank) is v.
+template <typename T, int MT, int KG, typename F>
+__device__ __forceinline__ void stage_v(int cnt, int rank, F of, uint4* s_v, float* s_scale) {
     constexpr int NS = Split<T>::N;
     const int kgs = (rank + 15) / 16, l8 = threadIdx.x & 7, cr = threadIdx.x >> 3;
     if (cr >= 16 * MT) return;                           // (whole warps: 16 rows are four)
-    auto value = [&](int r) { return cr < tile.cnt && r < rank ? sc * sum_parts(a, tile.p0 + cr, r) : 0.f; };
+    auto value = [&](int r) { return cr < cnt && r < rank ? of(cr, r) : 0.f; };
     float v[KG ? 2 * KG : 2], up = 1.f;
     if (KG) {
 #pragma unroll
@@ -377,34 +380,31 @@ __device__ __forceinline__ void stage_v(const LoraArgs& a, const LoraTile& tile,
     }
 }
 
-// KG = 1: at most 16 ranks, whose B values are loaded ahead together with y (0: any number of ranks, B loaded in turn).
+// One warp's way through features of a tile of 16 * MT rows, 32 at a time.  KG: groups of 16 ranks whose B values are
+// loaded ahead together with y (0: any number of ranks, B loaded in turn).
 template <typename T, typename Y, int MT, int KG>
-__global__ void __launch_bounds__(256, MT == 1 && KG == 1 ? 3 : 2)
-lora_expand_kernel(const LoraArgs a, int feats, int vec_b, int vec_y) {
-    constexpr int NS = Split<T>::N;
-    extern __shared__ uint4 s_v[];                    // [row tile of 16][16 ranks][part][lane]: A fragments
-    __shared__ int pre[kMaxE + 4], wsum[8];
-    __shared__ float s_scale[16 * MT];                // what a row's sums are multiplied by at the end
-    int descending = seg_scan(a.offsets, a.nA, a.P, MT == 1 ? 4 : 5, pre, wsum);
-    descending = __syncthreads_or(descending);
-    const LoraTile tile = lora_tile<16 * MT>(a, pre, blockIdx.x, descending);
-    if (tile.ad < 0) return;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int rank = rank_of(a, tile.ad), kgs = (rank + 15) / 16;
-    if (rank == 0) return;
-    int row[2 * MT];
-#pragma unroll
-    for (int m = 0; m < 2 * MT; ++m) {
-        const int c = m * 8 + g, r = c < tile.cnt ? __ldg(a.rows + tile.p0 + c) : -1;
-        row[m] = r < a.n ? r : -1;
-    }
-    const float sc = a.scales ? __ldg(a.scales + tile.ad) : 1.f;
-    const T* B = reinterpret_cast<const T*>(a.B) + (int64_t)tile.ad * a.N * a.R;
-    Y* y = reinterpret_cast<Y*>(a.y);
-    const int f_end = min(a.N, (int)(blockIdx.y + 1) * feats);
+struct Expand {
+    static constexpr int NS = Split<T>::N;
+    struct Ahead { Raw8<Y> y[2 * MT]; uint2 b[KG ? KG : 1][4]; };
+    const LoraArgs& a;
+    const T* B;
+    const uint4* s_v;
+    const float* s_scale;
+    int rank, kgs, f_end, row[2 * MT];
+    bool vec_b, vec_y;
 
+    __device__ __forceinline__ Expand(const LoraArgs& args, const LoraTile& tile, int rk, const uint4* v, const float* scale, int end, int flags)
+        : a(args), B(reinterpret_cast<const T*>(args.B) + (int64_t)tile.ad * args.N * args.R), s_v(v), s_scale(scale), rank(rk),
+          kgs((rk + 15) / 16), f_end(end), vec_b(flags & 1), vec_y(flags & 2) {
+#pragma unroll
+        for (int m = 0; m < 2 * MT; ++m) {
+            const int c = m * 8 + ((threadIdx.x & 31) >> 2), r = c < tile.cnt ? __ldg(a.rows + tile.p0 + c) : -1;
+            row[m] = r < a.n ? r : -1;
+        }
+    }
     // four ranks of feature n of n-tile j, as two packed pairs
-    auto load_b = [&](int f0, int kg, int j) {
+    __device__ __forceinline__ uint2 load_b(int f0, int kg, int j) const {
+        const int g = (threadIdx.x & 31) >> 2, t = threadIdx.x & 3;
         const int f = f0 + 8 * (g >> 1) + 2 * j + (g & 1), r = kg * 16 + t * 4;
         uint2 w = make_uint2(0, 0);
         if (f < a.N) {
@@ -419,20 +419,20 @@ lora_expand_kernel(const LoraArgs a, int feats, int vec_b, int vec_y) {
             }
         }
         return w;
-    };
-    struct Ahead { Raw8<Y> y[2 * MT]; uint2 b[KG ? KG : 1][4]; };
-    auto load = [&](Ahead& q, int f0) {
+    }
+    __device__ __forceinline__ void load(Ahead& q, int f0) const {
         if (f0 >= f_end) return;
 #pragma unroll
         for (int kg = 0; kg < KG; ++kg)
 #pragma unroll
             for (int j = 0; j < 4; ++j) q.b[kg][j] = kg < kgs ? load_b(f0, kg, j) : make_uint2(0, 0);
-        const int f = f0 + 8 * t;
+        const int f = f0 + 8 * (threadIdx.x & 3);
 #pragma unroll
         for (int m = 0; m < 2 * MT; ++m)
-            if (row[m] >= 0 && f < a.N) q.y[m] = load8(y + (int64_t)row[m] * a.N + f, min(8, a.N - f), vec_y);
-    };
-    auto finish = [&](const Ahead& q, int f0) {
+            if (row[m] >= 0 && f < a.N) q.y[m] = load8(reinterpret_cast<const Y*>(a.y) + (int64_t)row[m] * a.N + f, min(8, a.N - f), vec_y);
+    }
+    __device__ __forceinline__ void finish(const Ahead& q, int f0) const {
+        const int lane = threadIdx.x & 31, g = lane >> 2;
         float acc[MT][4][4] = {};
         for (int kg = 0; kg < (KG ? KG : kgs); ++kg) {
             if (kg >= kgs) break;
@@ -448,7 +448,7 @@ lora_expand_kernel(const LoraArgs a, int feats, int vec_b, int vec_y) {
                     for (int j = 0; j < 4; ++j) mma_k16<T>(acc[m][j], v.x, v.y, v.z, v.w, b[j].x, b[j].y);
                 }
         }
-        const int f = f0 + 8 * t, have = min(8, a.N - f);
+        const int f = f0 + 8 * (lane & 3), have = min(8, a.N - f);
 #pragma unroll
         for (int m = 0; m < 2 * MT; ++m) {
             if (row[m] < 0 || have <= 0) continue;
@@ -459,20 +459,82 @@ lora_expand_kernel(const LoraArgs a, int feats, int vec_b, int vec_y) {
                 d[2 * j] = back * acc[m >> 1][j][2 * (m & 1)];
                 d[2 * j + 1] = back * acc[m >> 1][j][2 * (m & 1) + 1];
             }
-            add_store8(y + (int64_t)row[m] * a.N + f, have, vec_y, q.y[m], d);
+            add_store8(reinterpret_cast<Y*>(a.y) + (int64_t)row[m] * a.N + f, have, vec_y, q.y[m], d);
         }
-    };
-
-    int f0 = blockIdx.y * feats + warp * 32;
-    Ahead q0;
-    load(q0, f0);                                        // B and y do not wait for the first launch
-    pdl_wait();                                          // v comes from it
-    stage_v<T, MT, KG>(a, tile, rank, sc, s_v, s_scale);
-    __syncthreads();
-    for (; f0 < f_end; f0 += 256) {
-        finish(q0, f0);
-        load(q0, f0 + 256);
     }
+};
+
+template <typename T, typename Y, int MT, int KG>
+__global__ void __launch_bounds__(256, MT == 1 && KG == 1 ? 3 : 2)
+lora_expand_kernel(const LoraArgs a, int feats, int flags) {
+    extern __shared__ uint4 s_v[];                    // [row tile of 16][16 ranks][part][lane]: A fragments
+    __shared__ int pre[kMaxE + 4], wsum[8];
+    __shared__ float s_scale[16 * MT];                // what a row's sums are multiplied by at the end
+    int descending = seg_scan(a.offsets, a.nA, a.P, MT == 1 ? 4 : 5, pre, wsum);
+    descending = __syncthreads_or(descending);
+    const LoraTile tile = lora_tile<16 * MT>(a, pre, blockIdx.x, descending);
+    if (tile.ad < 0) return;
+    const int rank = rank_of(a, tile.ad);
+    if (rank == 0) return;
+    const float sc = a.scales ? __ldg(a.scales + tile.ad) : 1.f;
+    const Expand<T, Y, MT, KG> ex(a, tile, rank, s_v, s_scale, min(a.N, (int)(blockIdx.y + 1) * feats), flags);
+    int f0 = blockIdx.y * feats + (threadIdx.x >> 5) * 32;
+    typename Expand<T, Y, MT, KG>::Ahead q;
+    ex.load(q, f0);                                      // B and y do not wait for the first launch
+    pdl_wait();                                          // v comes from it
+    stage_v<T, MT, KG>(tile.cnt, rank, [&](int c, int r) { return sc * sum_parts(a, tile.p0 + c, r); }, s_v, s_scale);
+    __syncthreads();
+    for (; f0 < ex.f_end; f0 += 256) {
+        ex.finish(q, f0);
+        ex.load(q, f0 + 256);
+    }
+}
+
+// ---- both sums in one launch, for few rows -------------------------------------------------------
+// A cluster of eight blocks takes eight rows of one adapter: each block an eighth of the sum over K, then, with the
+// others' parts read from their shared memory and added in rank order, an eighth of the output features.  One launch and
+// no scratch: with few rows the two-launch form waits for launches and its partial sums more than for memory.
+constexpr int kClusterBlocks = 8;
+template <typename T, typename Y, int KG>
+__global__ void __launch_bounds__(256, 2)
+lora_cluster_kernel(const LoraArgs a, int feats, int flags) {
+    constexpr int RT = 16 * KG;
+    __shared__ uint4 s_v[KG * Split<T>::N * 32];
+    __shared__ float s_red[kShWarps * RT * 8], s_part[RT * 8], s_scale[16];
+    __shared__ int pre[kMaxE + 4], wsum[8];
+    pdl_trigger();
+    pdl_wait();
+    int descending = seg_scan(a.offsets, a.nA, a.P, 3, pre, wsum);
+    descending = __syncthreads_or(descending);
+    const LoraTile tile = lora_tile<8>(a, pre, blockIdx.x / kClusterBlocks, descending);
+    const int rank = tile.ad < 0 ? 0 : rank_of(a, tile.ad), block = (int)tc5::cluster_rank(), warp = threadIdx.x >> 5;
+    if (rank == 0) return;                               // (the same for all blocks of the cluster)
+    const float sc = a.scales ? __ldg(a.scales + tile.ad) : 1.f;
+    const Expand<T, Y, 1, KG> ex(a, tile, rank, s_v, s_scale, min(a.N, (block + 1) * feats), flags);
+    int f0 = block * feats + warp * 32;
+    float acc[KG][4] = {};
+    shrink_sum<T, KG>(a, tile, rank, 0, block * kShWarps + warp, kShWarps * kClusterBlocks, acc);
+    typename Expand<T, Y, 1, KG>::Ahead q;
+    ex.load(q, f0);                                      // on its way while the parts of v are put together
+    shrink_add<KG>(acc, s_red, [&](int c, int r, float s) { s_part[r * 8 + c] = s; });
+    tc5::cluster_sync_all();
+    const uint32_t part = smem_u32(s_part);
+    stage_v<T, 1, KG>(tile.cnt, rank, [&](int c, int r) {
+        float v[kClusterBlocks], s = 0.f;
+#pragma unroll
+        for (int b = 0; b < kClusterBlocks; ++b) v[b] = tc5::ld_cluster(tc5::map_rank(part + (uint32_t)((r * 8 + c) * 4), (uint32_t)b));
+#pragma unroll
+        for (int b = 0; b < kClusterBlocks; ++b) s += v[b];
+        return sc * s;
+    }, s_v, s_scale);
+    __syncthreads();
+    tc5::cluster_arrive();                               // this block has read the others' parts
+    for (; f0 < ex.f_end; f0 += 256) {
+        ex.finish(q, f0);
+        ex.load(q, f0 + 256);
+    }
+    __syncwarp();
+    tc5::cluster_wait();                                 // and they have read its own
 }
 
 // The same on tcgen05, for ranks up to 64: D[feature, row] = sum over v's parts of B[feature, :] v_part[row, :], 128
@@ -745,6 +807,11 @@ lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b
     if (warp == 3) { tc5::fence_after(); tc5::tmem_dealloc(tmem, kTcGroups * kTcNT); }
 }
 
+// One launch for few tiles of eight rows and ranks up to 32.  (Measured, one launch against two: rank 16, 1024 to 1024, one
+// row 4.2 us and 4.9, 64 rows of 2 adapters 5.1 and 6.1, 256 rows of 8 9.3 and 6.3; rank 64, 6144 to 6144, one row 13.2 and
+// 9.1.  On the host it is one launch and no scratch.)
+inline bool lora_one_launch(int P, int R, int nA) { return R <= 32 && (nA < P ? nA : P) + P / 8 <= 24; }
+
 // How the first launch is cut: a rule on P and the number of adapters alone, because the scratch is sized by it.
 // Eight-row tiles (the least mma.sync multiplies) while an adapter has few rows, 64-row tiles above; the sum over K is
 // spread until two blocks per SM have work.
@@ -780,6 +847,18 @@ int run_shrink(const LoraArgs& a, cudaStream_t s) {
     return launch_status();
 }
 
+// whether B (1) and y (2) can be read in pieces of eight and sixteen bytes
+template <typename Y>
+int expand_flags(const LoraArgs& a) {
+    return (a.R % 4 == 0 && !misaligned(a.B, 8) ? 1 : 0) + (a.N % (16 / (int)sizeof(Y)) == 0 && !misaligned(a.y, 16) ? 2 : 0);
+}
+
+template <typename T, typename Y, int KG>
+int run_cluster(const LoraArgs& a, cudaStream_t s) {
+    const int tiles = (a.nA < a.P ? a.nA : a.P) + a.P / 8, feats = ((a.N + 31) / 32 + kClusterBlocks - 1) / kClusterBlocks * 32;
+    return launch_after(lora_cluster_kernel<T, Y, KG>, dim3((unsigned)tiles * kClusterBlocks), 256, 0, kClusterBlocks, s, a, feats, expand_flags<Y>(a));
+}
+
 template <typename T, typename Y, int MT, int KG>
 int run_expand(const LoraArgs& a, cudaStream_t s) {
     const size_t smem = (size_t)MT * ((a.R + 15) / 16) * Split<T>::N * 32 * sizeof(uint4);
@@ -791,9 +870,7 @@ int run_expand(const LoraArgs& a, cudaStream_t s) {
     const int passes = (a.N + 255) / 256;
     int per = (int)(((int64_t)passes * tiles + 591) / 592);
     per = per < 1 ? 1 : per > passes ? passes : per;
-    const int vec_b = a.R % 4 == 0 && !misaligned(a.B, 8);
-    const int vec_y = a.N % (16 / (int)sizeof(Y)) == 0 && !misaligned(a.y, 16);
-    return launch_after(kernel, dim3(tiles, (passes + per - 1) / per), 256, smem, 1, s, a, per * 256, vec_b, vec_y);
+    return launch_after(kernel, dim3(tiles, (passes + per - 1) / per), 256, smem, 1, s, a, per * 256, expand_flags<Y>(a));
 }
 
 template <typename T, typename Y>
@@ -812,6 +889,8 @@ int run_expand_tc(const LoraArgs& a, cudaStream_t s) {
 
 template <typename T, typename Y>
 int run_lora(const LoraArgs& a, cudaStream_t s) {
+    if (lora_one_launch(a.P, a.R, a.nA))
+        return a.R <= 16 ? run_cluster<T, Y, 1>(a, s) : run_cluster<T, Y, 2>(a, s);
     const bool wide = lora_wide(a.P, a.nA);
     int st;
     if (wide) st = a.R <= 16 ? run_shrink_wide<T, 1>(a, s) : a.R <= 32 ? run_shrink_wide<T, 2>(a, s) : run_shrink_wide<T, 4>(a, s);
@@ -844,7 +923,7 @@ using namespace gsb;
 
 extern "C" size_t gsb_lora_scratch_bytes(int P, int max_rank, int n_adapters) {
     if (P <= 0 || max_rank <= 0 || n_adapters <= 0) return 0;
-    return (size_t)lora_split(P, n_adapters) * P * max_rank * 4;
+    return lora_one_launch(P, max_rank, n_adapters) ? 0 : (size_t)lora_split(P, n_adapters) * P * max_rank * 4;
 }
 
 extern "C" int gsb_lora_add(const void* x, const void* A, const void* B, int type, const int* adapter_offsets,
@@ -859,8 +938,9 @@ extern "C" int gsb_lora_add(const void* x, const void* A, const void* B, int typ
         misaligned(adapter_offsets, 4) || misaligned(rows, 4) || misaligned(ranks, 4) || misaligned(scales, 4))
         return GSB_ERR_INVALID_ARG;
     if (in % 8 || max_rank > kMaxRank || n_adapters > 1024) return GSB_ERR_UNSUPPORTED;
-    if (!scratch || misaligned(scratch, 256)) return GSB_ERR_INVALID_ARG;
-    if (scratch_bytes < gsb_lora_scratch_bytes(P, max_rank, n_adapters)) return GSB_ERR_WORKSPACE;
+    const size_t need = gsb_lora_scratch_bytes(P, max_rank, n_adapters);
+    if (need && (!scratch || misaligned(scratch, 256))) return GSB_ERR_INVALID_ARG;
+    if (scratch_bytes < need) return GSB_ERR_WORKSPACE;
     LoraArgs a{};
     a.x = x; a.A = A; a.B = B; a.offsets = adapter_offsets; a.rows = rows; a.ranks = ranks; a.scales = scales;
     a.n = n; a.P = P; a.K = in; a.N = out; a.nA = n_adapters; a.R = max_rank;

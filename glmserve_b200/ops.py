@@ -135,7 +135,7 @@ def _out16(out, shape, x, out_dtype, name="out"):
         out_dtype = out_dtype or x.dtype
         if out_dtype not in (x.dtype, torch.float32):
             raise ValueError(f"out_dtype: expected {x.dtype} or torch.float32")
-        return torch.empty(shape, dtype=out_dtype, device=x.device)
+        return x.new_empty(shape, dtype=out_dtype)
     if out.dtype not in (x.dtype, torch.float32) or out.get_device() != x.get_device() or \
             not out.is_contiguous() or tuple(out.shape) != shape or out_dtype not in (None, out.dtype):
         raise ValueError(f"{name}: expected a contiguous tensor {shape} of {x.dtype} or torch.float32 on {x.device}")
@@ -160,7 +160,7 @@ def grouped_gemm(x, w, expert_offsets, rows=None, out=None, out_dtype=None):
     out = _out16(out, (P, N), x, out_dtype)
     nbytes = 0 if rows is None else lib().gsb_grouped_gemm_workspace_bytes(P, K, E)
     with _device(dev):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        ws = x.new_empty((nbytes + 1) // 2) if nbytes else None
         check(lib().gsb_grouped_gemm(x.data_ptr(), w.data_ptr(), _TYPE[dtype], expert_offsets.data_ptr(),
                                      None if rows is None else rows.data_ptr(), n, P, K, N, E, out.data_ptr(),
                                      _TYPE[out.dtype], None if ws is None else ws.data_ptr(), nbytes,
@@ -186,7 +186,7 @@ def moe_expert_ffn_w16(x, topk_ids, topk_w, gate_w, up_w, down_w, out=None, out_
     out = _out16(out, (n, H), x, out_dtype)
     nbytes = lib().gsb_moe_expert_ffn_w16_workspace_bytes(n, topk, H, I, E)
     with _device(dev):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        ws = x.new_empty((nbytes + 1) // 2)
         check(lib().gsb_moe_expert_ffn_w16(x.data_ptr(), topk_ids.data_ptr(), topk_w.data_ptr(), gate_w.data_ptr(),
                                            up_w.data_ptr(), down_w.data_ptr(), _TYPE[dtype], n, topk, H, I, E,
                                            out.data_ptr(), _TYPE[out.dtype], ws.data_ptr(), nbytes, _raw_stream(dev)),
@@ -207,22 +207,24 @@ def lora_add(y, x, A, B, adapter_offsets, rows, ranks=None, scales=None):
         raise ValueError("lora_add: expected contiguous tensors on one CUDA device: x, A and B of torch.bfloat16 or all of "
                          "torch.float16, adapter_offsets, rows and ranks of torch.int32, scales of torch.float32")
     n, K = x.shape
-    nA, R, _ = A.shape
-    N = B.shape[1]
-    if A.shape != (nA, R, K) or B.shape != (nA, N, R) or adapter_offsets.shape[0] != nA + 1 or \
+    nA, R, Ka = A.shape
+    nB, N, Rb = B.shape
+    if Ka != K or nB != nA or Rb != R or adapter_offsets.shape[0] != nA + 1 or \
             (ranks is not None and ranks.shape[0] != nA) or (scales is not None and scales.shape[0] != nA):
         raise ValueError("lora_add: expected A [nA,R,K], B [nA,N,R], adapter_offsets [nA+1], ranks and scales [nA]")
     P = rows.shape[0]
     if y is None:
         raise ValueError("y: expected the projection's result")
     _out16(y, (n, N), x, None, "y")
-    nbytes = lib().gsb_lora_scratch_bytes(P, R, nA)
+    L = lib()
+    nbytes = L.gsb_lora_scratch_bytes(P, R, nA)
     with _device(dev):
-        scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        check(lib().gsb_lora_add(x.data_ptr(), A.data_ptr(), B.data_ptr(), _TYPE[dtype], adapter_offsets.data_ptr(),
-                                 rows.data_ptr(), None if ranks is None else ranks.data_ptr(),
-                                 None if scales is None else scales.data_ptr(), n, P, K, N, nA, R, y.data_ptr(),
-                                 _TYPE[y.dtype], scratch.data_ptr(), nbytes, _raw_stream(dev)), "lora_add")
+        scratch = x.new_empty((nbytes + 1) // 2) if nbytes else None
+        check(L.gsb_lora_add(x.data_ptr(), A.data_ptr(), B.data_ptr(), _TYPE[dtype], adapter_offsets.data_ptr(),
+                             rows.data_ptr(), None if ranks is None else ranks.data_ptr(),
+                             None if scales is None else scales.data_ptr(), n, P, K, N, nA, R, y.data_ptr(),
+                             _TYPE[y.dtype], None if scratch is None else scratch.data_ptr(), nbytes,
+                             _raw_stream(dev)), "lora_add")
     return y
 
 

@@ -158,7 +158,8 @@ GSB_API int gsb_moe_expert_ffn_w16(const void* x, const int* topk_ids, const flo
  * once per batch and used for every projection of the model; rows that no list names are left as they were, indices
  * outside [0,n) are skipped, a row must not be listed twice.  A x is kept in fp32, B is applied to it without
  * rounding it to `type`; y is rounded once.  in % 8 == 0, 1 <= max_rank <= 256, n_adapters <= 1024; x and A 16-byte aligned;
- * scratch of gsb_lora_scratch_bytes() bytes, 256-byte aligned, any contents, not shared by calls that may overlap. */
+ * scratch of gsb_lora_scratch_bytes() bytes (0 for few rows: then it may be NULL), 256-byte aligned, any contents, not
+ * shared by calls that may overlap. */
 GSB_API size_t gsb_lora_scratch_bytes(int P, int max_rank, int n_adapters);
 GSB_API int gsb_lora_add(const void* x, const void* A, const void* B, int type, const int* adapter_offsets,
                          const int* rows, const int* ranks, const float* scales, int n, int P, int in,

@@ -59,8 +59,8 @@ def _lora(x=P16, A=P16, B=P16, type=1, offs=P16, rows=P16, ranks=0, scales=0, n=
     (dict(inn=0), INVALID), (dict(out=0), INVALID), (dict(nA=0), INVALID), (dict(R=0), INVALID), (dict(x=0), INVALID),
     (dict(A=0), INVALID), (dict(B=0), INVALID), (dict(offs=0), INVALID), (dict(rows=0), INVALID), (dict(y=0), INVALID),
     (dict(x=P2), INVALID), (dict(A=P2), INVALID), (dict(B=ODD), INVALID), (dict(y=P2), INVALID), (dict(ranks=P2), INVALID),
-    (dict(scales=P2), INVALID), (dict(sc=0), INVALID), (dict(sc=P16 + 16), INVALID),
-    (dict(inn=60), UNSUPPORTED), (dict(R=257), UNSUPPORTED), (dict(nA=1025), UNSUPPORTED), (dict(nb=64), WORKSPACE)])
+    (dict(scales=P2), INVALID), (dict(n=9999, P=9999, sc=0), INVALID), (dict(n=9999, P=9999, sc=P16 + 16), INVALID),
+    (dict(inn=60), UNSUPPORTED), (dict(R=257), UNSUPPORTED), (dict(nA=1025), UNSUPPORTED), (dict(n=9999, P=9999, nb=64), WORKSPACE)])
 def test_lora_refusals(kw, st):
     assert _lora(**kw) == st
 
