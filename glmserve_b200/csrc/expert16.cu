@@ -30,7 +30,10 @@ constexpr int kTokWarps = 4;
 constexpr int kRing = 5 * kKps * (kABytes + kBBytes);   // five stages of 128 weight rows, 9 of 64, 15 of 32
 constexpr int kMaxStages = 15;
 constexpr int kXch = 2 * kNT * 128 * 4;    // SwiGLU: two buffers of 16 columns x 128 rows
-constexpr size_t kGrSmem = (size_t)kRing + kXch + (kMaxE + 4) * 4 + 256;
+constexpr int kBars = (2 * kMaxStages + 4) * 8 + 16;     // barriers, TMEM address, abort flag
+constexpr int kLists = kRing + kXch + (kMaxE + 4) * 4 + kBars;   // lists of a few slots: offsets, tokens, ids
+constexpr size_t kGrSmem = (size_t)kLists + (kMaxE + 4) * 4 + 2 * kFewSlots * 4;
+static_assert(kLists % 16 == 0, "the lists are read 16 bytes at a time");
 // A token warp comes back to the ring kTokWarps stages later.  With fewer stages than that it could be two uses of a stage
 // ahead, where the parity it waits for is the one that an unfinished phase shows as well.
 static_assert(kRing / (kKps * (kABytes + kBBytes)) >= kTokWarps, "ring too short for the token warps");
@@ -40,14 +43,14 @@ __device__ int g_op16_status;
 
 // item i: experts in order; inside one, all token tiles of a feature block run next to each other (they read the
 // same weights, which the second one finds in L2).  `e` only moves forward.
-__device__ __forceinline__ GrItem gr_item(const GroupedArgs& a, const int* pre, int i, int fb_count, int fw, int& e) {
+__device__ __forceinline__ GrItem gr_item(const int* offsets, int P, const int* pre, int i, int fb_count, int fw, int& e) {
     while (i >= pre[e + 1] * fb_count) ++e;
     const int nt = pre[e + 1] - pre[e], local = i - pre[e] * fb_count;
     const int fb = local / nt, tt = local - fb * nt;
     GrItem it;
     it.e = e;
     it.f0 = fb * fw;
-    const int lo = seg_bound(a.offsets, e, a.P), hi = seg_bound(a.offsets, e + 1, a.P);
+    const int lo = seg_bound(offsets, e, P), hi = seg_bound(offsets, e + 1, P);
     it.p0 = lo + tt * kNT;
     it.cnt = min(kNT, hi - it.p0);
     return it;
@@ -56,6 +59,41 @@ __device__ __forceinline__ GrItem gr_item(const GroupedArgs& a, const int* pre, 
 __device__ __forceinline__ void gr_timeout(volatile int* abort_flag) {
     *abort_flag = 1;
     atomicCAS(&g_op16_status, 0, GSB_ERR_TIMEOUT);
+}
+
+// The lists of moe_dispatch for a few slots, by counting instead of sorting: slot i's place is the number of slots with a
+// smaller id plus the earlier ones of its own, expert e's start the number of slots below it.  off [E + 1], tok and id
+// [kFewSlots] in shared memory; block 0 leaves the offsets and the slots' places in memory.  All threads call, and meet.
+__device__ __forceinline__ void few_lists(const GroupedArgs& a, int* off, int* tok, int* id) {
+    for (int i = threadIdx.x; i < kFewSlots; i += blockDim.x) {
+        const int v = i < a.P ? __ldg(a.ids + i) : -1;
+        id[i] = v >= 0 && v < a.E ? v : a.E;               // what is nobody's sorts behind the last expert
+        tok[i] = 0;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i <= a.E || i < a.P; i += blockDim.x) {
+        const int mine = i < a.P ? id[i] : 0;
+        int below = 0, before = 0, start = 0;
+        for (int j = 0; j < a.P; j += 4) {
+            const int4 v = *reinterpret_cast<const int4*>(id + j);
+            const int w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                below += w[u] < mine;
+                before += w[u] == mine && j + u < i;
+                start += w[u] < i;
+            }
+        }
+        if (i <= a.E) {
+            off[i] = start;
+            if (blockIdx.x == 0) a.offsets_out[i] = start;
+        }
+        if (i < a.P && mine < a.E) {
+            tok[below + before] = i / a.topk;
+            if (blockIdx.x == 0) a.slot_pos_out[i] = below + before;
+        }
+    }
+    __syncthreads();
 }
 
 template <typename T, typename Y, bool GU>
@@ -83,7 +121,14 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
     pdl_trigger();
     pdl_wait();
     int descending = (smem_u32(smem) & 1023u) != 0;    // (the swizzled tiles need a 1 KiB boundary: as good as no list)
-    descending |= seg_scan(a.offsets, a.E, a.P, 4, pre, reinterpret_cast<int*>(s_xch));
+    const int *offsets = a.offsets, *rows = a.rows;
+    if (GU && a.ids) {                     // every block makes the lists of a few slots for itself
+        int* s_off = reinterpret_cast<int*>(smem + kLists);
+        few_lists(a, s_off, s_off + kMaxE + 4, s_off + kMaxE + 4 + kFewSlots);
+        offsets = s_off;
+        rows = s_off + kMaxE + 4;
+    }
+    descending |= seg_scan(offsets, a.E, a.P, 4, pre, reinterpret_cast<int*>(s_xch));
     tc5::fence_before();
     descending = __syncthreads_or(descending);
     tc5::fence_after();
@@ -106,7 +151,7 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
         int e = 0;
         bool dead = false;
         for (int i = first; i < items && !dead && !*abort_flag; i += step) {
-            const GrItem it = gr_item(a, pre, i, FB, fw, e);
+            const GrItem it = gr_item(offsets, a.P, pre, i, FB, fw, e);
             for (int kb = 0; kb < nkb; kb += kKps) {
                 if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
                 if (leader) {
@@ -144,7 +189,7 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
         int e = 0;
         bool dead = false;
         for (int i = first; i < items && !dead && !*abort_flag; i += step) {
-            const GrItem it = gr_item(a, pre, i, FB, fw, e);
+            const GrItem it = gr_item(offsets, a.P, pre, i, FB, fw, e);
             int r[kNT / 4];
 #pragma unroll
             for (int j = 0; j < kNT / 4; ++j) {
@@ -153,7 +198,7 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
                 const int q = j * 4 + (lane >> 3);
                 r[j] = -1;
                 if (q < it.cnt) {
-                    const int v = a.rows ? __ldg(a.rows + it.p0 + q) : it.p0 + q;
+                    const int v = rows ? rows[it.p0 + q] : it.p0 + q;
                     r[j] = v >= 0 && v < a.n ? v : 0;
                 }
             }
@@ -221,7 +266,7 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
         int e = 0;
         Y* y = reinterpret_cast<Y*>(a.y);
         for (int i = first; i < items; i += step, ++tl) {
-            const GrItem it = gr_item(a, pre, i, FB, fw, e);
+            const GrItem it = gr_item(offsets, a.P, pre, i, FB, fw, e);
             const uint32_t buf = tl & 1u;
             int ok = *abort_flag ? 0 : (int)mbar_wait(&acc_full[buf], (tl >> 1) & 1u, kGrWaitLimit);
             if (!ok) gr_timeout(abort_flag);
@@ -233,7 +278,7 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
             tc5::tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + buf * kNT, u);
             // which of the tokens exist
             int r = lane < it.cnt ? 0 : -1;
-            if (a.rows && r == 0) r = __ldg(a.rows + it.p0 + lane);
+            if (rows && r == 0) r = rows[it.p0 + lane];
             const uint32_t live = __ballot_sync(0xffffffffu, r >= 0 && r < a.n);
             tc5::tmem_ld_wait();
             tc5::fence_before();
@@ -298,42 +343,13 @@ int launch_grouped(const GroupedArgs& a, int type, int y_type, void* scratch, cu
     return type == GSB_TYPE_BF16 ? run_grouped_any<__nv_bfloat16>(a, y_type, s) : run_grouped_any<__half>(a, y_type, s);
 }
 
-// Dispatch of a few slots (P <= 256): the same lists as dispatch_kernel, by counting instead of sorting - thread i finds
-// slot i's place as the slots of smaller ids plus the earlier ones of its own, thread e expert e's start.
-constexpr int kFewSlots = 256;
+// The lists alone, for the pair kernel.
 __global__ void __launch_bounds__(1024)
-dispatch_few_kernel(const int* __restrict__ ids, int P, int topk, int E, int* __restrict__ offsets, int* __restrict__ tok,
-                    int* __restrict__ slot_pos) {
-    __shared__ __align__(16) int s_id[kFewSlots];
-    const int i = threadIdx.x;
+dispatch_few_kernel(const GroupedArgs a, int* tok) {
+    __shared__ __align__(16) int s_list[kMaxE + 4 + 2 * kFewSlots];
     pdl_trigger();
-    if (i < kFewSlots) {
-        const int id = i < P ? __ldg(ids + i) : -1;
-        s_id[i] = id >= 0 && id < E ? id : E;               // what is nobody's sorts behind the last expert
-    }
-    __syncthreads();
-    const int mine = i < kFewSlots ? s_id[i] : 0;
-    int below = 0, before = 0, start = 0;
-    for (int j = 0; j < P; j += 4) {
-        const int4 v = *reinterpret_cast<const int4*>(s_id + j);
-        const int w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            below += w[u] < mine;
-            before += w[u] == mine && j + u < i;
-            start += w[u] < i;
-        }
-    }
-    if (i < P && mine < E) {
-        tok[below + before] = i / topk;
-        slot_pos[i] = below + before;
-    }
-    if (i <= E) offsets[i] = start;
-    if (i == 1023 && E == 1024) {
-        int all = 0;
-        for (int j = 0; j < P; ++j) all += s_id[j] < E;
-        offsets[E] = all;
-    }
+    few_lists(a, s_list, s_list + kMaxE + 4, s_list + kMaxE + 4 + kFewSlots);
+    if (threadIdx.x < a.P) tok[threadIdx.x] = s_list[kMaxE + 4 + threadIdx.x];
 }
 
 // out[t] = sum over k, in order, of w[t, k] * y[slot_pos[t, k]]; slots whose id is outside [0, E) add nothing.  A block
@@ -480,17 +496,23 @@ extern "C" int gsb_moe_expert_ffn_w16(const void* x, const int* topk_ids, const 
     const Ffn16Ws ws = carve16(n, topk, hidden, moe_inter, E, workspace);
     if (workspace_bytes < ws.total) return GSB_ERR_WORKSPACE;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    int st;
-    if (n * topk <= kFewSlots) {
-        dispatch_few_kernel<<<1, 1024, 0, s>>>(topk_ids, n * topk, topk, E, ws.offsets, ws.tok, ws.slot_pos);
-        st = launch_status();
+    GroupedArgs g{};
+    g.x = x; g.w = gate_w; g.w2 = up_w; g.offsets = ws.offsets; g.rows = ws.tok;
+    g.n = n; g.P = n * topk; g.K = hidden; g.N = moe_inter; g.E = E; g.y = ws.h;
+    int st = GSB_OK;
+    if (g.P <= kFewSlots) {
+        g.ids = topk_ids; g.topk = topk; g.offsets_out = ws.offsets; g.slot_pos_out = ws.slot_pos;
+        if (use_pair(g.P, E)) {
+            dispatch_few_kernel<<<1, 1024, 0, s>>>(g, ws.tok);
+            st = launch_status();
+            g.ids = nullptr;
+        } else {
+            g.offsets = nullptr; g.rows = nullptr;
+        }
     } else {
         st = launch_dispatch(topk_ids, n, topk, E, ws.offsets, ws.tok, ws.row, ws.slot_pos, s, ws.disp);
     }
     if (st) return st;
-    GroupedArgs g{};
-    g.x = x; g.w = gate_w; g.w2 = up_w; g.offsets = ws.offsets; g.rows = ws.tok;
-    g.n = n; g.P = n * topk; g.K = hidden; g.N = moe_inter; g.E = E; g.y = ws.h;
     st = launch_grouped(g, type, type, ws.xs, s);
     if (st) return st;
     GroupedArgs d{};

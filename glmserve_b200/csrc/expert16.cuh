@@ -17,9 +17,17 @@ struct GroupedArgs {
     const int* rows;        // [P] row of x for every p, or null (row p)
     int n, P, K, N, E;
     void* y;                // [P, N]
+    // SwiGLU of few slots: the ids to make offsets and rows from (P = n * topk <= kFewSlots of them; offsets and rows are
+    // null), and where to leave the offsets and every slot's place
+    const int* ids;
+    int topk;
+    int* offsets_out;
+    int* slot_pos_out;
 };
 
 constexpr long long kGrWaitLimit = 2000000000LL;    // about a second of SM clocks
+
+constexpr int kFewSlots = 256;
 
 struct GrItem { int e, p0, cnt, f0; };
 

@@ -20,7 +20,7 @@ template <> __device__ __forceinline__ __half h_from_f(float v) { return sat_hal
 
 // Segment bounds as read from device memory, forced into [0, P]: a list that is not ascending gives wrong rows,
 // never an access outside the buffers.
-__device__ __forceinline__ int seg_bound(const int* offsets, int e, int P) { return min(max(__ldg(offsets + e), 0), P); }
+__device__ __forceinline__ int seg_bound(const int* offsets, int e, int P) { return min(max(offsets[e], 0), P); }
 
 constexpr int kMaxE = 1024;     // segments at most
 
