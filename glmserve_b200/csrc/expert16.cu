@@ -12,23 +12,26 @@ namespace {
 
 // ---- few rows per expert ----------------------------------------------------------------------
 // Bound by the weights, which are read once; everything is arranged around keeping that stream going.
-// One item = w weight rows (128, 64 or 32) x up to 16 token rows of one expert, as D[weight row, token] = sum_k W[row, k]
+// One item = w weight rows (128 or 64) x up to 16 token rows of one expert, as D[weight row, token] = sum_k W[row, k]
 // X[token, k]: the weights are tcgen05's M operand (128 TMEM lanes), so the tokens are padded to 16, not to 128.  For
 // SwiGLU w is made of gate rows followed by as many up rows.  The copies of the next items run while this one is
 // multiplied and stored (one ring over all items of a CTA).  Token rows are gathered by warps with 16-byte cp.async, only
-// as many as there are; through TMA's gather they would hold up the weights in the same queue (GATHER4 us instead of
-// FEW_US for 32 experts of 6144 x 2048 with two rows each).
-// w is chosen on the device, where the number of experts with rows is known: the widest that does not leave SMs idle in
-// the last round (512 items of 128 rows on 148 SMs take 4 rounds, 1024 of 64 rows 7 half as long: 135 us against 123 for
-// 32 experts of 6144 x 2048, SPLIT_US with the same items cut in two along K instead).
+// as many as there are; TMA is left to the weights.
+// w is chosen on the device, where the number of experts with rows is known: 64 where items of 128 would leave half the
+// SMs without one (2 experts of 4096 x 2048, one row each: 14.0 us against 14.5), else 128 - a last round that fills few
+// SMs does not matter, they get the whole bandwidth (32 experts of 6144 x 2048, two rows each: 121 us with 4 rounds of 128
+// rows, 119 with 7 of 64, 199 with 14 of 32, where the MMAs no longer keep up).
+// With so few items that a cluster of blocks can share each, every block sums its part of K; the partial tiles meet in
+// distributed shared memory, each block finishing some columns and adding the parts in rank order - no atomics, the same
+// bits every time.
 constexpr int kGrThreads = 384;            // warps: 0 weights, 1 MMA, 2 TMEM, 4-7 epilogue, 8-11 token rows
 constexpr int kABytes = 128 * 128;         // at most 128 weight rows x 64 columns
 constexpr int kNT = 16;                    // token rows per item at most (seg_scan is given its logarithm, 4)
 constexpr int kBBytes = kNT * 128;
 constexpr int kKps = 2;                    // k-blocks of 64 columns per stage
 constexpr int kTokWarps = 4;
-constexpr int kRing = 5 * kKps * (kABytes + kBBytes);   // five stages of 128 weight rows, 9 of 64, 15 of 32
-constexpr int kMaxStages = 15;
+constexpr int kRing = 5 * kKps * (kABytes + kBBytes);   // five stages of 128 weight rows, 9 of 64
+constexpr int kMaxStages = 9;
 constexpr int kXch = 2 * kNT * 128 * 4;    // SwiGLU: two buffers of 16 columns x 128 rows
 constexpr int kBars = (2 * kMaxStages + 4) * 8 + 16;     // barriers, TMEM address, abort flag
 constexpr int kLists = kRing + kXch + (kMaxE + 4) * 4 + kBars;   // lists of a few slots: offsets, tokens, ids
@@ -118,6 +121,7 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
     }
     if (warp == 0 && lane == 0) { tc5::prefetch_map(&tm_w); if (GU) tc5::prefetch_map(&tm_w2); }
     if (warp == 2) { tc5::tmem_alloc(tmem_slot, 2 * kNT); tc5::tmem_relinquish(); }
+    const int S = (int)tc5::cluster_size(), rank = (int)tc5::cluster_rank();
     pdl_trigger();
     pdl_wait();
     int descending = (smem_u32(smem) & 1023u) != 0;    // (the swizzled tiles need a 1 KiB boundary: as good as no list)
@@ -136,14 +140,22 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
     const int nkb = (a.K + 63) >> 6;
     // at most (E + P / 16) token tiles, and so many items as the host has checked to fit; a list that descends is no list
     const int tiles = descending ? 0 : pre[a.E];
-    const int w = best_width(tiles, a.N * (GU ? 2 : 1), (int)gridDim.x, GU ? 64 : 32);   // weight rows of an item
+    const int w = S == 1 && tiles * ((a.N + (GU ? 63 : 127)) / (GU ? 64 : 128)) * 2 <= (int)gridDim.x ? 64 : 128;   // weight rows of an item
     const int fw = GU ? w / 2 : w;         // output features of an item
     const int FB = (a.N + fw - 1) / fw;
     const int items = tiles * FB;
     // the ring's stages are as long as w rows need, so a narrow item has as many bytes on their way as a wide one (the
     // MMA's unused rows read on into what follows; their lanes are not stored)
     const int abytes = w * 128, stage_bytes = kKps * (abytes + kBBytes), stages = min(kMaxStages, kRing / stage_bytes);
-    const int first = blockIdx.x, step = gridDim.x;
+    const int first = (int)blockIdx.x / S, step = (int)gridDim.x / S;
+    const int kb0 = nkb * rank / S, kb1 = nkb * (rank + 1) / S;     // this block's part of the sum
+
+    // which of an item's tokens exist, as a mask (whole warps ask)
+    auto live_tokens = [&](const GrItem& it) {
+        int r = lane < it.cnt ? 0 : -1;
+        if (rows && r == 0) r = rows[it.p0 + lane];
+        return __ballot_sync(0xffffffffu, r >= 0 && r < a.n);
+    };
 
     if (warp == 0) {                       // ---- weights
         const bool leader = tc5::elect_one();
@@ -152,10 +164,10 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
         bool dead = false;
         for (int i = first; i < items && !dead && !*abort_flag; i += step) {
             const GrItem it = gr_item(offsets, a.P, pre, i, FB, fw, e);
-            for (int kb = 0; kb < nkb; kb += kKps) {
+            for (int kb = kb0; kb < kb1; kb += kKps) {
                 if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
                 if (leader) {
-                    const int nk = min(kKps, nkb - kb);
+                    const int nk = min(kKps, kb1 - kb);
                     mbar_arrive_expect_tx(&full[st], (uint32_t)(nk * w * 128));
                     uint8_t* dst = smem + st * stage_bytes;
                     for (int j = 0; j < nk; ++j)
@@ -202,7 +214,7 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
                     r[j] = v >= 0 && v < a.n ? v : 0;
                 }
             }
-            for (int kb = 0; kb < nkb; kb += kKps, ++cnt) {
+            for (int kb = kb0; kb < kb1; kb += kKps, ++cnt) {
                 if ((int)(cnt % kTokWarps) == group) {
                     if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
                     const uint32_t base = smem_u32(smem) + st * stage_bytes + kKps * abytes + (uint32_t)((lane >> 3) * 128);
@@ -212,7 +224,7 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
                         const T* xk = in ? x + (kb + u) * 64 : x;
 #pragma unroll
                         for (int j = 0; j < kNT / 4; ++j)     // 128-byte swizzle: piece c of row q lies at c ^ q % 8
-                            if (r[j] >= 0 && kb + u < nkb)
+                            if (r[j] >= 0 && kb + u < kb1)
                                 tc5::cp_async16(base + (uint32_t)(u * kBBytes + j * 512 + ((piece ^ ((j * 4 + (lane >> 3)) & 7)) << 4)),
                                                 xk + (int64_t)r[j] * a.K, in);
                     }
@@ -239,7 +251,7 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
             if (!mbar_wait(&acc_empty[buf], ((tl >> 1) & 1u) ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); break; }
             tc5::fence_after();
             uint32_t acc = 0;
-            for (int kb = 0; kb < nkb; kb += kKps) {
+            for (int kb = kb0; kb < kb1; kb += kKps) {
                 if (!mbar_wait(&full[st], ph, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
                 tc5::fence_after();
                 if (leader) {
@@ -247,7 +259,7 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
                     const uint64_t bd = ad + (uint64_t)(kKps * abytes >> 4);
 #pragma unroll
                     for (int j = 0; j < kKps; ++j)
-                        if (kb + j < nkb)
+                        if (kb + j < kb1)
 #pragma unroll
                             for (int k = 0; k < 4; ++k)
                                 tc5::mma_f16_ss(tmem + buf * kNT, ad + (uint64_t)(j * (abytes >> 4) + k * 2),
@@ -276,15 +288,17 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
             tc5::fence_after();
             uint32_t u[kNT];
             tc5::tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + buf * kNT, u);
-            // which of the tokens exist
-            int r = lane < it.cnt ? 0 : -1;
-            if (rows && r == 0) r = rows[it.p0 + lane];
-            const uint32_t live = __ballot_sync(0xffffffffu, r >= 0 && r < a.n);
+            const uint32_t live = live_tokens(it);
             tc5::tmem_ld_wait();
             tc5::fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&acc_empty[buf]);
-            if (GU) {
+            if (S > 1) {                   // to the block that finishes the column: [source][column][row]
+                const int per = kNT / S;
+#pragma unroll
+                for (int j = 0; j < kNT; ++j)
+                    tc5::st_cluster(tc5::map_rank(smem_u32(s_xch + (rank * per + j % per) * 128 + row), (uint32_t)(j / per)), __uint_as_float(u[j]));
+            } else if (GU) {
                 // rows [0, fw) are gate, [fw, 2 fw) the up rows of the same features
                 float* xs = s_xch + buf * kNT * 128;
 #pragma unroll
@@ -305,6 +319,25 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
     }
     __syncwarp();
     tc5::fence_before();
+    if (S > 1) {                           // (one item per cluster)
+        tc5::cluster_sync_all();
+        if (first < items && warp >= 4 && warp < 8 && !*abort_flag) {
+            int e = 0;
+            const GrItem it = gr_item(offsets, a.P, pre, first, FB, fw, e);
+            const uint32_t live = live_tokens(it);
+            const int per = kNT / S, row = (warp & 3) * 32 + lane, fl = GU ? row & 63 : row, f = it.f0 + fl;
+            for (int cl = GU ? row >> 6 : 0; cl < per; cl += GU ? 2 : 1) {
+                const int c = rank * per + cl;
+                if (f >= a.N || !((live >> c) & 1u)) continue;
+                float s0 = 0.f, s1 = 0.f;
+                for (int src = 0; src < S; ++src) {
+                    s0 += s_xch[(src * per + cl) * 128 + fl];
+                    if (GU) s1 += s_xch[(src * per + cl) * 128 + 64 + fl];
+                }
+                reinterpret_cast<Y*>(a.y)[(int64_t)(it.p0 + c) * a.N + f] = GU ? h_from_f<Y>(__fmul_rn(silu_ref(s0), s1)) : from_f<Y>(s0);
+            }
+        }
+    }
     __syncthreads();
     if (warp == 2) { tc5::fence_after(); tc5::tmem_dealloc(tmem, 2 * kNT); }
 }
@@ -321,13 +354,18 @@ int run_grouped(const GroupedArgs& a, cudaStream_t s) {
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kGrSmem) != cudaSuccess) return GSB_ERR_CUDA;
         if (dev < 64) ready.fetch_or(1ull << dev);
     }
-    const int64_t fbs = (a.N + 31) / 32, tiles = (a.E < a.P ? a.E : a.P) + a.P / kNT, items = tiles * fbs;
+    const int64_t fbs = (a.N + (GU ? 31 : 63)) / (GU ? 32 : 64), tiles = (a.E < a.P ? a.E : a.P) + a.P / kNT, items = tiles * fbs;
     if (items + sms >= (int64_t)1 << 31) return GSB_ERR_TOO_LARGE;
     CUtensorMap tw, tw2;
     constexpr bool bf = std::is_same<T, __nv_bfloat16>::value;
     if (!encode(&tw, a.w, bf, a.K, a.N, a.E, 32) || (GU && !encode(&tw2, a.w2, bf, a.K, a.N, a.E, 32))) return GSB_ERR_CUDA;
-    const int grid = (int)(items < sms ? items : sms);
-    return launch_after(kernel, dim3(grid), kGrThreads, kGrSmem, 1, s, a, tw, GU ? tw2 : tw);
+    // A cluster of four blocks per item where that many still run at once and the sum is long (1 expert, one row of 6144 to
+    // 2048: 10.9 us against 17.4, 4 experts, 4096 to 1000: 9.6 against 13.3; at 1024 the cluster costs 1 us more than it
+    // saves, at 2048 the two are equal; two or eight blocks were no better).
+    const int64_t wide = tiles * ((a.N + (GU ? 63 : 127)) / (GU ? 64 : 128));
+    const int S = a.K > 2048 && wide * 4 <= sms ? 4 : 1;
+    const int grid = S > 1 ? (int)wide * S : (int)(items < sms ? items : sms);
+    return launch_after(kernel, dim3(grid), kGrThreads, kGrSmem, S, s, a, tw, GU ? tw2 : tw);
 }
 
 template <typename T>

@@ -31,19 +31,6 @@ constexpr int kFewSlots = 256;
 
 struct GrItem { int e, p0, cnt, f0; };
 
-// Weight rows of an item (128, 64 or 32, not under `least`) for `tiles` token tiles x `rows` weight rows each on
-// `workers` CTAs that take items in turn: the one with the shortest way through, an item costing its rows and the time of
-// about 8 more.
-__device__ __forceinline__ int best_width(int tiles, int rows, int workers, int least) {
-    int best = 128;
-    int64_t cost = 0;
-    for (int w = 128; w >= least; w >>= 1) {
-        const int64_t items = (int64_t)tiles * ((rows + w - 1) / w), c = (items + workers - 1) / workers * (w + 8);
-        if (w == 128 || c < cost) { best = w; cost = c; }
-    }
-    return best;
-}
-
 // AND over the four epilogue warps
 __device__ __forceinline__ int epilogue_agree(int ok) {
     int all;

@@ -5,9 +5,9 @@
 // both halves, so a byte of shared memory feeds twice the products of a one-CTA tile - with a 128 x 256 tile per CTA the
 // operand reads plus the writes of the copies need 1.5 times the shared-memory bandwidth of an SM.
 // Both operands come by TMA, so the token rows lie in expert order: rows named by a list are copied into that order
-// first (one pass, GATHER_US for 16384 rows of 2048).  Gathering inside this kernel was slower: TMA's gather takes ~70
-// cycles per four rows, 4.5 times the 512 cycles a 64-column k-block multiplies for (250 TFLOP/s), and eight warps with
-// 16-byte cp.async deliver ~16 bytes a cycle where 32 are needed (1008 TFLOP/s against 1233 with rows in order).
+// first (16384 rows of 2048: 16 us, the rate of a copy).  Gathering inside this kernel was slower: 16384 rows of 8 experts,
+// 2048 to 4096, take 190 us in order, 211 with the copy, 307 with TMA's gather (~26 cycles per four rows, where a k-block
+// of 64 columns multiplies for 512) and 309 with half the rows by TMA's gather and half by cp.async.
 // SwiGLU: a CTA's 128 weight rows are 64 gate rows and their 64 up rows; the epilogue warps swap halves through shared
 // memory.  Two accumulators (2 x 256 TMEM columns), so the epilogue of a tile runs under the next one's main loop.  A
 // TMEM lane holds one feature of 32 tokens where memory wants a token's features side by side: 16-bit results are turned

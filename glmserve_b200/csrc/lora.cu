@@ -144,7 +144,7 @@ lora_shrink_kernel(const LoraArgs a) {
 // The same for adapters with many rows: 64 rows x 16 * MT ranks, D[row, rank], over K steps of 64 columns that 16-byte
 // asynchronous copies bring into a ring in shared memory (rows of 128 bytes, 16-byte piece c of row q at c ^ q % 8), so
 // that 48 KB a block stay in flight without a register: the direct kernel above, at 32 rows x 64 ranks a block, has room
-// for one step and measured 91 us for 8192 rows of 6144 at rank 64, this one WIDE_US.  Warps: four groups of 16 rows x two
+// for one step and measured 91 us for 8192 rows of 6144 at rank 64, this one 33 us.  Warps: four groups of 16 rows x two
 // halves of each K step.
 constexpr int kWdRows = 64, kWdStages = 4;
 template <int MT> constexpr int wd_stage_bytes() { return (kWdRows + 16 * MT) * 128; }
@@ -250,7 +250,7 @@ lora_shrink_wide_kernel(const LoraArgs a) {
 // v enters the 16-bit tensor cores as a sum of 16-bit numbers, so that y's fp32 sums keep (nearly) fp32 accuracy: three
 // bf16 numbers hold all 24 bits; two fp16 numbers hold 22, with each row of v scaled by a power of two to a largest
 // value in [2^14, 2^15) so that neither overflows or loses bits below fp16's normal range.  (tf32 would do it in two
-// for both types, but mma.sync runs tf32 at the rate of plain fp32 multiply-adds here: 192 us instead of EXP_US for 8192
+// for both types, but mma.sync runs tf32 at the rate of plain fp32 multiply-adds here: 192 us instead of 121 for 8192
 // rows of 6144 at rank 64.)  n-tile j of a warp's chunk holds features 8 (c / 2) + 2 j + c % 2 in its columns c: lane t
 // of a quad then owns eight contiguous features of a row.
 template <typename T> __device__ __forceinline__ float2 pair_f(uint32_t v);
@@ -473,9 +473,11 @@ lora_expand_kernel(const LoraArgs a, int feats, int flags) {
     int descending = seg_scan(a.offsets, a.nA, a.P, MT == 1 ? 4 : 5, pre, wsum);
     descending = __syncthreads_or(descending);
     const LoraTile tile = lora_tile<16 * MT>(a, pre, blockIdx.x, descending);
-    if (tile.ad < 0) return;
-    const int rank = rank_of(a, tile.ad);
-    if (rank == 0) return;
+    const int rank = tile.ad < 0 ? 0 : rank_of(a, tile.ad);
+    if (rank == 0) {
+        pdl_wait();                                      // this launch does not end before the first
+        return;
+    }
     const float sc = a.scales ? __ldg(a.scales + tile.ad) : 1.f;
     const Expand<T, Y, MT, KG> ex(a, tile, rank, s_v, s_scale, min(a.N, (int)(blockIdx.y + 1) * feats), flags);
     int f0 = blockIdx.y * feats + (threadIdx.x >> 5) * 32;
@@ -542,7 +544,7 @@ lora_cluster_kernel(const LoraArgs a, int feats, int flags) {
 // feature blocks).  The product is nothing; what this buys is the way y is met: a lane holds one feature of every row, so
 // a warp reads and writes whole 128-byte lines straight from registers, one load, one add and one store a value, with the
 // loads of 32 rows on their way before the product is waited for.  (mma.sync's fragments are 8-byte pieces of eight rows:
-// the kernel above took 121 us for 8192 rows of 6144 at rank 64, bound by its instructions, this one EXPT_US.)
+// the kernel above took 121 us for 8192 rows of 6144 at rank 64, bound by its instructions, this one 85 us.)
 // B comes by TMA as 128-byte rows of 64 ranks, zeros behind R; columns between an adapter's rank and the next multiple of
 // 16 are zeroed in shared memory, since v's zeros would not hide a NaN there.  Needs R % 8 == 0 and B 16-byte aligned.
 constexpr int kTcNT = 64;                  // rows per tile at most
@@ -639,6 +641,8 @@ lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b
     const int FB = (a.N + 127) / 128;
     const int units = descending ? 0 : pre[a.nA] * FB;                  // (checked to fit by the host)
     const int u_beg = (int)((int64_t)units * blockIdx.x / gridDim.x), u_end = (int)((int64_t)units * (blockIdx.x + 1) / gridDim.x);
+
+    if (u_beg == u_end) pdl_wait();        // this launch does not end before the first
 
     if (warp == 0) {                       // ---- B tiles
         const bool leader = tc5::elect_one();
@@ -933,7 +937,7 @@ extern "C" int gsb_lora_add(const void* x, const void* A, const void* B, int typ
     if ((type != GSB_TYPE_BF16 && type != GSB_TYPE_F16) || (y_type != type && y_type != GSB_TYPE_F32)) return GSB_ERR_INVALID_ARG;
     if (n < 0 || P < 0 || P > n || in <= 0 || out <= 0 || n_adapters <= 0 || max_rank <= 0) return GSB_ERR_INVALID_ARG;
     if (P == 0) return GSB_OK;
-    if (!x || !A || !B || !adapter_offsets || !rows || !y) return GSB_ERR_INVALID_ARG;
+    if (!x || !A || !B || !adapter_offsets || !rows || !y || y == x) return GSB_ERR_INVALID_ARG;
     if (misaligned(x, 16) || misaligned(A, 16) || misaligned(B, 2) || misaligned(y, y_type == GSB_TYPE_F32 ? 4 : 2) ||
         misaligned(adapter_offsets, 4) || misaligned(rows, 4) || misaligned(ranks, 4) || misaligned(scales, 4))
         return GSB_ERR_INVALID_ARG;

@@ -48,7 +48,7 @@ def test_ffn_refusals(kw, st):
 
 
 def _lora(x=P16, A=P16, B=P16, type=1, offs=P16, rows=P16, ranks=0, scales=0, n=4, P=4, inn=64, out=32, nA=2, R=8,
-          y=P16, yt=0, sc=P16, nb=1 << 30):
+          y=2 * P16, yt=0, sc=P16, nb=1 << 30):
     from glmserve_b200._lib import lib
     return lib().gsb_lora_add(_v(x), _v(A), _v(B), type, _v(offs), _v(rows), _v(ranks), _v(scales), n, P, inn, out, nA, R,
                               _v(y), yt, _v(sc), C.c_size_t(nb), None)
@@ -57,7 +57,7 @@ def _lora(x=P16, A=P16, B=P16, type=1, offs=P16, rows=P16, ranks=0, scales=0, n=
 @pytest.mark.parametrize("kw,st", [
     (dict(P=0), OK), (dict(type=0), INVALID), (dict(yt=2), INVALID), (dict(n=-1, P=-1), INVALID), (dict(P=5), INVALID),
     (dict(inn=0), INVALID), (dict(out=0), INVALID), (dict(nA=0), INVALID), (dict(R=0), INVALID), (dict(x=0), INVALID),
-    (dict(A=0), INVALID), (dict(B=0), INVALID), (dict(offs=0), INVALID), (dict(rows=0), INVALID), (dict(y=0), INVALID),
+    (dict(A=0), INVALID), (dict(B=0), INVALID), (dict(offs=0), INVALID), (dict(rows=0), INVALID), (dict(y=0), INVALID), (dict(y=P16), INVALID),
     (dict(x=P2), INVALID), (dict(A=P2), INVALID), (dict(B=ODD), INVALID), (dict(y=P2), INVALID), (dict(ranks=P2), INVALID),
     (dict(scales=P2), INVALID), (dict(n=9999, P=9999, sc=0), INVALID), (dict(n=9999, P=9999, sc=P16 + 16), INVALID),
     (dict(inn=60), UNSUPPORTED), (dict(R=257), UNSUPPORTED), (dict(nA=1025), UNSUPPORTED), (dict(n=9999, P=9999, nb=64), WORKSPACE)])

@@ -75,6 +75,14 @@ CASES = [  # counts of every expert, n tokens, K, N
     ([0, 0, 0], 4, 64, 64),
     ([700, 2, 0, 1400], 900, 2048, 640),
     ([40, 24, 70], 100, 6144, 320),
+    ([3], 3, 6144, 200),            # a cluster of blocks per item
+    ([2, 0, 5], 9, 2184, 333),
+    ([16, 15], 31, 4096, 128),
+    ([2], 2, 2056, 70),
+    ([30] * 9, 100, 136, 264),      # tiles of 32, 64 and 128 rows
+    ([100, 90, 0, 110], 130, 264, 520),
+    ([200] * 10, 500, 72, 1111),
+    ([255, 257, 512, 3, 300], 640, 200, 2050),
 ]
 
 
@@ -184,6 +192,11 @@ FFN = [  # n, topk, E, ids below `of`, H, I
     (333, 3, 5, 5, 520, 264),
     (700, 2, 8, 8, 1024, 1032),
     (2500, 4, 6, 6, 264, 136),
+    (2, 2, 3, 3, 4096, 200),        # a cluster of blocks per item
+    (32, 8, 20, 20, 128, 2304),     # 256 slots, lists made in the kernel
+    (100, 2, 3, 3, 264, 520),       # 200 slots, the pair kernel
+    (129, 2, 64, 64, 72, 128),      # 258 slots
+    (5, 300, 400, 400, 64, 64),     # more slots a token than a block has threads
 ]
 
 

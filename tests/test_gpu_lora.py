@@ -48,6 +48,15 @@ CASES = [  # n, K, N, adapters, R, ranks, share without an adapter
     (2000, 256, 264, 1000, 8, "zeros", 0.5),
     (700, 520, 1024, 5, 128, "mixed", 1.0),
     (40, 16, 6144, 2, 7, None, 0.0),
+    (3, 4104, 1032, 4, 32, "mixed", 0.0),       # one launch
+    (190, 264, 520, 1, 16, None, 0.0),
+    (100, 512, 264, 50, 64, "mixed", 0.1),      # 8-row tiles, 16-row tiles
+    (1100, 136, 264, 4, 16, "mixed", 0.1),      # 32-row tiles
+    (1300, 72, 130, 4, 60, "mixed", 0.1),
+    (1300, 264, 5300, 3, 64, "mixed", 0.1),     # tcgen05
+    (4500, 72, 5900, 9, 32, "zeros", 0.2),
+    (1210, 64, 5260, 40, 40, None, 0.0),
+    (1050, 128, 200, 3, 200, "mixed", 0.0),
 ]
 
 
