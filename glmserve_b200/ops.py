@@ -6,7 +6,6 @@ tensors used only as device buffers; every call runs on torch's current stream.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 
 import torch
@@ -103,41 +102,34 @@ def moe_expert_ffn(x, topk_ids, topk_w, gate_w, up_w, down_w):
 
 
 _TYPE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-_16BIT = (torch.bfloat16, torch.float16)
 
 
-_HERE = contextlib.nullcontext()
+def _launch(dev, fn, *args):
+    """fn(*args, stream) on device `dev` and torch's current stream there.  (Raw handles: torch.cuda.current_stream() and
+    a device context around every call take longer than a small call's launch.)"""
+    if dev == torch._C._cuda_getDevice():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    with torch.cuda.device(dev):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(dev))
 
 
-def _device(dev):
-    """Context in which device `dev` is the current one (nothing to do where it is already)."""
-    return _HERE if dev == torch.cuda.current_device() else torch.cuda.device(dev)
-
-
-def _raw_stream(dev):
-    """Handle of torch's current stream on device `dev`; torch.cuda.current_stream() builds an object around it, which
-    takes longer than a small call's kernel launch."""
-    return torch._C._cuda_getCurrentRawStream(dev)
-
-
-def _is16(x, dev, *named):
-    """Whether x is a contiguous 2-D bf16/fp16 CUDA tensor and every (t, dtype, dims) lies likewise on its device."""
-    if dev < 0 or x.dim() != 2 or not x.is_contiguous() or x.dtype not in _16BIT:
-        return False
-    for t, dtype, dims in named:
-        if t is not None and (t.dtype is not dtype or t.dim() != dims or t.get_device() != dev or not t.is_contiguous()):
+def _on(dev, dtype, *tensors):
+    """Whether all tensors are contiguous, of `dtype` and on device `dev` (None passes)."""
+    for t in tensors:
+        if t is not None and not (t.dtype is dtype and t.get_device() == dev and t.is_contiguous()):
             return False
     return True
 
 
 def _out16(out, shape, x, out_dtype, name="out"):
     if out is None:
-        out_dtype = out_dtype or x.dtype
-        if out_dtype not in (x.dtype, torch.float32):
+        if out_dtype is None or out_dtype is x.dtype:
+            return x.new_empty(shape)
+        if out_dtype is not torch.float32:
             raise ValueError(f"out_dtype: expected {x.dtype} or torch.float32")
         return x.new_empty(shape, dtype=out_dtype)
     if out.dtype not in (x.dtype, torch.float32) or out.get_device() != x.get_device() or \
-            not out.is_contiguous() or tuple(out.shape) != shape or out_dtype not in (None, out.dtype):
+            not out.is_contiguous() or out.shape != shape or out_dtype not in (None, out.dtype):
         raise ValueError(f"{name}: expected a contiguous tensor {shape} of {x.dtype} or torch.float32 on {x.device}")
     return out
 
@@ -149,22 +141,25 @@ def grouped_gemm(x, w, expert_offsets, rows=None, out=None, out_dtype=None):
     without ``rows`` row p is x[p].  Returns y [P,N] of x's type (or float32 with ``out_dtype`` / ``out``).  Rows
     that no segment covers are left as they were in ``out``; without ``out`` their contents are undefined."""
     dev, dtype = x.get_device(), x.dtype
-    if not _is16(x, dev, (w, dtype, 3), (expert_offsets, torch.int32, 1), (rows, torch.int32, 1)):
+    if dev < 0 or _TYPE.get(dtype, 0) == 0 or not _on(dev, dtype, x, w) or not _on(dev, torch.int32, expert_offsets, rows):
         raise ValueError("grouped_gemm: expected contiguous tensors on one CUDA device: x [n,K] and w [E,N,K] of "
                          "torch.bfloat16 or both of torch.float16, expert_offsets [E+1] and rows [P] of torch.int32")
     n, K = x.shape
     E, N, Kw = w.shape
-    if Kw != K or expert_offsets.shape[0] != E + 1:
-        raise ValueError("grouped_gemm: expected w [E,N,K] with x's K and expert_offsets [E+1]")
-    P = n if rows is None else rows.shape[0]
-    out = _out16(out, (P, N), x, out_dtype)
-    nbytes = 0 if rows is None else lib().gsb_grouped_gemm_workspace_bytes(P, K, E)
-    with _device(dev):
+    if Kw != K or expert_offsets.shape != (E + 1,) or (rows is not None and rows.dim() != 1):
+        raise ValueError("grouped_gemm: expected w [E,N,K] with x's K, expert_offsets [E+1] and rows [P]")
+    L = lib()
+    if rows is None:
+        P, nbytes, ws = n, 0, None
+    else:
+        P = rows.shape[0]
+        nbytes = L.gsb_grouped_gemm_workspace_bytes(P, K, E)
         ws = x.new_empty((nbytes + 1) // 2) if nbytes else None
-        check(lib().gsb_grouped_gemm(x.data_ptr(), w.data_ptr(), _TYPE[dtype], expert_offsets.data_ptr(),
-                                     None if rows is None else rows.data_ptr(), n, P, K, N, E, out.data_ptr(),
-                                     _TYPE[out.dtype], None if ws is None else ws.data_ptr(), nbytes,
-                                     _raw_stream(dev)), "grouped_gemm")
+    out = _out16(out, (P, N), x, out_dtype)
+    st = _launch(dev, L.gsb_grouped_gemm, x.data_ptr(), w.data_ptr(), _TYPE[dtype], expert_offsets.data_ptr(),
+                 None if rows is None else rows.data_ptr(), n, P, K, N, E, out.data_ptr(), _TYPE[out.dtype],
+                 None if ws is None else ws.data_ptr(), nbytes)
+    check(st, "grouped_gemm")
     return out
 
 
@@ -173,24 +168,24 @@ def moe_expert_ffn_w16(x, topk_ids, topk_w, gate_w, up_w, down_w, out=None, out_
     topk_w float32 [n,topk], gate_w/up_w [E,I,H], down_w [E,H,I] -> out [n,H] of x's type (or float32).  A slot
     whose id is outside [0,E) adds nothing (padding, or an expert on another GPU)."""
     dev, dtype = x.get_device(), x.dtype
-    if not _is16(x, dev, (topk_ids, torch.int32, 2), (topk_w, torch.float32, 2), (gate_w, dtype, 3), (up_w, dtype, 3),
-                 (down_w, dtype, 3)):
+    if dev < 0 or _TYPE.get(dtype, 0) == 0 or not _on(dev, dtype, x, gate_w, up_w, down_w) or \
+            not _on(dev, torch.int32, topk_ids) or not _on(dev, torch.float32, topk_w):
         raise ValueError("moe_expert_ffn_w16: expected contiguous tensors on one CUDA device: x, gate_w, up_w and down_w "
                          "of torch.bfloat16 or all of torch.float16, ids of torch.int32, w of torch.float32")
     n, H = x.shape
-    E, I, _ = gate_w.shape
+    E, I, Hw = gate_w.shape
     topk = topk_ids.shape[1]
-    if gate_w.shape != (E, I, H) or up_w.shape != (E, I, H) or down_w.shape != (E, H, I) or \
-            topk_ids.shape != (n, topk) or topk_w.shape != (n, topk):
+    if Hw != H or up_w.shape != gate_w.shape or down_w.shape != (E, H, I) or topk_ids.shape != (n, topk) or \
+            topk_w.shape != topk_ids.shape:
         raise ValueError("moe_expert_ffn_w16: expected gate_w, up_w [E,I,H], down_w [E,H,I], ids and w [n,topk]")
     out = _out16(out, (n, H), x, out_dtype)
-    nbytes = lib().gsb_moe_expert_ffn_w16_workspace_bytes(n, topk, H, I, E)
-    with _device(dev):
-        ws = x.new_empty((nbytes + 1) // 2)
-        check(lib().gsb_moe_expert_ffn_w16(x.data_ptr(), topk_ids.data_ptr(), topk_w.data_ptr(), gate_w.data_ptr(),
-                                           up_w.data_ptr(), down_w.data_ptr(), _TYPE[dtype], n, topk, H, I, E,
-                                           out.data_ptr(), _TYPE[out.dtype], ws.data_ptr(), nbytes, _raw_stream(dev)),
-              "moe_expert_ffn_w16")
+    L = lib()
+    nbytes = L.gsb_moe_expert_ffn_w16_workspace_bytes(n, topk, H, I, E)
+    ws = x.new_empty((nbytes + 1) // 2)
+    st = _launch(dev, L.gsb_moe_expert_ffn_w16, x.data_ptr(), topk_ids.data_ptr(), topk_w.data_ptr(), gate_w.data_ptr(),
+                 up_w.data_ptr(), down_w.data_ptr(), _TYPE[dtype], n, topk, H, I, E, out.data_ptr(), _TYPE[out.dtype],
+                 ws.data_ptr(), nbytes)
+    check(st, "moe_expert_ffn_w16")
     return out
 
 
@@ -202,29 +197,27 @@ def lora_add(y, x, A, B, adapter_offsets, rows, ranks=None, scales=None):
     ``moe_dispatch(adapter_ids[:, None], nA)``, once per batch: offsets and sorted_token_ids; an id of -1 = no
     adapter.  ``rows`` may be longer than the segments: what lies behind the last one is ignored."""
     dev, dtype = x.get_device(), x.dtype
-    if not _is16(x, dev, (A, dtype, 3), (B, dtype, 3), (adapter_offsets, torch.int32, 1), (rows, torch.int32, 1),
-                 (ranks, torch.int32, 1), (scales, torch.float32, 1)):
+    if dev < 0 or _TYPE.get(dtype, 0) == 0 or not _on(dev, dtype, x, A, B) or \
+            not _on(dev, torch.int32, adapter_offsets, rows, ranks) or not _on(dev, torch.float32, scales):
         raise ValueError("lora_add: expected contiguous tensors on one CUDA device: x, A and B of torch.bfloat16 or all of "
                          "torch.float16, adapter_offsets, rows and ranks of torch.int32, scales of torch.float32")
     n, K = x.shape
     nA, R, Ka = A.shape
     nB, N, Rb = B.shape
-    if Ka != K or nB != nA or Rb != R or adapter_offsets.shape[0] != nA + 1 or \
-            (ranks is not None and ranks.shape[0] != nA) or (scales is not None and scales.shape[0] != nA):
+    P, = rows.shape
+    if Ka != K or nB != nA or Rb != R or adapter_offsets.shape != (nA + 1,) or \
+            (ranks is not None and ranks.shape != (nA,)) or (scales is not None and scales.shape != (nA,)):
         raise ValueError("lora_add: expected A [nA,R,K], B [nA,N,R], adapter_offsets [nA+1], ranks and scales [nA]")
-    P = rows.shape[0]
     if y is None:
         raise ValueError("y: expected the projection's result")
     _out16(y, (n, N), x, None, "y")
     L = lib()
     nbytes = L.gsb_lora_scratch_bytes(P, R, nA)
-    with _device(dev):
-        scratch = x.new_empty((nbytes + 1) // 2) if nbytes else None
-        check(L.gsb_lora_add(x.data_ptr(), A.data_ptr(), B.data_ptr(), _TYPE[dtype], adapter_offsets.data_ptr(),
-                             rows.data_ptr(), None if ranks is None else ranks.data_ptr(),
-                             None if scales is None else scales.data_ptr(), n, P, K, N, nA, R, y.data_ptr(),
-                             _TYPE[y.dtype], None if scratch is None else scratch.data_ptr(), nbytes,
-                             _raw_stream(dev)), "lora_add")
+    scratch = x.new_empty((nbytes + 1) // 2) if nbytes else None
+    st = _launch(dev, L.gsb_lora_add, x.data_ptr(), A.data_ptr(), B.data_ptr(), _TYPE[dtype], adapter_offsets.data_ptr(),
+                 rows.data_ptr(), None if ranks is None else ranks.data_ptr(), None if scales is None else scales.data_ptr(),
+                 n, P, K, N, nA, R, y.data_ptr(), _TYPE[y.dtype], None if scratch is None else scratch.data_ptr(), nbytes)
+    check(st, "lora_add")
     return y
 
 
