@@ -283,7 +283,7 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
             int ok = *abort_flag ? 0 : (int)mbar_wait(&acc_full[buf], (tl >> 1) & 1u, kGrWaitLimit);
             if (!ok) gr_timeout(abort_flag);
             // all four warps must agree to go on: they meet at a barrier below
-            if (GU) ok = epilogue_agree(ok);
+            if (GU) ok = epilogue_agree(ok, 1);
             if (!ok) break;
             tc5::fence_after();
             uint32_t u[kNT];
@@ -303,11 +303,11 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
                 float* xs = s_xch + buf * kNT * 128;
 #pragma unroll
                 for (int j = 0; j < kNT; ++j) xs[j * 128 + row] = __uint_as_float(u[j]);
-                asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
+                epilogue_sync(1);
                 const int fl = row & (fw - 1), f = it.f0 + fl, groups = 128 / fw;     // fw is 64 or 32
                 for (int c = row / fw; c < it.cnt; c += groups)
                     if (f < a.N && ((live >> c) & 1u))
-                        y[(int64_t)(it.p0 + c) * a.N + f] = h_from_f<Y>(__fmul_rn(silu_ref(xs[c * 128 + fl]), xs[c * 128 + fw + fl]));
+                        y[(int64_t)(it.p0 + c) * a.N + f] = h_from_f<Y>(swiglu(xs[c * 128 + fl], xs[c * 128 + fw + fl]));
             } else {
                 const int f = it.f0 + row;
                 if (row < w && f < a.N)
@@ -334,7 +334,7 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
                     s0 += s_xch[(src * per + cl) * 128 + fl];
                     if (GU) s1 += s_xch[(src * per + cl) * 128 + 64 + fl];
                 }
-                reinterpret_cast<Y*>(a.y)[(int64_t)(it.p0 + c) * a.N + f] = GU ? h_from_f<Y>(__fmul_rn(silu_ref(s0), s1)) : from_f<Y>(s0);
+                reinterpret_cast<Y*>(a.y)[(int64_t)(it.p0 + c) * a.N + f] = GU ? h_from_f<Y>(swiglu(s0, s1)) : from_f<Y>(s0);
             }
         }
     }

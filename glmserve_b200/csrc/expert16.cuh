@@ -31,13 +31,18 @@ constexpr int kFewSlots = 256;
 
 struct GrItem { int e, p0, cnt, f0; };
 
-// AND over the four epilogue warps
-__device__ __forceinline__ int epilogue_agree(int ok) {
+// AND over the four warps that meet at named barrier `bar`
+__device__ __forceinline__ int epilogue_agree(int ok, int bar) {
     int all;
-    asm volatile("{\n\t.reg .pred p, r;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred r, 1, 128, p;\n\tselp.u32 %0, 1, 0, r;\n\t}"
-                 : "=r"(all) : "r"(ok) : "memory");
+    asm volatile("{\n\t.reg .pred p, r;\n\tsetp.ne.b32 p, %1, 0;\n\tbarrier.cta.red.and.pred r, %2, 128, p;\n\tselp.u32 %0, 1, 0, r;\n\t}"
+                 : "=r"(all) : "r"(ok), "r"(bar) : "memory");
     return all;
 }
+__device__ __forceinline__ void epilogue_sync(int bar) { asm volatile("barrier.cta.sync %0, 128;" ::"r"(bar) : "memory"); }
+
+// silu(gate) * up.  expf and the divide are good to 2^-21 together; the result is rounded to 16 bits next.  (An IEEE divide
+// here is a third of an epilogue's instructions; where 1 + exp passes 2^126 this one gives 0 for a silu below 2^-119.)
+__device__ __forceinline__ float swiglu(float g, float u) { return __fmul_rn(__fdividef(g, 1.0f + expf(-g)), u); }
 
 // The two kernels; types as in gsb_grouped_gemm (a.w2 given: SwiGLU of two products, y of x's type).
 int launch_grouped_split(const GroupedArgs& a, int type, int y_type, cudaStream_t s);

@@ -22,9 +22,9 @@ constexpr int kPrNT = 256;                 // token rows per tile at most
 constexpr int kPrStages = 6;
 constexpr int kPrHalf = 128 * 128;         // 128 rows x 64 columns: weights, or this CTA's tokens
 constexpr int kPrStageBytes = 2 * kPrHalf;
-constexpr int kPrXch = 2 * 2 * 16 * 64 * 4; // two buffers of 2 x 16 columns x 64 rows fp32
-constexpr int kPrTurn = 4 * 32 * 32 * 2;   // per epilogue warp: 32 tokens x 32 features, 16-bit
-constexpr int kPrThreads = 256;            // warps: 0 weights, 1 MMA, 2 TMEM, 3 tokens, 4-7 epilogue
+constexpr int kPrXch = 2 * 2 * 2 * 8 * 64 * 4;   // per epilogue group: two buffers of 2 x 8 columns x 64 rows fp32
+constexpr int kPrTurn = 8 * 16 * 32 * 2;   // per epilogue warp: 16 tokens x 32 features, 16-bit
+constexpr int kPrThreads = 384;            // warps: 0 weights, 1 MMA, 2 TMEM, 3 tokens, 4-11 epilogue (two groups)
 constexpr size_t kPrSmem = (size_t)kPrStages * kPrStageBytes + kPrXch + kPrTurn + (kMaxE + 4) * 4 + 256;
 static_assert(kPrSmem <= 227 * 1024, "stages exceed the shared memory of an SM");
 
@@ -54,7 +54,7 @@ __device__ __forceinline__ GrItem pr_item(const GroupedArgs& a, const int* pre, 
 template <typename T, typename Y, bool GU>
 __global__ void __launch_bounds__(kPrThreads, 1)
 grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, const __grid_constant__ CUtensorMap tm_w2,
-                    const __grid_constant__ CUtensorMap tm_x, int vec, int lg) {
+                    const __grid_constant__ CUtensorMap tm_x, int vec) {
     extern __shared__ __align__(1024) uint8_t smem[];
     float* s_xch = reinterpret_cast<float*>(smem + kPrStages * kPrStageBytes);
     uint8_t* s_turn = smem + kPrStages * kPrStageBytes + kPrXch;
@@ -65,6 +65,7 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
     uint64_t* acc_empty = acc_full + 2;                                // the leader's are used
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* s_tot = reinterpret_cast<int*>(tmem_slot + 2);                // [3] token tiles if cut into 32, 64, 128 rows
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int rank = (int)tc5::cluster_rank();
@@ -73,27 +74,42 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
             mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
-        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 2 * 4); }
+        for (int i = 0; i < 2; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 2 * 8); }
         *abort_flag = 0;
         fence_barrier_init();
     }
     if (warp == 0 && lane == 0) { tc5::prefetch_map(&tm_w); tc5::prefetch_map(&tm_x); if (GU) tc5::prefetch_map(&tm_w2); }
-    pdl_trigger();
-    pdl_wait();
-    int descending = (smem_u32(smem) & 1023u) != 0;
-    descending |= seg_scan(a.offsets, a.E, a.P, lg, pre, reinterpret_cast<int*>(s_xch));
-    descending = __syncthreads_or(descending);
+    if (tid < 3) s_tot[tid] = 0;
     tc5::cluster_sync_all();
     if (warp == 2) { tc5::tmem_alloc2(tmem_slot, 512); tc5::tmem_relinquish2(); }
     tc5::fence_before();
     tc5::cluster_sync_all();               // the peer has its barriers and its TMEM
     tc5::fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int nkb = (a.K + 63) >> 6;
-    const int tiles = descending ? 0 : pre[a.E];
+    pdl_trigger();
+    pdl_wait();
     constexpr int fc = GU ? 64 : 128, fw = 2 * fc;     // output features of this CTA, and of an item (both CTAs)
     const int FB = (a.N + fw - 1) / fw;
-    const int items = tiles * FB;
+    int n[4], descending = (smem_u32(smem) & 1023u) != 0;
+    descending |= seg_count(a.offsets, a.E, a.P, n);
+    // Tiles of 256 rows, or of fewer (down to 32) where all of them still run at once: a small problem is then spread over
+    // more SMs and its epilogues are shorter (256 rows for each of 4 experts, 1024 x 1024: 12 us with 256 rows a tile, 8 with
+    // 64, 11 with 32, which take two rounds).  Only the device knows how many rows the list names.
+    if (tid < 256)
+        for (int k = 0; k < 3; ++k) {
+            int t = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) t += n[j] > 0 ? (n[j] + (32 << k) - 1) >> (5 + k) : 0;
+            t = __reduce_add_sync(0xffffffffu, t);
+            if (lane == 0 && t) atomicAdd(&s_tot[k], t);
+        }
+    descending = __syncthreads_or(descending);
+    int lg = 8;
+    while (lg > 5 && (int64_t)s_tot[lg - 6] * FB <= (int)gridDim.x >> 1) --lg;
+    seg_scan(n, a.E, lg, pre, reinterpret_cast<int*>(s_xch));
+    __syncthreads();
+    const int nkb = (a.K + 63) >> 6;
+    const int items = descending ? 0 : pre[a.E] * FB;
     const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
     const int fr = rank * fc;              // this CTA's features start here inside an item
 
@@ -183,52 +199,52 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
             }
         }
     } else if (warp >= 4) {                // ---- epilogue: this thread's TMEM lane = weight row of this CTA
-        const int q = warp & 3, row = q * 32 + lane;
-        uint32_t tl = 0;
+        // two groups of four warps take 16 token columns in turn
+        const int group = (warp - 4) >> 2, bar = 1 + group, q = warp & 3, row = q * 32 + lane;
+        uint32_t tl = 0, xb = 0;
         int e = 0;
         Y* y = reinterpret_cast<Y*>(a.y);
-        uint32_t xb = 0;
+        Y* turn = reinterpret_cast<Y*>(s_turn + (warp - 4) * 1024);
         for (int i = first; i < items; i += step, ++tl) {
             const GrItem it = pr_item(a, pre, i, FB, fw, e);
             const uint32_t buf = tl & 1u;
-            // all four warps must agree to go on: they meet at a block barrier in the loop below
             int ok = *abort_flag ? 0 : (int)mbar_wait(&acc_full[buf], (tl >> 1) & 1u, kGrWaitLimit);
             if (!ok) pr_timeout(abort_flag);
-            if (GU) ok = epilogue_agree(ok);
+            // the group's four warps must agree to go on: they meet at a barrier in the loop below
+            if (GU) ok = epilogue_agree(ok, bar);
             if (!ok) break;
             tc5::fence_after();
             const int f = it.f0 + fr + (GU ? row & 63 : row);
-            for (int c0 = 0; c0 < it.cnt; c0 += 32) {
-                uint32_t v[32];
-                tc5::tmem_ld32(tmem + ((uint32_t)(q * 32) << 16) + buf * kPrNT + (uint32_t)c0, v);
-                // which of the 32 tokens exist
-                int r = c0 + lane < it.cnt ? 0 : -1;
+            for (int c0 = group * 16; c0 < it.cnt; c0 += 32) {
+                uint32_t v[16];
+                tc5::tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + buf * kPrNT + (uint32_t)c0, v);
+                // which of the 16 tokens exist
+                int r = lane < 16 && c0 + lane < it.cnt ? 0 : -1;
                 if (a.rows && r == 0) r = __ldg(a.rows + it.p0 + c0 + lane);
                 const uint32_t live = __ballot_sync(0xffffffffu, r >= 0 && r < a.n);
                 tc5::tmem_ld_wait();
-                Y* o = y + (int64_t)(it.p0 + c0) * a.N + f;
-                Y* turn = reinterpret_cast<Y*>(s_turn + q * 2048);
-                constexpr int NC = GU ? 16 : 32;       // columns this thread finishes, from column cb on
-                const int cb = GU && q >= 2 ? 16 : 0;
+                constexpr int NC = GU ? 8 : 16;        // columns this thread finishes, from column cb on
+                const int cb = GU && q >= 2 ? 8 : 0;
                 float d[NC];
                 if (GU) {
-                    // warps 0, 1 hold gate rows, 2, 3 the up rows of the same features: each side keeps 16 of the
-                    // 32 columns and passes the other 16 on
-                    float* xs = s_xch + xb * 2048 + (q >> 1) * 1024 + (row & 63);
+                    // warps 0, 1 of the group hold gate rows, 2, 3 the up rows of the same features: each side keeps 8 of
+                    // the 16 columns and passes the other 8 on
+                    float* xs = s_xch + group * 2048 + xb * 1024 + (q >> 1) * 512 + (row & 63);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) xs[j * 64] = __uint_as_float(q < 2 ? v[16 + j] : v[j]);
-                    asm volatile("barrier.cta.sync 1, 128;" ::: "memory");
-                    const float* xo = s_xch + xb * 2048 + ((q >> 1) ^ 1) * 1024 + (row & 63);
+                    for (int j = 0; j < 8; ++j) xs[j * 64] = __uint_as_float(q < 2 ? v[8 + j] : v[j]);
+                    epilogue_sync(bar);
+                    const float* xo = s_xch + group * 2048 + xb * 1024 + ((q >> 1) ^ 1) * 512 + (row & 63);
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float mine = __uint_as_float(q < 2 ? v[j] : v[16 + j]), other = xo[j * 64];
-                        d[j] = __fmul_rn(silu_ref(q < 2 ? mine : other), q < 2 ? other : mine);
+                    for (int j = 0; j < 8; ++j) {
+                        const float mine = __uint_as_float(q < 2 ? v[j] : v[8 + j]), other = xo[j * 64];
+                        d[j] = swiglu(q < 2 ? mine : other, q < 2 ? other : mine);
                     }
                     xb ^= 1u;
                 } else {
 #pragma unroll
                     for (int j = 0; j < NC; ++j) d[j] = __uint_as_float(v[j]);
                 }
+                Y* o = y + (int64_t)(it.p0 + c0 + cb) * a.N + f;
                 if (sizeof(Y) == 2 && vec) {
 #pragma unroll
                     for (int j = 0; j < NC; ++j) turn[j * 32 + lane] = GU ? h_from_f<Y>(d[j]) : from_f<Y>(d[j]);
@@ -242,14 +258,13 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
                             *reinterpret_cast<uint4*>(y + (int64_t)(it.p0 + c0 + cb + c) * a.N + f8) = o8;
                     }
                     __syncwarp();
-                } else if (live == 0xffffffffu && f - lane + 32 <= a.N) {
-                    Y* oj = o + (int64_t)cb * a.N;
+                } else if (live == 0xffffu && f - lane + 32 <= a.N) {
 #pragma unroll
-                    for (int j = 0; j < NC; ++j, oj += a.N) *oj = GU ? h_from_f<Y>(d[j]) : from_f<Y>(d[j]);
+                    for (int j = 0; j < NC; ++j, o += a.N) *o = GU ? h_from_f<Y>(d[j]) : from_f<Y>(d[j]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < NC; ++j)
-                        if (f < a.N && ((live >> (cb + j)) & 1u)) o[(int64_t)(cb + j) * a.N] = GU ? h_from_f<Y>(d[j]) : from_f<Y>(d[j]);
+                        if (f < a.N && ((live >> (cb + j)) & 1u)) o[(int64_t)j * a.N] = GU ? h_from_f<Y>(d[j]) : from_f<Y>(d[j]);
                 }
             }
             tc5::fence_before();
@@ -302,13 +317,8 @@ int run_pair(const GroupedArgs& a, void* scratch, cudaStream_t s) {
         if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPrSmem) != cudaSuccess) return GSB_ERR_CUDA;
         if (dev < 64) ready.fetch_or(1ull << dev);
     }
-    // Tiles of 256 rows, or of fewer (down to 32) where all of them still run at once: a small problem is then spread over
-    // more SMs and its epilogues are shorter (256 rows for each of 4 experts, 1024 x 1024: 12 us with 256 rows a tile, 8 with
-    // 64, 11 with 32, which take two rounds).
     const int64_t fbs = (a.N + FW - 1) / FW, hit = a.E < a.P ? a.E : a.P;
-    int lg = 8;
-    while (lg > 5 && (hit > (a.P >> (lg - 1)) ? hit : a.P >> (lg - 1)) * fbs <= sms / 2) --lg;
-    const int64_t items = (hit + (a.P >> lg)) * fbs;
+    const int64_t items = (hit + (a.P >> 8)) * fbs, most = (hit + (a.P >> 5)) * fbs;    // with tiles of 256 and of 32 rows
     if (items + sms >= (int64_t)1 << 31) return GSB_ERR_TOO_LARGE;
     const void* sorted = a.x;
     if (a.rows) {
@@ -322,8 +332,8 @@ int run_pair(const GroupedArgs& a, void* scratch, cudaStream_t s) {
     if (!encode(&tw, a.w, bf, a.K, a.N, a.E, GU ? 64 : 128) || (GU && !encode(&tw2, a.w2, bf, a.K, a.N, a.E, 64)) ||
         !encode(&tx, sorted, bf, a.K, a.rows ? a.P : a.n, 0, 32))
         return GSB_ERR_CUDA;
-    const int64_t pairs = items < sms / 2 ? items : sms / 2;
-    return launch_after(kernel, dim3((unsigned)(pairs * 2)), kPrThreads, kPrSmem, 2, s, a, tw, GU ? tw2 : tw, tx, (int)(a.N % 8 == 0 && !misaligned(a.y, 16)), lg);
+    const int64_t pairs = most < sms / 2 ? most : sms / 2;
+    return launch_after(kernel, dim3((unsigned)(pairs * 2)), kPrThreads, kPrSmem, 2, s, a, tw, GU ? tw2 : tw, tx, (int)(a.N % 8 == 0 && !misaligned(a.y, 16)));
 }
 
 template <typename T>

@@ -900,12 +900,16 @@ int run_lora(const LoraArgs& a, cudaStream_t s) {
     if (wide) st = a.R <= 16 ? run_shrink_wide<T, 1>(a, s) : a.R <= 32 ? run_shrink_wide<T, 2>(a, s) : run_shrink_wide<T, 4>(a, s);
     else st = a.R <= 16 ? run_shrink<T, 1>(a, s) : a.R <= 32 ? run_shrink<T, 2>(a, s) : run_shrink<T, 4>(a, s);
     if (st) return st;
-    // Measured over 16 .. 8192 rows, 1024 and 6144 features, 2 .. 32 adapters.  16-row tiles with B loaded ahead while
-    // there are few rows (rank 64, 256 rows of 1024: 11 us against 13 for 32-row tiles and 16 for tcgen05); 32-row tiles
-    // halve the reads of B above (rank 16, 8192 rows of 6144: 111 us against 135 and 120); tcgen05 where rank and output
-    // are large (rank 64, 8192 rows of 6144: 125 us against 166 and 182; rank 32: 121, 127, 136).
+    // Measured over 16 .. 8192 rows, 901 .. 6144 features, 2 .. 32 adapters.  16-row tiles with B loaded ahead while there
+    // are few rows (rank 64, 256 rows of 1024: 11 us against 13 for 32-row tiles and 16 for tcgen05); 32-row tiles halve the
+    // reads of B above (rank 16, 8192 rows of 6144: 111 us against 135 and 120).  tcgen05 where fp32 outputs and the rank
+    // are large (rank 64, 8192 rows of 6144: 103 us against 165; rank 32: 99 and 133; 16-bit y: 116 and 106) and for
+    // outputs whose rows are not 16-byte pieces, which the others take value by value (8192 rows of 3941, rank 16: 75 us
+    // against 217).
     const int64_t outputs = (int64_t)a.P * a.N;
-    if (a.R > 16 && a.R <= 64 && a.R % 8 == 0 && !misaligned(a.B, 16) && outputs >= (a.R > 32 ? 6 << 20 : 24 << 20)) return run_expand_tc<T, Y>(a, s);
+    const bool pieces = expand_flags<Y>(a) & 2;
+    const int64_t enough = !pieces ? 5 << 19 : sizeof(Y) == 4 && a.R > 32 ? 6 << 20 : sizeof(Y) == 4 && a.R > 16 ? 12 << 20 : INT64_MAX;
+    if (a.R <= 64 && a.R % 8 == 0 && !misaligned(a.B, 16) && outputs >= enough) return run_expand_tc<T, Y>(a, s);
     if (a.R > 64) return run_expand<T, Y, 1, 0>(a, s);
     if (wide && a.P >= 1024) return a.R <= 16 ? run_expand<T, Y, 2, 1>(a, s) : run_expand<T, Y, 2, 0>(a, s);
     return a.R <= 16 ? run_expand<T, Y, 1, 1>(a, s) : a.R <= 32 ? run_expand<T, Y, 1, 2>(a, s) : run_expand<T, Y, 1, 4>(a, s);

@@ -24,21 +24,30 @@ __device__ __forceinline__ int seg_bound(const int* offsets, int e, int P) { ret
 
 constexpr int kMaxE = 1024;     // segments at most
 
-// pre[e] = tiles of at most 2^lg rows before segment e, e = 0..E (E <= kMaxE); the first 256 threads work, all call.
-// Returns non-zero in a thread that saw the list descend.  `wsum`: shared scratch of 8 ints.
-__device__ __forceinline__ int seg_scan(const int* offsets, int E, int P, int lg, int* pre, int* wsum) {
+// The walk over the segments: the first 256 threads hold four segments each (n[j] = rows of segment 4 tid + j), all call.
+// Returns non-zero in a thread that saw the list descend.
+__device__ __forceinline__ int seg_count(const int* offsets, int E, int P, int (&n)[4]) {
+    int descending = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int e = (int)threadIdx.x * 4 + j;
+        n[j] = 0;
+        if (e < E) {
+            n[j] = seg_bound(offsets, e + 1, P) - seg_bound(offsets, e, P);
+            descending |= n[j] < 0;
+        }
+    }
+    return descending;
+}
+// pre[e] = tiles of at most 2^lg rows before segment e, e = 0..E (E <= kMaxE).  `wsum`: shared scratch of 8 ints.
+__device__ __forceinline__ void seg_scan(const int (&n)[4], int E, int lg, int* pre, int* wsum) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    int c[4], sum = 0, incl = 0, descending = 0;
+    int c[4], sum = 0, incl = 0;
     if (tid < 256) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int e = tid * 4 + j;
             c[j] = sum;
-            if (e < E) {
-                const int lo = seg_bound(offsets, e, P), hi = seg_bound(offsets, e + 1, P);
-                sum += hi > lo ? (hi - lo + (1 << lg) - 1) >> lg : 0;
-                descending |= hi < lo;
-            }
+            sum += n[j] > 0 ? (n[j] + (1 << lg) - 1) >> lg : 0;
         }
         incl = sum;
 #pragma unroll
@@ -57,6 +66,11 @@ __device__ __forceinline__ int seg_scan(const int* offsets, int E, int P, int lg
             if (tid * 4 + j <= E) pre[tid * 4 + j] = base + c[j];
         if (tid == 255 && E == kMaxE) pre[kMaxE] = base + sum;
     }
+}
+__device__ __forceinline__ int seg_scan(const int* offsets, int E, int P, int lg, int* pre, int* wsum) {
+    int n[4];
+    const int descending = seg_count(offsets, E, P, n);
+    seg_scan(n, E, lg, pre, wsum);
     return descending;
 }
 
