@@ -545,16 +545,21 @@ lora_cluster_kernel(const LoraArgs a, int feats, int flags) {
 // a warp reads and writes whole 128-byte lines straight from registers, one load, one add and one store a value, with the
 // loads of 32 rows on their way before the product is waited for.  (mma.sync's fragments are 8-byte pieces of eight rows:
 // the kernel above took 121 us for 8192 rows of 6144 at rank 64, bound by its instructions, this one 85 us.)
-// B comes by TMA as 128-byte rows of 64 ranks, zeros behind R; columns between an adapter's rank and the next multiple of
-// 16 are zeroed in shared memory, since v's zeros would not hide a NaN there.  Needs R % 8 == 0 and B 16-byte aligned.
+// B comes by TMA as 128-byte rows of 64 ranks, zeros behind R, where R % 8 == 0; columns between an adapter's rank and the
+// next multiple of 16 are zeroed in shared memory, since v's zeros would not hide a NaN there.  With any other R the tile's
+// 128 rows are one piece of memory without 16-byte rows: it is copied as it lies and two warps lay it out.  Needs B
+// 16-byte aligned.
 constexpr int kTcNT = 64;                  // rows per tile at most
 constexpr int kTcStages = 4;               // ring of B tiles
 constexpr int kTcABytes = 128 * 128;
 constexpr int kTcVBytes = kTcNT * 128;     // one part of v: 64 rows x 64 ranks
 constexpr int kTcGroups = 4;               // of four epilogue warps, units in turn; accumulator slots
-constexpr int kTcThreads = 128 + kTcGroups * 128;   // warps: 0 B, 1 MMA, 2 zeroes, 3 TMEM, 4-19 epilogue
+constexpr int kTcThreads = 128 + kTcGroups * 128;   // warps: 0 B, 1 MMA, 2 zeroes, 3 TMEM (2 and 3 lay B out), 4-19 epilogue
+constexpr int kTcLinBytes = 128 * 64 * 2 + 256, kTcLin = 2;     // B tiles as they lie in memory: ring of two
 constexpr long long kTcWaitLimit = 2000000000LL;
-template <typename T> constexpr size_t tc_smem() { return (size_t)kTcStages * kTcABytes + (size_t)Split<T>::N * kTcVBytes + (kMaxE + 4) * 4 + 1280; }
+template <typename T> constexpr size_t tc_smem(bool tma) {
+    return (size_t)kTcStages * kTcABytes + (size_t)Split<T>::N * kTcVBytes + (kMaxE + 4) * 4 + 1280 + (tma ? 0 : kTcLin * kTcLinBytes);
+}
 
 __device__ int g_lora_status;
 
@@ -604,9 +609,22 @@ __device__ __forceinline__ void stage_v_rows(const LoraArgs& a, const LoraTile& 
     }
 }
 
+// B's 128 rows from feature f0 on as one piece of memory: 16-byte aligned start and size, `head` elements before the first
+// row.  The piece stays inside B; the last elements of B that a whole 16 bytes would overshoot are left out of it.
+struct TcLin { const uint8_t* src; int bytes, head; };
+__device__ __forceinline__ TcLin tc_lin(const LoraArgs& a, int ad, int f0) {
+    const int64_t first = ((int64_t)ad * a.N + f0) * a.R * 2, last = first + (int64_t)min(128, a.N - f0) * a.R * 2;
+    const int64_t all = (int64_t)a.nA * a.N * a.R * 2, beg = first & ~(int64_t)15, end = min((last + 15) & ~(int64_t)15, all & ~(int64_t)15);
+    TcLin l;
+    l.src = reinterpret_cast<const uint8_t*>(a.B) + beg;
+    l.bytes = end > beg ? (int)(end - beg) : 0;
+    l.head = (int)(first - beg) / 2;
+    return l;
+}
+
 template <typename T, typename Y>
 __global__ void __launch_bounds__(kTcThreads, 1)
-lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b) {
+lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b, int tma) {
     constexpr int NS = Split<T>::N;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* s_vp = smem + kTcStages * kTcABytes;                       // parts of v, 128-byte swizzled rows
@@ -622,10 +640,14 @@ lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(s_back + kTcNT);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     int* wsum = reinterpret_cast<int*>(tmem_slot + 2);                 // [8]
+    uint64_t* lin_full = reinterpret_cast<uint64_t*>(wsum + 8);        // [2] tile as it lies in memory -> warps 2 and 3
+    uint64_t* lin_empty = lin_full + kTcLin;
+    uint8_t* s_lin = smem + kTcStages * kTcABytes + NS * kTcVBytes + (kMaxE + 4) * 4 + 1280;
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
-        for (int i = 0; i < kTcStages; ++i) { mbar_init(&b_full[i], 1); mbar_init(&b_ready[i], 1); mbar_init(&b_empty[i], 1); }
+        for (int i = 0; i < kTcStages; ++i) { mbar_init(&b_full[i], 1); mbar_init(&b_ready[i], tma ? 1 : 2); mbar_init(&b_empty[i], 1); }
+        for (int i = 0; i < kTcLin; ++i) { mbar_init(&lin_full[i], 1); mbar_init(&lin_empty[i], 2); }
         for (int i = 0; i < kTcGroups; ++i) { mbar_init(&acc_full[i], 1); mbar_init(&acc_empty[i], 4); }
         mbar_init(v_full, 4 * kTcGroups);
         *abort_flag = 0;
@@ -647,41 +669,98 @@ lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b
     if (warp == 0) {                       // ---- B tiles
         const bool leader = tc5::elect_one();
         uint32_t st = 0, ph = 0;
-        for (int u = u_beg, ti = -1; u < u_end && !*abort_flag; ++u) {
-            ti = u / FB;
-            const LoraTile tile = lora_tile<kTcNT>(a, pre, ti, 0);
-            if (!mbar_wait(&b_empty[st], ph ^ 1u, kTcWaitLimit)) { lora_timeout(abort_flag); break; }
+        const uint32_t ring = tma ? kTcStages : kTcLin;
+        uint64_t *fullb = tma ? b_full : lin_full, *emptyb = tma ? b_empty : lin_empty;
+        LoraTile tile{-1, 0, 0};
+        for (int u = u_beg; u < u_end && !*abort_flag; ++u) {
+            if (u == u_beg || u % FB == 0) tile = lora_tile<kTcNT>(a, pre, u / FB, 0);
+            if (!mbar_wait(&emptyb[st], ph ^ 1u, kTcWaitLimit)) { lora_timeout(abort_flag); break; }
             if (leader) {
-                mbar_arrive_expect_tx(&b_full[st], kTcABytes);
-                tc5::tma_load_3d(smem + st * kTcABytes, &tm_b, 0, (u - ti * FB) * 128, tile.ad, &b_full[st]);
+                const int f0 = u % FB * 128;
+                if (tma) {
+                    mbar_arrive_expect_tx(&fullb[st], kTcABytes);
+                    tc5::tma_load_3d(smem + st * kTcABytes, &tm_b, 0, f0, tile.ad, &fullb[st]);
+                } else {
+                    const TcLin l = tc_lin(a, tile.ad, f0);
+                    mbar_arrive_expect_tx(&fullb[st], (uint32_t)l.bytes);
+                    if (l.bytes) bulk_g2s(s_lin + st * kTcLinBytes, l.src, (uint32_t)l.bytes, &fullb[st]);
+                }
             }
-            if (++st == kTcStages) { st = 0; ph ^= 1u; }
+            if (++st == ring) { st = 0; ph ^= 1u; }
         }
-        for (int j = 0; j < kTcStages && !*abort_flag; ++j) {           // the last MMAs' signals have arrived
-            mbar_wait(&b_empty[st], ph ^ 1u, kTcWaitLimit);
-            if (++st == kTcStages) { st = 0; ph ^= 1u; }
+        for (uint32_t j = 0; j < ring && !*abort_flag; ++j) {           // the last tiles are done with, their signals in
+            mbar_wait(&emptyb[st], ph ^ 1u, kTcWaitLimit);
+            if (++st == ring) { st = 0; ph ^= 1u; }
         }
         if (*abort_flag)                   // after a time-out: nothing may still be copying when the block ends
-            for (int j = 0; j < kTcStages; ++j) {
-                if (st == 0) { st = kTcStages; ph ^= 1u; }
+            for (uint32_t j = 0; j < ring; ++j) {
+                if (st == 0) { st = ring; ph ^= 1u; }
                 --st;
-                mbar_wait(&b_full[st], ph, kTcWaitLimit / 16);
+                mbar_wait(&fullb[st], ph, kTcWaitLimit / 16);
             }
-    } else if (warp == 2) {                // ---- zeroes between an adapter's rank and the next multiple of 16
-        uint32_t st = 0, ph = 0;
+    } else if (warp == 2 || (warp == 3 && !tma)) {
+        // ---- tma: zeroes between an adapter's rank and the next multiple of 16; else: the tile laid out, a warp 64 rows
+        uint32_t st = 0, ph = 0, ls = 0, lph = 0;
+        LoraTile tile{-1, 0, 0};
+        int rank = 0;
         for (int u = u_beg; u < u_end && !*abort_flag; ++u) {
-            const int rank = rank_of(a, lora_tile<kTcNT>(a, pre, u / FB, 0).ad);
-            if (!mbar_wait(&b_full[st], ph, kTcWaitLimit)) { lora_timeout(abort_flag); break; }
-            if (rank & 15) {
-                for (int f = lane; f < 128; f += 32)
-                    for (int r = rank; r < ((rank + 15) & ~15); ++r)    // piece c of row f lies at c ^ f % 8
-                        *reinterpret_cast<unsigned short*>(smem + st * kTcABytes + f * 128 + (((r >> 3) ^ (f & 7)) << 4) + (r & 7) * 2) = 0;
+            if (u == u_beg || u % FB == 0) { tile = lora_tile<kTcNT>(a, pre, u / FB, 0); rank = rank_of(a, tile.ad); }
+            uint8_t* at = smem + st * kTcABytes;
+            if (tma) {
+                if (!mbar_wait(&b_full[st], ph, kTcWaitLimit)) { lora_timeout(abort_flag); break; }
+                if (rank & 15) {
+                    for (int f = lane; f < 128; f += 32)
+                        for (int r = rank; r < ((rank + 15) & ~15); ++r)    // piece c of row f lies at c ^ f % 8
+                            *reinterpret_cast<unsigned short*>(at + f * 128 + (((r >> 3) ^ (f & 7)) << 4) + (r & 7) * 2) = 0;
+                    fence_proxy_async();
+                }
+            } else {
+                if (!mbar_wait(&lin_full[ls], lph, kTcWaitLimit) || !mbar_wait(&b_empty[st], ph ^ 1u, kTcWaitLimit)) { lora_timeout(abort_flag); break; }
+                const int f0 = u % FB * 128;
+                const TcLin l = tc_lin(a, tile.ad, f0);
+                const uint32_t* s32 = reinterpret_cast<const uint32_t*>(s_lin + ls * kTcLinBytes);
+                const bool whole = (l.head + min(128, a.N - f0) * a.R) * 2 <= l.bytes;      // all but the last tile of B
+                for (int f = (warp - 2) * 64 + lane, k = 0; k < 2; ++k, f += 32) {
+                    const bool have = f0 + f < a.N;
+                    const int i0 = have ? l.head + f * a.R : 0;                 // the row's first element in the piece
+                    const uint32_t shift = (uint32_t)(i0 & 1) * 16;
+                    const uint32_t* src = s32 + (i0 >> 1);
+                    uint32_t low = src[0];
+                    for (int c = 0; c < (rank + 15) / 16 * 2; ++c) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {       // two elements at once, half a word on where the row starts odd
+                            const int r = c * 8 + j * 2;
+                            if (whole || !have) {
+                                const uint32_t high = src[(r >> 1) + 1];
+                                w[j] = __funnelshift_r(low, high, shift);
+                                low = high;
+                            } else {
+                                const unsigned short *in = reinterpret_cast<const unsigned short*>(s32), *out = reinterpret_cast<const unsigned short*>(l.src);
+                                w[j] = 0;
+                                for (int h = 0; h < 2; ++h)
+                                    if (r + h < rank) w[j] |= (uint32_t)((i0 + r + h + 1) * 2 <= l.bytes ? in[i0 + r + h] : out[i0 + r + h]) << (16 * h);
+                            }
+                            if (!have || r >= rank) w[j] = 0;
+                            else if (r + 1 == rank) w[j] &= 0xffffu;
+                        }
+                        *reinterpret_cast<uint4*>(at + f * 128 + ((c ^ (f & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
                 fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&lin_empty[ls]);
+                if (++ls == kTcLin) { ls = 0; lph ^= 1u; }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(&b_ready[st]);
             if (++st == kTcStages) { st = 0; ph ^= 1u; }
         }
+        if (!tma)
+            for (int j = 0; j < kTcStages && !*abort_flag; ++j) {       // the last MMAs' signals have arrived
+                mbar_wait(&b_empty[st], ph ^ 1u, kTcWaitLimit);
+                if (++st == kTcStages) { st = 0; ph ^= 1u; }
+            }
     } else if (warp == 1) {                // ---- MMA issue
         const bool leader = tc5::elect_one();
         uint32_t st = 0, ph = 0, n = 0, vph = 0;
@@ -883,12 +962,13 @@ int run_expand_tc(const LoraArgs& a, cudaStream_t s) {
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return GSB_ERR_CUDA;
     const int sms = sm_count_of(dev);
-    if (!sms || cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tc_smem<T>()) != cudaSuccess) return GSB_ERR_CUDA;
+    const bool tma = a.R % 8 == 0;
+    if (!sms || cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)tc_smem<T>(false)) != cudaSuccess) return GSB_ERR_CUDA;
     const int64_t units = ((int64_t)(a.nA < a.P ? a.nA : a.P) + a.P / kTcNT) * ((a.N + 127) / 128);
     if (units >= (int64_t)1 << 31) return GSB_ERR_TOO_LARGE;
-    CUtensorMap tb;
-    if (!encode(&tb, a.B, std::is_same<T, __nv_bfloat16>::value, a.R, a.N, a.nA, 128)) return GSB_ERR_CUDA;
-    return launch_after(kernel, dim3((unsigned)(units < sms ? units : sms)), kTcThreads, tc_smem<T>(), 1, s, a, tb);
+    CUtensorMap tb{};
+    if (tma && !encode(&tb, a.B, std::is_same<T, __nv_bfloat16>::value, a.R, a.N, a.nA, 128)) return GSB_ERR_CUDA;
+    return launch_after(kernel, dim3((unsigned)(units < sms ? units : sms)), kTcThreads, tc_smem<T>(tma), 1, s, a, tb, (int)tma);
 }
 
 template <typename T, typename Y>
@@ -905,11 +985,11 @@ int run_lora(const LoraArgs& a, cudaStream_t s) {
     // reads of B above (rank 16, 8192 rows of 6144: 111 us against 135 and 120).  tcgen05 where fp32 outputs and the rank
     // are large (rank 64, 8192 rows of 6144: 103 us against 165; rank 32: 99 and 133; 16-bit y: 116 and 106) and for
     // outputs whose rows are not 16-byte pieces, which the others take value by value (8192 rows of 3941, rank 16: 75 us
-    // against 217).
+    // against 217; rank 49: 125 and 213).
     const int64_t outputs = (int64_t)a.P * a.N;
-    const bool pieces = expand_flags<Y>(a) & 2;
-    const int64_t enough = !pieces ? 5 << 19 : sizeof(Y) == 4 && a.R > 32 ? 6 << 20 : sizeof(Y) == 4 && a.R > 16 ? 12 << 20 : INT64_MAX;
-    if (a.R <= 64 && a.R % 8 == 0 && !misaligned(a.B, 16) && outputs >= enough) return run_expand_tc<T, Y>(a, s);
+    const bool pieces = expand_flags<Y>(a) & 2, rows8 = a.R % 8 == 0;
+    const int64_t enough = !pieces ? 5 << 19 : sizeof(Y) == 2 ? INT64_MAX : a.R > 32 ? (rows8 ? 6 << 20 : 20 << 20) : a.R > 16 && rows8 ? 12 << 20 : INT64_MAX;
+    if (a.R <= 64 && !misaligned(a.B, 16) && outputs >= enough) return run_expand_tc<T, Y>(a, s);
     if (a.R > 64) return run_expand<T, Y, 1, 0>(a, s);
     if (wide && a.P >= 1024) return a.R <= 16 ? run_expand<T, Y, 2, 1>(a, s) : run_expand<T, Y, 2, 0>(a, s);
     return a.R <= 16 ? run_expand<T, Y, 1, 1>(a, s) : a.R <= 32 ? run_expand<T, Y, 1, 2>(a, s) : run_expand<T, Y, 1, 4>(a, s);

@@ -57,6 +57,9 @@ CASES = [  # n, K, N, adapters, R, ranks, share without an adapter
     (4500, 72, 5900, 9, 32, "zeros", 0.2),
     (1210, 64, 5260, 40, 40, None, 0.0),
     (1050, 128, 200, 3, 200, "mixed", 0.0),
+    (1300, 72, 2055, 3, 33, "mixed", 0.1),      # tcgen05, B laid out by hand
+    (700, 72, 3941, 5, 7, None, 0.1),
+    (600, 136, 4501, 2, 61, "zeros", 0.0),
 ]
 
 
