@@ -136,11 +136,13 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
     tc5::fence_before();
     descending = __syncthreads_or(descending);
     tc5::fence_after();
+    if (S > 1) tc5::cluster_arrive();      // this block runs, and s_xch is no longer the scan's
     const uint32_t tmem = *tmem_slot;
     const int nkb = (a.K + 63) >> 6;
     // at most (E + P / 16) token tiles, and so many items as the host has checked to fit; a list that descends is no list
     const int tiles = descending ? 0 : pre[a.E];
-    const int w = S == 1 && tiles * ((a.N + (GU ? 63 : 127)) / (GU ? 64 : 128)) * 2 <= (int)gridDim.x ? 64 : 128;   // weight rows of an item
+    const int64_t wide = (int64_t)tiles * ((a.N + (GU ? 63 : 127)) / (GU ? 64 : 128));
+    const int w = S == 1 && wide * 2 <= (int)gridDim.x ? 64 : 128;      // weight rows of an item
     const int fw = GU ? w / 2 : w;         // output features of an item
     const int FB = (a.N + fw - 1) / fw;
     const int items = tiles * FB;
@@ -157,15 +159,17 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
         return __ballot_sync(0xffffffffu, r >= 0 && r < a.n);
     };
 
+    bool met = false;                      // S > 1: whether this warp has waited for the cluster's first meeting
+
     if (warp == 0) {                       // ---- weights
         const bool leader = tc5::elect_one();
         uint32_t st = 0, ph = 0;
         int e = 0;
         bool dead = false;
-        for (int i = first; i < items && !dead && !*abort_flag; i += step) {
+        for (int i = first; i < items && !dead && !tc5::warp_set(abort_flag); i += step) {
             const GrItem it = gr_item(offsets, a.P, pre, i, FB, fw, e);
             for (int kb = kb0; kb < kb1; kb += kKps) {
-                if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
+                if (!tc5::warp_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
                 if (leader) {
                     const int nk = min(kKps, kb1 - kb);
                     mbar_arrive_expect_tx(&full[st], (uint32_t)(nk * w * 128));
@@ -178,19 +182,18 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
                 }
                 if (++st == (uint32_t)stages) { st = 0; ph ^= 1u; }
             }
-            dead = __any_sync(0xffffffffu, dead);
         }
         // the signals of the last MMAs have arrived before the block ends
-        for (int j = 0; j < stages && !*abort_flag; ++j) {
-            mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit);
+        for (int j = 0; j < stages && !tc5::warp_set(abort_flag); ++j) {
+            tc5::warp_wait(&empty[st], ph ^ 1u, kGrWaitLimit);
             if (++st == (uint32_t)stages) { st = 0; ph ^= 1u; }
         }
         // after a time-out: nothing may still be copying into this block's memory when it ends
-        if (*abort_flag)
+        if (tc5::warp_set(abort_flag))
             for (int j = 0; j < stages; ++j) {
                 if (st == 0) { st = (uint32_t)stages; ph ^= 1u; }
                 --st;
-                mbar_wait(&full[st], ph, kGrWaitLimit / 16);
+                tc5::warp_wait(&full[st], ph, kGrWaitLimit / 16);
             }
     } else if (warp >= 8) {                // ---- token rows: the four warps take stages in turn
         // eight lanes copy the 128 bytes of a row's k-block; a warp fences its copies before it hands the stage over, and
@@ -200,7 +203,7 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
         uint32_t st = 0, ph = 0, cnt = 0;
         int e = 0;
         bool dead = false;
-        for (int i = first; i < items && !dead && !*abort_flag; i += step) {
+        for (int i = first; i < items && !dead && !tc5::warp_set(abort_flag); i += step) {
             const GrItem it = gr_item(offsets, a.P, pre, i, FB, fw, e);
             int r[kNT / 4];
 #pragma unroll
@@ -216,7 +219,7 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
             }
             for (int kb = kb0; kb < kb1; kb += kKps, ++cnt) {
                 if ((int)(cnt % kTokWarps) == group) {
-                    if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
+                    if (!tc5::warp_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
                     const uint32_t base = smem_u32(smem) + st * stage_bytes + kKps * abytes + (uint32_t)((lane >> 3) * 128);
 #pragma unroll
                     for (int u = 0; u < kKps; ++u) {
@@ -236,7 +239,6 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
                 }
                 if (++st == (uint32_t)stages) { st = 0; ph ^= 1u; }
             }
-            dead = __any_sync(0xffffffffu, dead);
         }
         tc5::cp_async_wait<0>();
     } else if (warp == 1) {                // ---- MMA issue
@@ -246,13 +248,13 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
         constexpr uint32_t idesc_ab = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
         const uint32_t idesc = tc5::idesc_f16(idesc_ab, 128, kNT);
         const uint64_t d0 = tc5::desc_sw128(smem_u32(smem));
-        for (int i = first; i < items && !dead && !*abort_flag; i += step, ++tl) {
+        for (int i = first; i < items && !dead && !tc5::warp_set(abort_flag); i += step, ++tl) {
             const uint32_t buf = tl & 1u;
-            if (!mbar_wait(&acc_empty[buf], ((tl >> 1) & 1u) ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); break; }
+            if (!tc5::warp_wait(&acc_empty[buf], ((tl >> 1) & 1u) ^ 1u, kGrWaitLimit)) { gr_timeout(abort_flag); break; }
             tc5::fence_after();
             uint32_t acc = 0;
             for (int kb = kb0; kb < kb1; kb += kKps) {
-                if (!mbar_wait(&full[st], ph, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
+                if (!tc5::warp_wait(&full[st], ph, kGrWaitLimit)) { gr_timeout(abort_flag); dead = true; break; }
                 tc5::fence_after();
                 if (leader) {
                     const uint64_t ad = d0 + (uint64_t)(st * (uint32_t)(stage_bytes >> 4));
@@ -269,7 +271,6 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
                 acc = 1u;
                 if (++st == (uint32_t)stages) { st = 0; ph ^= 1u; }
             }
-            dead = __any_sync(0xffffffffu, dead);
             if (!dead && leader) tc5::commit(&acc_full[buf]);
         }
     } else if (warp >= 4) {                // ---- epilogue: this thread's TMEM lane = weight row
@@ -280,7 +281,7 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
         for (int i = first; i < items; i += step, ++tl) {
             const GrItem it = gr_item(offsets, a.P, pre, i, FB, fw, e);
             const uint32_t buf = tl & 1u;
-            int ok = *abort_flag ? 0 : (int)mbar_wait(&acc_full[buf], (tl >> 1) & 1u, kGrWaitLimit);
+            int ok = tc5::warp_set(abort_flag) ? 0 : (int)tc5::warp_wait(&acc_full[buf], (tl >> 1) & 1u, kGrWaitLimit);
             if (!ok) gr_timeout(abort_flag);
             // all four warps must agree to go on: they meet at a barrier below
             if (GU) ok = epilogue_agree(ok, 1);
@@ -295,6 +296,9 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
             if (lane == 0) mbar_arrive(&acc_empty[buf]);
             if (S > 1) {                   // to the block that finishes the column: [source][column][row]
                 const int per = kNT / S;
+                __syncwarp();
+                if (!met) tc5::cluster_wait();
+                met = true;                // (one item per cluster)
 #pragma unroll
                 for (int j = 0; j < kNT; ++j)
                     tc5::st_cluster(tc5::map_rank(smem_u32(s_xch + (rank * per + j % per) * 128 + row), (uint32_t)(j / per)), __uint_as_float(u[j]));
@@ -319,9 +323,10 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
     }
     __syncwarp();
     tc5::fence_before();
-    if (S > 1) {                           // (one item per cluster)
+    if (S > 1) {
+        if (!met) tc5::cluster_wait();
         tc5::cluster_sync_all();
-        if (first < items && warp >= 4 && warp < 8 && !*abort_flag) {
+        if (first < items && warp >= 4 && warp < 8 && !tc5::warp_set(abort_flag)) {
             int e = 0;
             const GrItem it = gr_item(offsets, a.P, pre, first, FB, fw, e);
             const uint32_t live = live_tokens(it);
@@ -503,7 +508,7 @@ extern "C" int gsb_grouped_gemm(const void* x, const void* w, int type, const in
     if (misaligned(x, 16) || misaligned(w, 16) || misaligned(expert_offsets, 4) || misaligned(rows, 4) ||
         misaligned(y, type_bytes(y_type)))
         return GSB_ERR_INVALID_ARG;
-    if (in % 8 || E > 1024 || P > kMaxSlots) return GSB_ERR_UNSUPPORTED;
+    if (in % 8 || E > 1024 || P > kMaxSlots || in > kMaxDim || out > kMaxDim) return GSB_ERR_UNSUPPORTED;
     const size_t need = rows ? gsb_grouped_gemm_workspace_bytes(P, in, E) : 0;
     if (need && (!workspace || misaligned(workspace, 256))) return GSB_ERR_INVALID_ARG;
     if (need > workspace_bytes) return GSB_ERR_WORKSPACE;
@@ -529,7 +534,8 @@ extern "C" int gsb_moe_expert_ffn_w16(const void* x, const int* topk_ids, const 
     if (misaligned(x, 16) || misaligned(gate_w, 16) || misaligned(up_w, 16) || misaligned(down_w, 16) ||
         misaligned(out, 16) || misaligned(topk_ids, 4) || misaligned(topk_weights, 4))
         return GSB_ERR_INVALID_ARG;
-    if (hidden % 8 || moe_inter % 8 || E > 1024 || (int64_t)n * topk > kMaxSlots) return GSB_ERR_UNSUPPORTED;
+    if (hidden % 8 || moe_inter % 8 || E > 1024 || (int64_t)n * topk > kMaxSlots || hidden > kMaxDim || moe_inter > kMaxDim)
+        return GSB_ERR_UNSUPPORTED;
     if (!workspace || misaligned(workspace, 256)) return GSB_ERR_INVALID_ARG;
     const Ffn16Ws ws = carve16(n, topk, hidden, moe_inter, E, workspace);
     if (workspace_bytes < ws.total) return GSB_ERR_WORKSPACE;

@@ -118,11 +118,11 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
         uint32_t st = 0, ph = 0;
         int e = 0;
         bool dead = false;
-        for (int i = first; i < items && !dead && !*abort_flag; i += step) {
+        for (int i = first; i < items && !dead && !tc5::warp_set(abort_flag); i += step) {
             const GrItem it = pr_item(a, pre, i, FB, fw, e);
             const int nb = ((it.cnt + 31) / 32 * 16 + 31) / 32;         // token boxes of 32 rows per CTA
             for (int kb = 0; kb < nkb; ++kb) {
-                if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { pr_timeout(abort_flag); dead = true; break; }
+                if (!tc5::warp_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { pr_timeout(abort_flag); dead = true; break; }
                 if (leader) {
                     if (rank == 0) mbar_arrive_expect_tx(&full[st], 2u * (kPrHalf + (uint32_t)nb * 4096u));
                     const uint32_t bar = tc5::map_rank(smem_u32(&full[st]), 0);
@@ -132,30 +132,29 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
                 }
                 if (++st == kPrStages) { st = 0; ph ^= 1u; }
             }
-            dead = __any_sync(0xffffffffu, dead);
         }
         // the signals of the last MMAs have arrived before the block ends
-        for (int j = 0; j < kPrStages && !*abort_flag; ++j) {
-            mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit);
+        for (int j = 0; j < kPrStages && !tc5::warp_set(abort_flag); ++j) {
+            tc5::warp_wait(&empty[st], ph ^ 1u, kGrWaitLimit);
             if (++st == kPrStages) { st = 0; ph ^= 1u; }
         }
         // after a time-out: nothing may still be copying into this block's memory when it ends
-        if (*abort_flag && rank == 0)
+        if (tc5::warp_set(abort_flag) && rank == 0)
             for (int j = 0; j < kPrStages; ++j) {
                 if (st == 0) { st = kPrStages; ph ^= 1u; }
                 --st;
-                mbar_wait(&full[st], ph, kGrWaitLimit / 16);
+                tc5::warp_wait(&full[st], ph, kGrWaitLimit / 16);
             }
     } else if (warp == 3) {                // ---- this CTA's half of the token rows
         const bool leader = tc5::elect_one();
         uint32_t st = 0, ph = 0;
         int e = 0;
         bool dead = false;
-        for (int i = first; i < items && !dead && !*abort_flag; i += step) {
+        for (int i = first; i < items && !dead && !tc5::warp_set(abort_flag); i += step) {
             const GrItem it = pr_item(a, pre, i, FB, fw, e);
             const int half = (it.cnt + 31) / 32 * 16, nb = (half + 31) / 32;
             for (int kb = 0; kb < nkb; ++kb) {
-                if (!mbar_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { pr_timeout(abort_flag); dead = true; break; }
+                if (!tc5::warp_wait(&empty[st], ph ^ 1u, kGrWaitLimit)) { pr_timeout(abort_flag); dead = true; break; }
                 if (leader) {
                     const uint32_t bar = tc5::map_rank(smem_u32(&full[st]), 0);
                     for (int b = 0; b < nb; ++b)
@@ -163,7 +162,6 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
                 }
                 if (++st == kPrStages) { st = 0; ph ^= 1u; }
             }
-            dead = __any_sync(0xffffffffu, dead);
         }
     } else if (warp == 1) {                // ---- MMA issue for the pair
         if (rank == 0) {
@@ -173,15 +171,15 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
             bool dead = false;
             constexpr uint32_t ab = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
             const uint64_t d0 = tc5::desc_sw128(smem_u32(smem));
-            for (int i = first; i < items && !dead && !*abort_flag; i += step, ++tl) {
+            for (int i = first; i < items && !dead && !tc5::warp_set(abort_flag); i += step, ++tl) {
                 const GrItem it = pr_item(a, pre, i, FB, fw, e);
                 const uint32_t buf = tl & 1u;
-                if (!tc5::wait_cluster(&acc_empty[buf], ((tl >> 1) & 1u) ^ 1u, kGrWaitLimit)) { pr_timeout(abort_flag); break; }
+                if (!tc5::warp_wait_cluster(&acc_empty[buf], ((tl >> 1) & 1u) ^ 1u, kGrWaitLimit)) { pr_timeout(abort_flag); break; }
                 tc5::fence_after();
                 const uint32_t idesc = tc5::idesc_f16(ab, 256, (uint32_t)((it.cnt + 31) & ~31));
                 uint32_t acc = 0;
                 for (int kb = 0; kb < nkb; ++kb) {
-                    if (!tc5::wait_cluster(&full[st], ph, kGrWaitLimit)) { pr_timeout(abort_flag); dead = true; break; }
+                    if (!tc5::warp_wait_cluster(&full[st], ph, kGrWaitLimit)) { pr_timeout(abort_flag); dead = true; break; }
                     tc5::fence_after();
                     if (leader) {
                         const uint64_t ad = d0 + (uint64_t)(st * (uint32_t)(kPrStageBytes >> 4));
@@ -194,7 +192,6 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
                     acc = 1u;
                     if (++st == kPrStages) { st = 0; ph ^= 1u; }
                 }
-                dead = __any_sync(0xffffffffu, dead);
                 if (!dead && leader) tc5::commit2(&acc_full[buf]);
             }
         }
@@ -208,7 +205,7 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
         for (int i = first; i < items; i += step, ++tl) {
             const GrItem it = pr_item(a, pre, i, FB, fw, e);
             const uint32_t buf = tl & 1u;
-            int ok = *abort_flag ? 0 : (int)mbar_wait(&acc_full[buf], (tl >> 1) & 1u, kGrWaitLimit);
+            int ok = tc5::warp_set(abort_flag) ? 0 : (int)tc5::warp_wait(&acc_full[buf], (tl >> 1) & 1u, kGrWaitLimit);
             if (!ok) pr_timeout(abort_flag);
             // the group's four warps must agree to go on: they meet at a barrier in the loop below
             if (GU) ok = epilogue_agree(ok, bar);

@@ -672,9 +672,9 @@ lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b
         const uint32_t ring = tma ? kTcStages : kTcLin;
         uint64_t *fullb = tma ? b_full : lin_full, *emptyb = tma ? b_empty : lin_empty;
         LoraTile tile{-1, 0, 0};
-        for (int u = u_beg; u < u_end && !*abort_flag; ++u) {
+        for (int u = u_beg; u < u_end && !tc5::warp_set(abort_flag); ++u) {
             if (u == u_beg || u % FB == 0) tile = lora_tile<kTcNT>(a, pre, u / FB, 0);
-            if (!mbar_wait(&emptyb[st], ph ^ 1u, kTcWaitLimit)) { lora_timeout(abort_flag); break; }
+            if (!tc5::warp_wait(&emptyb[st], ph ^ 1u, kTcWaitLimit)) { lora_timeout(abort_flag); break; }
             if (leader) {
                 const int f0 = u % FB * 128;
                 if (tma) {
@@ -688,26 +688,26 @@ lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b
             }
             if (++st == ring) { st = 0; ph ^= 1u; }
         }
-        for (uint32_t j = 0; j < ring && !*abort_flag; ++j) {           // the last tiles are done with, their signals in
-            mbar_wait(&emptyb[st], ph ^ 1u, kTcWaitLimit);
+        for (uint32_t j = 0; j < ring && !tc5::warp_set(abort_flag); ++j) {           // the last tiles are done with, their signals in
+            tc5::warp_wait(&emptyb[st], ph ^ 1u, kTcWaitLimit);
             if (++st == ring) { st = 0; ph ^= 1u; }
         }
-        if (*abort_flag)                   // after a time-out: nothing may still be copying when the block ends
+        if (tc5::warp_set(abort_flag))                   // after a time-out: nothing may still be copying when the block ends
             for (uint32_t j = 0; j < ring; ++j) {
                 if (st == 0) { st = ring; ph ^= 1u; }
                 --st;
-                mbar_wait(&fullb[st], ph, kTcWaitLimit / 16);
+                tc5::warp_wait(&fullb[st], ph, kTcWaitLimit / 16);
             }
     } else if (warp == 2 || (warp == 3 && !tma)) {
         // ---- tma: zeroes between an adapter's rank and the next multiple of 16; else: the tile laid out, a warp 64 rows
         uint32_t st = 0, ph = 0, ls = 0, lph = 0;
         LoraTile tile{-1, 0, 0};
         int rank = 0;
-        for (int u = u_beg; u < u_end && !*abort_flag; ++u) {
+        for (int u = u_beg; u < u_end && !tc5::warp_set(abort_flag); ++u) {
             if (u == u_beg || u % FB == 0) { tile = lora_tile<kTcNT>(a, pre, u / FB, 0); rank = rank_of(a, tile.ad); }
             uint8_t* at = smem + st * kTcABytes;
             if (tma) {
-                if (!mbar_wait(&b_full[st], ph, kTcWaitLimit)) { lora_timeout(abort_flag); break; }
+                if (!tc5::warp_wait(&b_full[st], ph, kTcWaitLimit)) { lora_timeout(abort_flag); break; }
                 if (rank & 15) {
                     for (int f = lane; f < 128; f += 32)
                         for (int r = rank; r < ((rank + 15) & ~15); ++r)    // piece c of row f lies at c ^ f % 8
@@ -715,7 +715,7 @@ lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b
                     fence_proxy_async();
                 }
             } else {
-                if (!mbar_wait(&lin_full[ls], lph, kTcWaitLimit) || !mbar_wait(&b_empty[st], ph ^ 1u, kTcWaitLimit)) { lora_timeout(abort_flag); break; }
+                if (!tc5::warp_wait(&lin_full[ls], lph, kTcWaitLimit) || !tc5::warp_wait(&b_empty[st], ph ^ 1u, kTcWaitLimit)) { lora_timeout(abort_flag); break; }
                 const int f0 = u % FB * 128;
                 const TcLin l = tc_lin(a, tile.ad, f0);
                 const uint32_t* s32 = reinterpret_cast<const uint32_t*>(s_lin + ls * kTcLinBytes);
@@ -757,8 +757,8 @@ lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b
             if (++st == kTcStages) { st = 0; ph ^= 1u; }
         }
         if (!tma)
-            for (int j = 0; j < kTcStages && !*abort_flag; ++j) {       // the last MMAs' signals have arrived
-                mbar_wait(&b_empty[st], ph ^ 1u, kTcWaitLimit);
+            for (int j = 0; j < kTcStages && !tc5::warp_set(abort_flag); ++j) {       // the last MMAs' signals have arrived
+                tc5::warp_wait(&b_empty[st], ph ^ 1u, kTcWaitLimit);
                 if (++st == kTcStages) { st = 0; ph ^= 1u; }
             }
     } else if (warp == 1) {                // ---- MMA issue
@@ -768,15 +768,15 @@ lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b
         const uint64_t b0 = tc5::desc_sw128(smem_u32(smem)), v0 = tc5::desc_sw128(smem_u32(s_vp));
         LoraTile tile{-1, 0, 0};
         int kgs = 0;
-        for (int u = u_beg; u < u_end && !*abort_flag; ++u, ++n) {
+        for (int u = u_beg; u < u_end && !tc5::warp_set(abort_flag); ++u, ++n) {
             if (u == u_beg || u % FB == 0) {
                 tile = lora_tile<kTcNT>(a, pre, u / FB, 0);
                 kgs = (rank_of(a, tile.ad) + 15) / 16;
-                if (!mbar_wait(v_full, vph, kTcWaitLimit)) { lora_timeout(abort_flag); break; }
+                if (!tc5::warp_wait(v_full, vph, kTcWaitLimit)) { lora_timeout(abort_flag); break; }
                 vph ^= 1u;
             }
             const uint32_t slot = n % kTcGroups;
-            if (!mbar_wait(&b_ready[st], ph, kTcWaitLimit) || !mbar_wait(&acc_empty[slot], ((n / kTcGroups) & 1u) ^ 1u, kTcWaitLimit)) {
+            if (!tc5::warp_wait(&b_ready[st], ph, kTcWaitLimit) || !tc5::warp_wait(&acc_empty[slot], ((n / kTcGroups) & 1u) ^ 1u, kTcWaitLimit)) {
                 lora_timeout(abort_flag);
                 break;
             }
@@ -838,7 +838,7 @@ lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b
             auto finish = [&](const float (&v)[16]) {
                 const int n = now.u - u_beg;
                 if (now.c0 == 0) {
-                    if (*abort_flag || !mbar_wait(&acc_full[group], (n / kTcGroups) & 1u, kTcWaitLimit)) {
+                    if (tc5::warp_set(abort_flag) || !tc5::warp_wait(&acc_full[group], (n / kTcGroups) & 1u, kTcWaitLimit)) {
                         if (!*abort_flag) lora_timeout(abort_flag);
                     }
                     tc5::fence_after();
@@ -1025,7 +1025,7 @@ extern "C" int gsb_lora_add(const void* x, const void* A, const void* B, int typ
     if (misaligned(x, 16) || misaligned(A, 16) || misaligned(B, 2) || misaligned(y, y_type == GSB_TYPE_F32 ? 4 : 2) ||
         misaligned(adapter_offsets, 4) || misaligned(rows, 4) || misaligned(ranks, 4) || misaligned(scales, 4))
         return GSB_ERR_INVALID_ARG;
-    if (in % 8 || max_rank > kMaxRank || n_adapters > 1024) return GSB_ERR_UNSUPPORTED;
+    if (in % 8 || max_rank > kMaxRank || n_adapters > 1024 || in > kMaxDim || out > kMaxDim || P > kMaxDim) return GSB_ERR_UNSUPPORTED;
     const size_t need = gsb_lora_scratch_bytes(P, max_rank, n_adapters);
     if (need && (!scratch || misaligned(scratch, 256))) return GSB_ERR_INVALID_ARG;
     if (scratch_bytes < need) return GSB_ERR_WORKSPACE;

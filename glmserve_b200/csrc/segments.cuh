@@ -18,11 +18,12 @@ template <> __device__ __forceinline__ __half from_f(float v) { return __float2h
 template <typename T> __device__ __forceinline__ T h_from_f(float v) { return from_f<T>(v); }
 template <> __device__ __forceinline__ __half h_from_f(float v) { return sat_half(v); }
 
-// Segment bounds as read from device memory, forced into [0, P]: a list that is not ascending gives wrong rows,
-// never an access outside the buffers.
+// Segment bounds as read from device memory, forced into [0, P], so that no list leads outside the buffers; the
+// kernels write nothing for one that descends.
 __device__ __forceinline__ int seg_bound(const int* offsets, int e, int P) { return min(max(offsets[e], 0), P); }
 
 constexpr int kMaxE = 1024;     // segments at most
+constexpr int kMaxDim = 1 << 30;    // of a row; sums of a dimension and a tile stay ints
 
 // The walk over the segments: the first 256 threads hold four segments each (n[j] = rows of segment 4 tid + j), all call.
 // Returns non-zero in a thread that saw the list descend.
@@ -101,7 +102,9 @@ inline int launch_after(K kernel, dim3 grid, int threads, size_t smem, int clust
     at[1].id = cudaLaunchAttributeClusterDimension;
     at[1].val.clusterDim.x = (unsigned)cluster; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
     cfg.attrs = at; cfg.numAttrs = cluster > 1 ? 2 : 1;
-    return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? GSB_OK : GSB_ERR_LAUNCH;
+    if (cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess) return GSB_OK;
+    cudaGetLastError();     // the status says it; a later call must not find it again
+    return GSB_ERR_LAUNCH;
 }
 
 inline bool misaligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a != 0; }

@@ -70,12 +70,6 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* tmap, 
         "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
         ::"r"(smem_u32(dst)), "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
 }
-// Four rows of a 2-D tensor (box one row high), 128 bytes each, to consecutive shared-memory rows.
-__device__ __forceinline__ void tma_gather4(void* dst, const CUtensorMap* tmap, int x, int r0, int r1, int r2, int r3, uint64_t* bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-        ::"r"(smem_u32(dst)), "l"(tmap), "r"(smem_u32(bar)), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3) : "memory");
-}
 
 // ---- two CTAs on one tile (cta_group::2) -------------------------------------------------------
 __device__ __forceinline__ void tmem_alloc2(uint32_t* smem_dst, uint32_t ncols) {
@@ -168,6 +162,17 @@ __device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, lon
         if (clock64() - start > limit_cycles) return false;
     return true;
 }
+
+// The bounded waits for a whole warp: all lanes go on or none does, so that a time-out cannot leave part of a warp behind
+// at its next meeting.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, long long limit_cycles) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, limit_cycles));
+}
+__device__ __forceinline__ bool warp_wait_cluster(uint64_t* bar, uint32_t parity, long long limit_cycles) {
+    return __all_sync(0xffffffffu, wait_cluster(bar, parity, limit_cycles));
+}
+// a flag of the block that other warps may set at any time, read alike by all lanes
+__device__ __forceinline__ bool warp_set(const volatile int* flag) { return __any_sync(0xffffffffu, *flag); }
 
 }  // namespace tc5
 
