@@ -900,7 +900,8 @@ inline bool lora_one_launch(int P, int R, int nA) { return R <= 32 && (nA < P ? 
 // spread until two blocks per SM have work.
 inline bool lora_wide(int P, int nA) { return P > 8 * (int64_t)nA; }
 inline int lora_split(int P, int nA) {
-    const int64_t tiles = (nA < P ? nA : P) + P / (lora_wide(P, nA) ? kWdRows : 8);
+    // (a tile per adapter is begun and on average half filled)
+    const int64_t tiles = lora_wide(P, nA) ? nA / 2 + (P + kWdRows - 1) / kWdRows : (nA < P ? nA : P) + P / 8;
     const int64_t s = 296 / tiles;
     return s < 1 ? 1 : s > kMaxSplit ? kMaxSplit : (int)s;
 }
