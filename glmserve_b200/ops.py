@@ -174,7 +174,7 @@ def moe_expert_ffn_w16(x, topk_ids, topk_w, gate_w, up_w, down_w, out=None, out_
                          "of torch.bfloat16 or all of torch.float16, ids of torch.int32, w of torch.float32")
     n, H = x.shape
     E, I, Hw = gate_w.shape
-    topk = topk_ids.shape[1]
+    topk = topk_ids.shape[-1] if topk_ids.dim() else 0
     if Hw != H or up_w.shape != gate_w.shape or down_w.shape != (E, H, I) or topk_ids.shape != (n, topk) or \
             topk_w.shape != topk_ids.shape:
         raise ValueError("moe_expert_ffn_w16: expected gate_w, up_w [E,I,H], down_w [E,H,I], ids and w [n,topk]")

@@ -304,7 +304,7 @@ def test_expert16_graph_replay_and_two_streams(dev):
         out.zero_(), y.zero_()
         graph.replay()
         assert torch.equal(out, ops.moe_expert_ffn_w16(x, *b[1:])) and torch.equal(y, ops.grouped_gemm(x, b[3], offs, rows=tok))
-    assert torch.equal(out, out) and ops.operators16_status() == 0
+    assert ops.operators16_status() == 0
 
 
 def test_empty_batches(dev):
@@ -315,3 +315,65 @@ def test_empty_batches(dev):
     assert ops.grouped_gemm(x0, w, offs).shape == (0, 32)
     ids, wt = torch.empty((0, 2), dtype=torch.int32, device=dev), torch.empty((0, 2), device=dev)
     assert ops.moe_expert_ffn_w16(x0, ids, wt, w, w, w.transpose(1, 2).contiguous()).shape == (0, 64)
+
+
+@pytest.mark.parametrize("P", [900, 18000])             # few rows per expert, and many
+def test_grouped_gemm_of_1024_experts(dev, P):
+    from glmserve_b200 import ops
+    rng = np.random.default_rng(P)
+    counts = np.bincount(rng.integers(0, 1024, P), minlength=1024)
+    counts[-1] += 1                                      # the last expert has a row
+    P = int(counts.sum())
+    x, w = _randn((300, 72), torch.bfloat16, dev, 5), _randn((1024, 40, 72), torch.bfloat16, dev, 6)
+    offs, rows = _offsets(counts, dev), _i32(rng.integers(0, 300, P), dev)
+    y = ops.grouped_gemm(x, w, offs, rows=rows, out_dtype=torch.float32)
+    ref, b, written = _grouped_ref(x, w, offs, rows)
+    assert written.all()
+    _check(y, ref, b + HALF[torch.float32] * ref.abs(), "1024 experts")
+
+
+@pytest.mark.parametrize("n", [32, 100])                 # lists made inside the product, and by the dispatch
+def test_expert_ffn_of_1024_experts(dev, n):
+    from glmserve_b200 import ops
+    E, topk, H, I = 1024, 8, 64, 40
+    x, wt = _randn((n, H), torch.bfloat16, dev, 1), _randn((n, topk), torch.float32, dev, 5)
+    gate, up = _randn((E, I, H), torch.bfloat16, dev, 2, 0.05), _randn((E, I, H), torch.bfloat16, dev, 3, 0.05)
+    down = _randn((E, H, I), torch.bfloat16, dev, 4, 0.05)
+    ids = _i32(np.random.default_rng(n).integers(0, E, (n, topk)), dev)
+    ids[0, 0] = E - 1
+    out = ops.moe_expert_ffn_w16(x, ids, wt, gate, up, down, out_dtype=torch.float32)
+    ref, b = _ffn_ref(x, ids, wt, gate, up, down, torch.bfloat16)
+    _check(out, ref, b + HALF[torch.float32] * ref.abs(), "1024 experts")
+
+
+@pytest.mark.parametrize("K,N,P", [(64, 130, 40), (4096, 64, 12), (264, 520, 300)])     # few rows, a cluster per item, many rows
+def test_grouped_gemm_bad_offsets_stay_inside(dev, K, N, P):
+    from glmserve_b200 import ops
+    x, w = _randn((P, K), torch.bfloat16, dev, 1), _randn((3, N, K), torch.bfloat16, dev, 2)
+    for rows in (None, torch.arange(P, dtype=torch.int32, device=dev)):
+        y = torch.full((P, N), 7.0, dtype=torch.bfloat16, device=dev)
+        ops.grouped_gemm(x, w, _i32([0, P, P // 2, P], dev), rows=rows, out=y)          # descends: nothing is written
+        assert bool((y == 7).all())
+        ops.grouped_gemm(x, w, _i32([-9, 2, 2, 2 ** 31 - 1], dev), rows=rows, out=y)    # clamped to [0, P]
+        want = ops.grouped_gemm(x, w, _i32([0, 2, 2, P], dev), rows=rows)
+        assert torch.equal(y, want)
+    assert ops.operators16_status() == 0
+
+
+def test_calls_of_different_kernels_follow_each_other(dev):
+    """Every kernel's launch may begin while the one ahead ends: 16-bit and int4 operators, small and large, in turn."""
+    from glmserve_b200 import ops
+    a, b, c = (_ffn_case(i, torch.bfloat16, dev) for i in (1, 6, 8))
+    offs, tok, _ = ops.moe_dispatch(b[1], b[3].shape[0])
+    one, three = ops.moe_expert_ffn_w16(*a), ops.moe_expert_ffn_w16(*c)
+    two, rows = ops.moe_expert_ffn_w16(*b), ops.grouped_gemm(b[0], b[3], offs, rows=tok)
+    x = a[0].clone()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        x.zero_()
+        x.copy_(a[0])
+        got = [ops.moe_expert_ffn_w16(x, *a[1:]), ops.moe_expert_ffn_w16(*c)]
+        x.zero_()                                        # after its last reader
+        o2, t2, _ = ops.moe_dispatch(b[1], b[3].shape[0])
+        got += [ops.grouped_gemm(b[0], b[3], o2, rows=t2), ops.moe_expert_ffn_w16(*b), ops.moe_expert_ffn_w16(*c)]
+        assert all(torch.equal(g, w) for g, w in zip(got, (one, three, rows, two, three)))

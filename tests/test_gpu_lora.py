@@ -164,3 +164,67 @@ def test_lora_empty_lists(dev):
     offs, rows, _ = ops.moe_dispatch(torch.full_like(ids, -1)[:, None].contiguous(), A.shape[0])
     assert torch.equal(ops.lora_add(y0.clone(), x, A, B, offs, rows), y0)
     assert torch.equal(ops.lora_add(y0.clone(), x, A, B, offs, rows[:0]), y0)
+
+
+def test_lora_of_1024_adapters(dev):
+    from glmserve_b200 import ops
+    for n in (1, 900, 9000):
+        x, A, B = _randn((n, 64), torch.bfloat16, dev, n), _randn((1024, 8, 64), torch.bfloat16, dev, 2, 0.1), _randn((1024, 40, 8), torch.bfloat16, dev, 3)
+        ids = _i32(np.random.default_rng(n).integers(0, 1024, n), dev)
+        ids[0] = 1023
+        offs, rows, _ = ops.moe_dispatch(ids[:, None].contiguous(), 1024)
+        y0 = _randn((n, 40), torch.float32, dev, 4)
+        y = ops.lora_add(y0.clone(), x, A, B, offs, rows)
+        ref, b = _ref(y0, x, A, B, offs, rows, None, None)
+        _check(y, ref, b + HALF[torch.float32] * (ref.abs() + b), "1024 adapters")
+
+
+SHAPES = [1, 6, 14, 15, 17, 21]       # one launch; two of each kind; tcgen05 with and without TMA
+
+
+@pytest.mark.parametrize("case", SHAPES + [3, 8])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_lora_nan_and_infinity_stay_in_their_row(dev, case, dtype):
+    from glmserve_b200 import ops
+    y0, x, A, B, ids, ranks, scales = _case(case, dtype, torch.float32, dev)
+    n = x.shape[0]
+    offs, rows, _ = ops.moe_dispatch(ids[:, None].contiguous(), A.shape[0])
+    want = ops.lora_add(y0.clone(), x, A, B, offs, rows, ranks=ranks, scales=scales)
+    bad = sorted({n // 2, n // 3})
+    for i, t in enumerate(bad):
+        x[t, i] = [float("nan"), float("inf")][i % 2]
+    y = ops.lora_add(y0.clone(), x, A, B, offs, rows, ranks=ranks, scales=scales)
+    keep = torch.ones(n, dtype=torch.bool, device=dev)
+    keep[bad] = False
+    assert torch.equal(y[keep], want[keep])
+    for t in bad:
+        if int(ids[t]) >= 0 and (ranks is None or int(ranks[int(ids[t])]) > 0):
+            assert not bool(torch.isfinite(y[t]).any())
+
+
+@pytest.mark.parametrize("case", SHAPES)
+@pytest.mark.parametrize("big", [3000.0, 2.0 ** -14])
+def test_lora_products_outside_fp16(dev, case, big):
+    """A x far beyond 65504, or below fp16's normal range, beside fp16 weights: it is never a 16-bit number by itself."""
+    from glmserve_b200 import ops
+    y0, x, A, B, ids, ranks, scales = _case(case, torch.float16, torch.float32, dev)
+    y0, x, A, B = y0 * 0, (x * big).clamp(-60000, 60000), A * (20.0 if big > 1 else 2.0 ** -6), B * 0.125
+    offs, rows, _ = ops.moe_dispatch(ids[:, None].contiguous(), A.shape[0])
+    y = ops.lora_add(y0.clone(), x, A, B, offs, rows, ranks=ranks, scales=scales)
+    ref, b = _ref(y0, x, A, B, offs, rows, ranks, scales)
+    assert bool(torch.isfinite(y).all())
+    _check(y, ref, b + HALF[torch.float32] * (ref.abs() + b), "scaled")
+
+
+@pytest.mark.parametrize("case", SHAPES)
+def test_lora_bad_offsets_stay_inside(dev, case):
+    from glmserve_b200 import ops
+    y0, x, A, B, ids, _, _ = _case(case, torch.bfloat16, torch.float32, dev)
+    A, B = torch.nan_to_num(A), torch.nan_to_num(B)
+    nA, n = A.shape[0], x.shape[0]
+    rows = torch.arange(n, dtype=torch.int32, device=dev)
+    y = y0.clone()
+    ops.lora_add(y, x, A, B, _i32([0, n, n - 1] + [n] * (nA - 2), dev), rows)          # descends: nothing is written
+    assert torch.equal(y, y0)
+    ops.lora_add(y, x, A, B, _i32([-5] + [0] * (nA - 1) + [2 ** 31 - 1], dev), rows)    # clamped to [0, P]
+    assert torch.equal(y, ops.lora_add(y0.clone(), x, A, B, _i32([0] * nA + [n], dev), rows))
