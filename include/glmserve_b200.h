@@ -127,7 +127,7 @@ enum { GSB_TYPE_F32 = 0, GSB_TYPE_BF16 = 1, GSB_TYPE_F16 = 2 };
  * or F32).  Sums in fp32, one rounding at the end.  Rows of y that no segment covers, or whose rows[p] is outside
  * [0,n), are left as they were; an expert with an empty segment costs nothing.  Offsets are clamped to [0,P]; with
  * offsets that descend nothing is written.
- * in % 8 == 0, E <= 1024, P <= 2^30; x and w 16-byte aligned; y must not overlap the inputs.  workspace: with a row
+ * in % 8 == 0, E <= 1024, P, in and out <= 2^30; x and w 16-byte aligned; y must not overlap the inputs.  workspace: with a row
  * list gsb_grouped_gemm_workspace_bytes() bytes (0 for few rows per expert: then it may be NULL), 256-byte aligned, any
  * contents; two calls that may overlap on the GPU need a workspace each. */
 GSB_API size_t gsb_grouped_gemm_workspace_bytes(int P, int in, int E);
@@ -140,7 +140,7 @@ GSB_API int gsb_grouped_gemm(const void* x, const void* w, int type, const int* 
  * [E,moe_inter,hidden], down_w [E,hidden,moe_inter] of `type`; out [n,hidden] of out_type (`type`, or F32) is
  * OVERWRITTEN.  A slot whose id is outside [0,E) adds nothing (padding, or an expert that lives on another GPU);
  * a token without a slot gets zeros.  Sums in fp32; silu(gate x) * up x is rounded once to `type`, in fp16
- * saturating at +-65504.  hidden and moe_inter multiples of 8, E <= 1024, n * topk <= 2^30; all pointers but ids
+ * saturating at +-65504.  hidden and moe_inter multiples of 8, E <= 1024, n * topk and each dimension <= 2^30; all pointers but ids
  * and weights 16-byte aligned; workspace 256-byte aligned, any contents; two calls that may overlap on the GPU
  * need a workspace each. */
 GSB_API size_t gsb_moe_expert_ffn_w16_workspace_bytes(int n, int topk, int hidden, int moe_inter, int E);
@@ -158,7 +158,7 @@ GSB_API int gsb_moe_expert_ffn_w16(const void* x, const int* topk_ids, const flo
  * once per batch and used for every projection of the model; rows that no list names are left as they were, indices
  * outside [0,n) are skipped, a row must not be listed twice; y must not overlap the inputs.  A x is kept in fp32 and B
  * applied to it without rounding it to `type` (it enters the products in parts, so an infinity in B may give NaN); y is
- * rounded once.  in % 8 == 0, 1 <= max_rank <= 256, n_adapters <= 1024; x and A 16-byte aligned;
+ * rounded once.  in % 8 == 0, 1 <= max_rank <= 256, n_adapters <= 1024, P, in and out <= 2^30; x and A 16-byte aligned;
  * scratch of gsb_lora_scratch_bytes() bytes (0 for few rows: then it may be NULL), 256-byte aligned, any contents, not
  * shared by calls that may overlap. */
 GSB_API size_t gsb_lora_scratch_bytes(int P, int max_rank, int n_adapters);

@@ -25,6 +25,7 @@ def _grouped(x=P16, w=P16, type=1, offs=P16, rows=P16, n=4, P=4, inn=64, out=32,
     (dict(offs=0), INVALID), (dict(y=0), INVALID), (dict(x=P2), INVALID), (dict(w=P2), INVALID), (dict(y=ODD), INVALID),
     (dict(y=P2, yt=0), INVALID), (dict(offs=P2), INVALID), (dict(rows=P2), INVALID),
     (dict(inn=60), UNSUPPORTED), (dict(E=1025), UNSUPPORTED), (dict(P=(1 << 30) + 1), UNSUPPORTED),
+    (dict(inn=(1 << 30) + 8), UNSUPPORTED), (dict(out=(1 << 30) + 1), UNSUPPORTED),
     (dict(P=2000), INVALID), (dict(P=2000, ws=P16 + 16, nb=1 << 30), INVALID), (dict(P=2000, ws=P16, nb=64), WORKSPACE)])
 def test_grouped_gemm_refusals(kw, st):
     assert _grouped(**kw) == st
@@ -42,7 +43,7 @@ def _ffn(x=P16, ids=P16, wt=P16, g=P16, u=P16, d=P16, type=2, n=4, topk=2, H=64,
     (dict(wt=0), INVALID), (dict(g=0), INVALID), (dict(u=0), INVALID), (dict(d=0), INVALID), (dict(out=0), INVALID),
     (dict(ws=0), INVALID), (dict(ws=P16 + 16), INVALID), (dict(g=P2), INVALID), (dict(out=P2), INVALID),
     (dict(H=60), UNSUPPORTED), (dict(I=36), UNSUPPORTED), (dict(E=1025), UNSUPPORTED),
-    (dict(n=1 << 30, topk=2), UNSUPPORTED), (dict(nb=64), WORKSPACE)])
+    (dict(n=1 << 30, topk=2), UNSUPPORTED), (dict(H=(1 << 30) + 8), UNSUPPORTED), (dict(I=(1 << 30) + 8), UNSUPPORTED), (dict(nb=64), WORKSPACE)])
 def test_ffn_refusals(kw, st):
     assert _ffn(**kw) == st
 
@@ -60,7 +61,8 @@ def _lora(x=P16, A=P16, B=P16, type=1, offs=P16, rows=P16, ranks=0, scales=0, n=
     (dict(A=0), INVALID), (dict(B=0), INVALID), (dict(offs=0), INVALID), (dict(rows=0), INVALID), (dict(y=0), INVALID), (dict(y=P16), INVALID),
     (dict(x=P2), INVALID), (dict(A=P2), INVALID), (dict(B=ODD), INVALID), (dict(y=P2), INVALID), (dict(ranks=P2), INVALID),
     (dict(scales=P2), INVALID), (dict(n=9999, P=9999, sc=0), INVALID), (dict(n=9999, P=9999, sc=P16 + 16), INVALID),
-    (dict(inn=60), UNSUPPORTED), (dict(R=257), UNSUPPORTED), (dict(nA=1025), UNSUPPORTED), (dict(n=9999, P=9999, nb=64), WORKSPACE)])
+    (dict(inn=60), UNSUPPORTED), (dict(R=257), UNSUPPORTED), (dict(nA=1025), UNSUPPORTED), (dict(inn=(1 << 30) + 8), UNSUPPORTED),
+    (dict(out=(1 << 30) + 1), UNSUPPORTED), (dict(n=(1 << 30) + 1, P=(1 << 30) + 1), UNSUPPORTED), (dict(n=9999, P=9999, nb=64), WORKSPACE)])
 def test_lora_refusals(kw, st):
     assert _lora(**kw) == st
 
