@@ -14,9 +14,12 @@ template <typename T> __device__ __forceinline__ T from_f(float v);
 template <> __device__ __forceinline__ float from_f(float v) { return v; }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
-// h of the FFN: fp16 saturates instead of turning into infinity and then NaN in the next product
+// h of the FFN: a finite value beyond fp16 saturates instead of turning into infinity and then NaN in the next product;
+// infinities and NaN are the activations' own and go on (the minimum and maximum of a NaN would be the border)
 template <typename T> __device__ __forceinline__ T h_from_f(float v) { return from_f<T>(v); }
-template <> __device__ __forceinline__ __half h_from_f(float v) { return sat_half(v); }
+template <> __device__ __forceinline__ __half h_from_f(float v) {
+    return isfinite(v) ? sat_half(v) : __float2half_rn(v);
+}
 
 // Segment bounds as read from device memory, forced into [0, P], so that no list leads outside the buffers; the
 // kernels write nothing for one that descends.

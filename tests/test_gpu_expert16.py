@@ -377,3 +377,45 @@ def test_calls_of_different_kernels_follow_each_other(dev):
         o2, t2, _ = ops.moe_dispatch(b[1], b[3].shape[0])
         got += [ops.grouped_gemm(b[0], b[3], o2, rows=t2), ops.moe_expert_ffn_w16(*b), ops.moe_expert_ffn_w16(*c)]
         assert all(torch.equal(g, w) for g, w in zip(got, (one, three, rows, two, three)))
+
+
+# few rows per expert, a cluster of blocks per item, many rows per expert; and lists of more than 256 slots
+NONFINITE = [(4, 2, 4, 136, 72), (2, 2, 3, 4096, 200), (100, 2, 3, 264, 520), (150, 2, 3, 264, 520), (70, 4, 64, 136, 72)]
+
+
+@pytest.mark.parametrize("shape", NONFINITE)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_expert_ffn_nan_and_infinite_tokens_stay_in_their_row(dev, shape, dtype):
+    """A NaN reaches every gate sum of its token; an infinity makes gate sums of both signs, and silu(-inf) is NaN."""
+    from glmserve_b200 import ops
+    n, topk, E, H, I = shape
+    x = _randn((n, H), dtype, dev, 1)
+    gate, up, down = (_randn(s, dtype, dev, 2 + i, 0.05) for i, s in enumerate([(E, I, H), (E, I, H), (E, H, I)]))
+    rng = np.random.default_rng(n)
+    ids = _i32(np.stack([rng.permutation(E)[:topk] for _ in range(n)]), dev)
+    wt = torch.from_numpy((rng.random((n, topk)) + 0.1).astype(np.float32)).to(dev)
+    clean = ops.moe_expert_ffn_w16(x, ids, wt, gate, up, down)
+    for bad, value in ((n - 1, float("nan")), (n // 2, float("inf")), (0, -float("inf"))):
+        y = x.clone()
+        y[bad, H - 3] = value
+        out = ops.moe_expert_ffn_w16(y, ids, wt, gate, up, down)
+        assert bool(out[bad].isnan().all()), value
+        keep = [t for t in range(n) if t != bad]
+        assert torch.equal(out[keep], clean[keep])
+    assert bool(clean.isfinite().all())
+
+
+@pytest.mark.parametrize("shape", NONFINITE)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_expert_ffn_infinity_goes_through(dev, shape, dtype):
+    """Positive weights: an infinite activation gives an infinite gate, an infinite h and an infinite result."""
+    from glmserve_b200 import ops
+    n, topk, E, H, I = shape
+    x = _randn((n, H), dtype, dev, 1)
+    gate, up, down = (_randn(s, dtype, dev, 2 + i, 0.05).abs() + 0.01 for i, s in enumerate([(E, I, H), (E, I, H), (E, H, I)]))
+    ids = _i32(np.stack([np.random.default_rng(t).permutation(E)[:topk] for t in range(n)]), dev)
+    x[n // 2, 1] = float("inf")
+    out = ops.moe_expert_ffn_w16(x, ids, torch.ones((n, topk), device=dev), gate, up, down, out_dtype=torch.float32)
+    want = torch.zeros_like(out, dtype=torch.bool)
+    want[n // 2] = True
+    assert torch.equal(out == float("inf"), want) and not bool(out.isnan().any())
