@@ -247,25 +247,41 @@ lora_shrink_wide_kernel(const LoraArgs a) {
 
 // ---- second launch: y += B v ---------------------------------------------------------------------
 // Block: up to 16 * MT rows of one adapter x a range of features, 32 features a warp at a time, D[row, feature].
-// v enters the 16-bit tensor cores as a sum of 16-bit numbers, so that y's fp32 sums keep (nearly) fp32 accuracy: three
-// bf16 numbers hold all 24 bits; two fp16 numbers hold 22, with each row of v scaled by a power of two to a largest
-// value in [2^14, 2^15) so that neither overflows or loses bits below fp16's normal range.  (tf32 would do it in two
-// for both types, but mma.sync runs tf32 at the rate of plain fp32 multiply-adds here: 192 us instead of 121 for 8192
+// v enters the 16-bit tensor cores as a sum of three 16-bit numbers, so that y's fp32 sums keep fp32 accuracy: three bf16
+// numbers hold all 24 bits.  For fp16 each row of v is scaled by a power of two to a largest finite value in
+// [2^14, 2^15), and every part holds 2^11 times the rest that the part before left, or its bits would fall below fp16's
+// range: v = p0 + 2^-11 p1 + 2^-22 p2 holds all 24 bits of what is above 2^-37 of the row's largest, and is off by at most
+// 2^-61 of the largest below that.  The sums over the parts are scaled alike, the last part's first.  (tf32 would do it in
+// two for both types, but mma.sync runs tf32 at the rate of plain fp32 multiply-adds here: 192 us instead of 121 for 8192
 // rows of 6144 at rank 64.)  n-tile j of a warp's chunk holds features 8 (c / 2) + 2 j + c % 2 in its columns c: lane t
 // of a quad then owns eight contiguous features of a row.
 template <typename T> __device__ __forceinline__ float2 pair_f(uint32_t v);
 template <> __device__ __forceinline__ float2 pair_f<__nv_bfloat16>(uint32_t v) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&v)); }
 template <> __device__ __forceinline__ float2 pair_f<__half>(uint32_t v) { return __half22float2(*reinterpret_cast<__half2*>(&v)); }
 
-template <typename T> struct Split;      // v as the sum of N numbers of type T
-template <> struct Split<__nv_bfloat16> { static constexpr int N = 3; static constexpr bool scaled = false; };
-template <> struct Split<__half> { static constexpr int N = 2; static constexpr bool scaled = true; };
+template <typename T> struct Split;      // v as the sum of N numbers of type T, each after the first times 2^lg
+template <> struct Split<__nv_bfloat16> { static constexpr int N = 3, lg = 0; static constexpr bool scaled = false; };
+template <> struct Split<__half> { static constexpr int N = 3, lg = 11; static constexpr bool scaled = true; };
 
-// The power of two that lifts `top` into [2^14, 2^15), kept where it and its inverse are normal; 0 for zero and infinity.
+// One part of v, and in v what the next is taken from.  Infinity and NaN have no rest; a finite value that rounds to
+// infinity is cut instead.
+template <typename T>
+__device__ __forceinline__ T next_part(float& v) {
+    T p = from_f<T>(v);
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        if (isinf(to_f(p)) && isfinite(v)) p = __float2bfloat16_rz(v);
+    }
+    v = isfinite(v) ? (v - to_f(p)) * (float)(1 << Split<T>::lg) : 0.f;
+    return p;
+}
+
+// The power of two that lifts `top` into [2^14, 2^15), kept where it and its inverse are normal; 0 for zero.
 __device__ __forceinline__ int row_exponent(float top) {
     const int ex = 14 - ((int)((__float_as_uint(top) >> 23) & 0xff) - 127);
-    return top > 0.f && top < __int_as_float(0x7f800000) ? min(max(ex, -126), 126) : 0;
+    return top > 0.f ? min(max(ex, -126), 126) : 0;
 }
+// what a value counts for the row's largest: infinity and NaN nothing, or the finite ones beside them would leave the range
+__device__ __forceinline__ float magnitude(float v) { return isfinite(v) ? fabsf(v) : 0.f; }
 
 template <typename T> __device__ __forceinline__ uint32_t pack2(T a, T b) {
     const unsigned short x = *reinterpret_cast<const unsigned short*>(&a), y = *reinterpret_cast<const unsigned short*>(&b);
@@ -350,9 +366,9 @@ __device__ __forceinline__ void stage_v(int cnt, int rank, F of, uint4* s_v, flo
         float top = 0.f;
         if (KG) {
 #pragma unroll
-            for (int i = 0; i < 2 * KG; ++i) top = fmaxf(top, fabsf(v[i]));
+            for (int i = 0; i < 2 * KG; ++i) top = fmaxf(top, magnitude(v[i]));
         } else {
-            for (int r = l8 * 2; r < kgs * 16; r += 16) top = fmaxf(top, fmaxf(fabsf(value(r)), fabsf(value(r + 1))));
+            for (int r = l8 * 2; r < kgs * 16; r += 16) top = fmaxf(top, fmaxf(magnitude(value(r)), magnitude(value(r + 1))));
         }
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
@@ -371,11 +387,8 @@ __device__ __forceinline__ void stage_v(int cnt, int rank, F of, uint4* s_v, flo
                       hi_pair * 2 + ((cr >> 3) & 1);
 #pragma unroll
         for (int u = 0; u < NS; ++u) {
-            const T p0 = from_f<T>(v0), p1 = from_f<T>(v1);
+            const T p0 = next_part<T>(v0), p1 = next_part<T>(v1);
             d[u * 128] = pack2(p0, p1);
-            // the rest; infinity and NaN have none
-            v0 = isfinite(v0) ? v0 - to_f(p0) : 0.f;
-            v1 = isfinite(v1) ? v1 - to_f(p1) : 0.f;
         }
     }
 }
@@ -431,22 +444,63 @@ struct Expand {
         for (int m = 0; m < 2 * MT; ++m)
             if (row[m] >= 0 && f < a.N) q.y[m] = load8(reinterpret_cast<const Y*>(a.y) + (int64_t)row[m] * a.N + f, min(8, a.N - f), vec_y);
     }
+    __device__ __forceinline__ static void lower(float (&d)[4]) {
+#pragma unroll
+        for (int h = 0; h < 4; ++h) d[h] *= 1.f / (1 << Split<T>::lg);
+    }
     __device__ __forceinline__ void finish(const Ahead& q, int f0) const {
         const int lane = threadIdx.x & 31, g = lane >> 2;
         float acc[MT][4][4] = {};
-        for (int kg = 0; kg < (KG ? KG : kgs); ++kg) {
-            if (kg >= kgs) break;
-            uint2 b[4];
+        // small parts first; where the parts are scaled, so are the sums between two parts: all of them where B is in
+        // registers, else those of 16 ranks
+        if constexpr (Split<T>::scaled && KG > 0) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) b[j] = KG ? q.b[kg][j] : load_b(f0, kg, j);
+            for (int u = NS - 1; u >= 0; --u) {
+                if (u < NS - 1) {
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+                    for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int u = NS - 1; u >= 0; --u) {    // small parts first
-                    const uint4 v = s_v[((m * kgs + kg) * NS + u) * 32 + lane];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) mma_k16<T>(acc[m][j], v.x, v.y, v.z, v.w, b[j].x, b[j].y);
+                        for (int j = 0; j < 4; ++j) lower(acc[m][j]);
                 }
+#pragma unroll
+                for (int kg = 0; kg < KG; ++kg) {
+                    if (kg >= kgs) break;
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        const uint4 v = s_v[((m * kgs + kg) * NS + u) * 32 + lane];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) mma_k16<T>(acc[m][j], v.x, v.y, v.z, v.w, q.b[kg][j].x, q.b[kg][j].y);
+                    }
+                }
+            }
+        } else {
+            for (int kg = 0; kg < (KG ? KG : kgs); ++kg) {
+                if (kg >= kgs) break;
+                uint2 b[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) b[j] = KG ? q.b[kg][j] : load_b(f0, kg, j);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    float rest[4][4] = {};
+#pragma unroll
+                    for (int u = NS - 1; u >= 0; --u) {
+                        const uint4 v = s_v[((m * kgs + kg) * NS + u) * 32 + lane];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (Split<T>::scaled && u) {
+                                mma_k16<T>(rest[j], v.x, v.y, v.z, v.w, b[j].x, b[j].y);
+                                lower(rest[j]);
+                            } else {
+                                if (Split<T>::scaled) {
+#pragma unroll
+                                    for (int h = 0; h < 4; ++h) acc[m][j][h] += rest[j][h];
+                                }
+                                mma_k16<T>(acc[m][j], v.x, v.y, v.z, v.w, b[j].x, b[j].y);
+                            }
+                        }
+                    }
+                }
+            }
         }
         const int f = f0 + 8 * (lane & 3), have = min(8, a.N - f);
 #pragma unroll
@@ -484,7 +538,9 @@ lora_expand_kernel(const LoraArgs a, int feats, int flags) {
     typename Expand<T, Y, MT, KG>::Ahead q;
     ex.load(q, f0);                                      // B and y do not wait for the first launch
     pdl_wait();                                          // v comes from it
-    stage_v<T, MT, KG>(tile.cnt, rank, [&](int c, int r) { return sc * sum_parts(a, tile.p0 + c, r); }, s_v, s_scale);
+    // 32-row tiles take ranks up to 64, which registers hold where v would be read twice (8192 rows of 6144 to 6144 at rank
+    // 64, fp16 and a 16-bit y: 135 us against 163)
+    stage_v<T, MT, MT == 2 && !KG && Split<T>::scaled ? 4 : KG>(tile.cnt, rank, [&](int c, int r) { return sc * sum_parts(a, tile.p0 + c, r); }, s_v, s_scale);
     __syncthreads();
     for (; f0 < ex.f_end; f0 += 256) {
         ex.finish(q, f0);
@@ -584,7 +640,7 @@ __device__ __forceinline__ void stage_v_rows(const LoraArgs& a, const LoraTile& 
     for (int j = 0; j < 8; ++j) {
         const int r = p8 * 8 + j;
         v[j] = in && r < rank ? sc * sum_parts(a, tile.p0 + c, r) : 0.f;
-        top = fmaxf(top, fabsf(v[j]));
+        top = fmaxf(top, magnitude(v[j]));
     }
     if (Split<T>::scaled) {
 #pragma unroll
@@ -600,10 +656,8 @@ __device__ __forceinline__ void stage_v_rows(const LoraArgs& a, const LoraTile& 
         uint32_t w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const T h0 = from_f<T>(v[2 * j]), h1 = from_f<T>(v[2 * j + 1]);
+            const T h0 = next_part<T>(v[2 * j]), h1 = next_part<T>(v[2 * j + 1]);
             w[j] = pack2(h0, h1);
-            v[2 * j] = isfinite(v[2 * j]) ? v[2 * j] - to_f(h0) : 0.f;       // the rest; infinity and NaN have none
-            v[2 * j + 1] = isfinite(v[2 * j + 1]) ? v[2 * j + 1] - to_f(h1) : 0.f;
         }
         *reinterpret_cast<uint4*>(s_vp + u * kTcNT * 128 + c * 128 + ((p8 ^ (c & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
     }
@@ -785,9 +839,11 @@ lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b
                 const uint32_t idesc = tc5::idesc_f16(ab, 128, (uint32_t)((tile.cnt + 15) & ~15));
                 const uint64_t bd = b0 + (uint64_t)(st * (uint32_t)(kTcABytes >> 4));
                 uint32_t acc = 0;
-                for (int p = NS - 1; p >= 0; --p)          // small parts first
+                for (int p = NS - 1; p >= 0; --p)          // small parts first; their sum is scaled by the next part's first product
                     for (int k = 0; k < kgs; ++k) {
-                        tc5::mma_f16_ss(tmem + slot * kTcNT, bd + (uint64_t)(k * 2), v0 + (uint64_t)(p * (kTcVBytes >> 4) + k * 2), idesc, acc);
+                        const uint64_t vd = v0 + (uint64_t)(p * (kTcVBytes >> 4) + k * 2);
+                        if (Split<T>::lg && !k && acc) tc5::mma_f16_ss_lower<Split<T>::lg>(tmem + slot * kTcNT, bd, vd, idesc);
+                        else tc5::mma_f16_ss(tmem + slot * kTcNT, bd + (uint64_t)(k * 2), vd, idesc, acc);
                         acc = 1u;
                     }
                 tc5::commit(&b_empty[st]);

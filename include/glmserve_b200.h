@@ -157,8 +157,8 @@ GSB_API int gsb_moe_expert_ffn_w16(const void* x, const int* topk_ids, const flo
  * of gsb_moe_dispatch on one adapter id a row (topk = 1, E = n_adapters, an id outside the range = no adapter), made
  * once per batch and used for every projection of the model; rows that no list names are left as they were, indices
  * outside [0,n) are skipped, a row must not be listed twice; y must not overlap the inputs.  A x is kept in fp32 and B
- * applied to it without rounding it to `type` (it enters the products in parts, so an infinity in B may give NaN); y is
- * rounded once.  in % 8 == 0, 1 <= max_rank <= 256, n_adapters <= 1024, P, in and out <= 2^30; x and A 16-byte aligned;
+ * applied to it without rounding it to `type` (it enters the products in parts, so an infinity in B may give NaN; with
+ * F16, entries of A x below 2^-37 of their row's largest are off by up to 2^-61 of the largest); y is rounded once.  in % 8 == 0, 1 <= max_rank <= 256, n_adapters <= 1024, P, in and out <= 2^30; x and A 16-byte aligned;
  * scratch of gsb_lora_scratch_bytes() bytes (0 for few rows: then it may be NULL), 256-byte aligned, any contents, not
  * shared by calls that may overlap. */
 GSB_API size_t gsb_lora_scratch_bytes(int P, int max_rank, int n_adapters);

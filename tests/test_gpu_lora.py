@@ -228,3 +228,58 @@ def test_lora_bad_offsets_stay_inside(dev, case):
     assert torch.equal(y, y0)
     ops.lora_add(y, x, A, B, _i32([-5] + [0] * (nA - 1) + [2 ** 31 - 1], dev), rows)    # clamped to [0, P]
     assert torch.equal(y, ops.lora_add(y0.clone(), x, A, B, _i32([0] * nA + [n], dev), rows))
+
+
+@pytest.mark.parametrize("case", SHAPES + [8, 19])      # and ranks whose B is loaded in turn, tcgen05 at rank 40
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_lora_small_ranks_beside_large_ones(dev, case, dtype):
+    """Odd ranks of A are 2^-36 of the even ones, and half of the features of B read the odd ranks alone: what is small
+    in a row of A x keeps its bits beside the row's largest."""
+    from glmserve_b200 import ops
+    y0, x, A, B, ids, ranks, scales = _case(case, dtype, torch.float32, dev)
+    y0 = y0 * 0
+    big, small = (_randn(A.shape, torch.float32, dev, s) for s in (500 + case, 600 + case))
+    new = (big * 2.0 ** 15).clamp(-60000, 60000)
+    new[:, 1::2] = ((small[:, 1::2] * 8).round() * 2.0 ** -24)
+    A = torch.where(A.isnan(), A, new.to(dtype))
+    new = _randn(B.shape, torch.float32, dev, 700 + case) * 2.0 ** 12
+    new[:, :, 0::2] *= 2.0 ** -26
+    new[:, 1::2, 0::2] = 0
+    B = torch.where(B.isnan(), B, new.to(dtype))
+    offs, rows, _ = ops.moe_dispatch(ids[:, None].contiguous(), A.shape[0])
+    y = ops.lora_add(y0.clone(), x, A, B, offs, rows, ranks=ranks, scales=scales)
+    ref, b = _ref(y0, x, A, B, offs, rows, ranks, scales)
+    _check(y, ref, b + HALF[torch.float32] * (ref.abs() + b), "small ranks")
+
+
+@pytest.mark.parametrize("case", SHAPES + [8, 19])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_lora_infinite_entry_beside_large_ones(dev, case, dtype):
+    """One rank of A x is infinite, the others are finite beyond 65504: y is infinity of the sign of that rank's B."""
+    from glmserve_b200 import ops
+    y0, x, A, B, ids, _, _ = _case(case, dtype, torch.float32, dev)
+    x, A, B = x.abs() + 1, A.nan_to_num().abs() * 20 + 1000, B.nan_to_num()
+    if A.shape[1] < 2:
+        pytest.skip("one rank")
+    B = torch.where(B.abs() < 0.01, torch.full_like(B, 0.01), B)
+    A[:, 0, 0] = float("inf")
+    offs, rows, _ = ops.moe_dispatch(ids[:, None].contiguous(), A.shape[0])
+    y = ops.lora_add(y0.clone(), x, A, B, offs, rows)
+    on = ids >= 0
+    want = torch.copysign(torch.full_like(y0, float("inf")), B[ids.clamp(min=0).long(), :, 0].float())
+    assert torch.equal(y[on], want[on]) and torch.equal(y[~on], y0[~on])
+
+
+@pytest.mark.parametrize("case", [0, 3, 14, 15, 17, 21])
+def test_lora_products_next_to_the_largest_fp32(dev, case):
+    """A x between the largest bf16 number and the largest fp32 number is finite, and so is B A x."""
+    from glmserve_b200 import ops
+    y0, x, A, B, ids, _, _ = _case(case, torch.bfloat16, torch.float32, dev)
+    y0, x, A, B = (torch.zeros_like(t) for t in (y0, x, A, B))
+    x[:, 0], x[:, 1] = (2 - 2.0 ** -7) * 2.0 ** 127, 1.25 * 2.0 ** 119
+    A[:, 0, :2] = 1
+    B[:, :, 0] = 2.0 ** -10
+    offs, rows, _ = ops.moe_dispatch(ids[:, None].contiguous(), A.shape[0])
+    y = ops.lora_add(y0.clone(), x, A, B, offs, rows)
+    value = ((2 - 2.0 ** -7) * 2.0 ** 127 + 1.25 * 2.0 ** 119) * 2.0 ** -10      # exact in fp32
+    assert torch.equal(y, torch.where(ids[:, None] >= 0, torch.full_like(y0, value), y0))
