@@ -403,7 +403,7 @@ template <typename O, int U>
 __global__ void __launch_bounds__(256)
 combine16_kernel(const float* __restrict__ y, const int* __restrict__ ids, const int* __restrict__ slot_pos,
                  const float* __restrict__ w, int topk, int H, int E, O* __restrict__ out) {
-    const int64_t t = blockIdx.x;
+    const int64_t t = U == 1 ? blockIdx.y : blockIdx.x;
     __shared__ int s_pos[256];
     __shared__ float s_w[256];
     pdl_trigger();
@@ -412,7 +412,7 @@ combine16_kernel(const float* __restrict__ y, const int* __restrict__ ids, const
     float4 acc[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-    const int c0 = blockIdx.y * 1024 * U + threadIdx.x * 4;             // H is a multiple of 8
+    const int c0 = (int)(U == 1 ? blockIdx.x : blockIdx.y) * 1024 * U + threadIdx.x * 4;     // H is a multiple of 8
     for (int k0 = 0; k0 < topk; k0 += 256) {
         __syncthreads();
         if (k0 + (int)threadIdx.x < topk) {
@@ -455,11 +455,15 @@ combine16_kernel(const float* __restrict__ y, const int* __restrict__ ids, const
     }
 }
 
+constexpr int kManyTokens = 256;
+
 template <typename O>
 int run_combine16(const float* y, const int* ids, const int* slot_pos, const float* w, int n, int topk, int H, int E,
                   void* out, cudaStream_t s) {
     O* o = reinterpret_cast<O*>(out);
-    if (n < 256) return launch_after(combine16_kernel<O, 1>, dim3(n, (H + 1023) / 1024), 256, 0, 1, s, y, ids, slot_pos, w, topk, H, E, o);
+    // a grid's second dimension ends at 65535: few tokens may have more feature blocks than that (256 tokens and more would
+    // need per-slot rows of 275 GB for it, and are refused)
+    if (n < kManyTokens) return launch_after(combine16_kernel<O, 1>, dim3((H + 1023) / 1024, n), 256, 0, 1, s, y, ids, slot_pos, w, topk, H, E, o);
     return launch_after(combine16_kernel<O, 4>, dim3(n, (H + 4095) / 4096), 256, 0, 1, s, y, ids, slot_pos, w, topk, H, E, o);
 }
 
@@ -536,6 +540,7 @@ extern "C" int gsb_moe_expert_ffn_w16(const void* x, const int* topk_ids, const 
         return GSB_ERR_INVALID_ARG;
     if (hidden % 8 || moe_inter % 8 || E > 1024 || (int64_t)n * topk > kMaxSlots || hidden > kMaxDim || moe_inter > kMaxDim)
         return GSB_ERR_UNSUPPORTED;
+    if (n >= kManyTokens && (hidden + 4095) / 4096 > 65535) return GSB_ERR_TOO_LARGE;
     if (!workspace || misaligned(workspace, 256)) return GSB_ERR_INVALID_ARG;
     const Ffn16Ws ws = carve16(n, topk, hidden, moe_inter, E, workspace);
     if (workspace_bytes < ws.total) return GSB_ERR_WORKSPACE;

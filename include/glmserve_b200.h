@@ -139,10 +139,11 @@ GSB_API int gsb_grouped_gemm(const void* x, const void* w, int type, const int* 
  * out[t] = sum_k w[t,k] * down(silu(gate x) * up x), slots added in order.  x [n,hidden], gate_w/up_w
  * [E,moe_inter,hidden], down_w [E,hidden,moe_inter] of `type`; out [n,hidden] of out_type (`type`, or F32) is
  * OVERWRITTEN.  A slot whose id is outside [0,E) adds nothing (padding, or an expert that lives on another GPU);
- * a token without a slot gets zeros.  Sums in fp32; silu(gate x) * up x is rounded once to `type`; in fp16
- * finite values saturate at +-65504, infinities and NaN stay what they are.  hidden and moe_inter multiples of 8, E <= 1024, n * topk and each dimension <= 2^30; all pointers but ids
- * and weights 16-byte aligned; workspace 256-byte aligned, any contents; two calls that may overlap on the GPU
- * need a workspace each. */
+ * a token without a slot gets zeros.  Sums in fp32; silu(gate x) * up x is rounded once to `type`; in fp16 finite
+ * values saturate at +-65504, infinities and NaN stay what they are.  hidden and moe_inter multiples of 8, E <= 1024,
+ * n * topk and each dimension <= 2^30 (hidden <= 65535 * 4096 for 256 tokens or more); all pointers but ids and
+ * weights 16-byte aligned; workspace 256-byte aligned, any contents; two calls that may overlap on the GPU need a
+ * workspace each. */
 GSB_API size_t gsb_moe_expert_ffn_w16_workspace_bytes(int n, int topk, int hidden, int moe_inter, int E);
 GSB_API int gsb_moe_expert_ffn_w16(const void* x, const int* topk_ids, const float* topk_weights,
                                    const void* gate_w, const void* up_w, const void* down_w, int type,

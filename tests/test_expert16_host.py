@@ -85,3 +85,9 @@ def test_python_refuses_wrong_tensors():
                  lambda: ops.lora_add(x, x, x, x, i, i)):
         with pytest.raises(ValueError, match="expected"):
             call()
+
+
+def test_ffn_refuses_what_its_last_launch_could_not_cover():
+    """256 tokens or more of over 65535 * 4096 features: before anything is launched (fewer tokens: no such limit)."""
+    assert _ffn(n=256, H=65535 * 4096 + 8, nb=1 << 62) == 7
+    assert _ffn(n=255, H=65535 * 4096 + 8) == WORKSPACE and _ffn(n=256, H=65535 * 4096) == WORKSPACE

@@ -419,3 +419,30 @@ def test_expert_ffn_infinity_goes_through(dev, shape, dtype):
     want = torch.zeros_like(out, dtype=torch.bool)
     want[n // 2] = True
     assert torch.equal(out == float("inf"), want) and not bool(out.isnan().any())
+
+
+def test_expert_ffn_of_more_features_than_a_grid_has_blocks_for(dev):
+    """65535 blocks of 1024 features and a ragged rest, one token; x has few values, so that 64-bit sums are quick."""
+    from glmserve_b200 import ops
+    H, I, dtype = 65535 * 1024 + 2056, 8, torch.bfloat16
+    g = torch.Generator(device=dev)
+    g.manual_seed(1)
+    x = torch.zeros((1, H), dtype=dtype, device=dev)
+    at = torch.cat([torch.randint(H, (62,), generator=g, device=dev), torch.tensor([0, H - 1], device=dev)])
+    x[0, at] = torch.randn(64, generator=g, device=dev).to(dtype)
+    gate, up, down = (torch.empty(s, dtype=dtype, device=dev).normal_(0, 0.05, generator=g) for s in ((1, I, H), (1, I, H), (1, H, I)))
+    ids, wt = torch.zeros((1, 1), dtype=torch.int32, device=dev), torch.full((1, 1), 0.75, device=dev)
+    out = ops.moe_expert_ffn_w16(x, ids, wt, gate, up, down, out=torch.full((1, H), float("nan"), device=dev))
+    assert ops.operators16_status() == 0
+    at = at.unique()
+    xs = x[0, at].double()
+    gs, us = gate[0][:, at].double(), up[0][:, at].double()
+    g64, u64 = gs @ xs, us @ xs
+    h = torch.nn.functional.silu(g64) * u64
+    # sums of 64 products: the zeros beside them add nothing
+    dg, du = gs.abs() @ xs.abs() * (72 * U), us.abs() @ xs.abs() * (72 * U)
+    dh = (1.1 * dg * (u64.abs() + du) + torch.nn.functional.silu(g64).abs() * du) * (1 + U) + (HALF[dtype] + 2.0 ** -20) * h.abs()
+    for a in range(0, H, 1 << 24):
+        d = down[0, a:a + (1 << 24)].double()
+        ref, mag = 0.75 * (d @ h), d.abs() @ h.abs()
+        _check(out[0, a:a + (1 << 24)], ref, 0.75 * (d.abs() @ dh) + mag * (20 * U), f"features from {a}")
