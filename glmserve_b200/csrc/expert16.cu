@@ -281,7 +281,7 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
         for (int i = first; i < items; i += step, ++tl) {
             const GrItem it = gr_item(offsets, a.P, pre, i, FB, fw, e);
             const uint32_t buf = tl & 1u;
-            int ok = tc5::warp_set(abort_flag) ? 0 : (int)tc5::warp_wait(&acc_full[buf], (tl >> 1) & 1u, kGrWaitLimit);
+            int ok = tc5::warp_set(abort_flag) ? 0 : (int)tc5::warp_wait(&acc_full[buf], (tl >> 1) & 1u, a.sum_limit);
             if (!ok) gr_timeout(abort_flag);
             // all four warps must agree to go on: they meet at a barrier below
             if (GU) ok = epilogue_agree(ok, 1);
@@ -381,7 +381,8 @@ int run_grouped_any(const GroupedArgs& a, int y_type, cudaStream_t s) {
 
 bool use_pair(int P, int E) { return P / E > 16; }
 
-int launch_grouped(const GroupedArgs& a, int type, int y_type, void* scratch, cudaStream_t s) {
+int launch_grouped(GroupedArgs a, int type, int y_type, void* scratch, cudaStream_t s) {
+    a.sum_limit = gr_sum_limit(a.K);
     if (use_pair(a.P, a.E)) return launch_grouped_pair(a, type, y_type, scratch, s);
     return type == GSB_TYPE_BF16 ? run_grouped_any<__nv_bfloat16>(a, y_type, s) : run_grouped_any<__half>(a, y_type, s);
 }

@@ -23,9 +23,13 @@ struct GroupedArgs {
     int topk;
     int* offsets_out;
     int* slot_pos_out;
+    long long sum_limit;    // clocks to wait for a whole sum over K
 };
 
 constexpr long long kGrWaitLimit = 2000000000LL;    // about a second of SM clocks
+// The wait for a whole sum over K lasts as long as the sum: a second more for every 250,000 k-blocks of 64 columns.  (A
+// block alone on the GPU takes 270 clocks for one; 38 experts of one row, 2^29 to 1, are 2.2 G clocks.)
+inline long long gr_sum_limit(int K) { return kGrWaitLimit + ((long long)K + 63) / 64 * 8192; }
 
 constexpr int kFewSlots = 256;
 

@@ -205,7 +205,7 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
         for (int i = first; i < items; i += step, ++tl) {
             const GrItem it = pr_item(a, pre, i, FB, fw, e);
             const uint32_t buf = tl & 1u;
-            int ok = tc5::warp_set(abort_flag) ? 0 : (int)tc5::warp_wait(&acc_full[buf], (tl >> 1) & 1u, kGrWaitLimit);
+            int ok = tc5::warp_set(abort_flag) ? 0 : (int)tc5::warp_wait(&acc_full[buf], (tl >> 1) & 1u, a.sum_limit);
             if (!ok) pr_timeout(abort_flag);
             // the group's four warps must agree to go on: they meet at a barrier in the loop below
             if (GU) ok = epilogue_agree(ok, bar);

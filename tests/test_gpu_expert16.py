@@ -446,3 +446,27 @@ def test_expert_ffn_of_more_features_than_a_grid_has_blocks_for(dev):
         d = down[0, a:a + (1 << 24)].double()
         ref, mag = 0.75 * (d @ h), d.abs() @ h.abs()
         _check(out[0, a:a + (1 << 24)], ref, 0.75 * (d.abs() @ dh) + mag * (20 * U), f"features from {a}")
+
+
+def _sparse(n, K, at, dev, seed):
+    """[n, K] of zeros but for the columns `at`, made without a dense copy in another type."""
+    x = torch.zeros((n, K), dtype=torch.bfloat16, device=dev)
+    x[:, at] = _randn((n, at.numel()), torch.bfloat16, dev, seed)
+    return x
+
+
+@pytest.mark.parametrize("E,P,K", [(38, 38, 1 << 29), (1, 17, 1 << 30)])     # few rows per expert, and many
+def test_grouped_gemm_sum_that_takes_a_second(dev, E, P, K):
+    """One block (pair) after the other takes over 2^23 steps along K: its waits must last as long as the sum does."""
+    from glmserve_b200 import ops
+    at = torch.tensor([0, 5, 70, K // 3, K // 2, K - 65, K - 2, K - 1], device=dev)
+    x, w = _sparse(P if E == 1 else 1, K, at, dev, 1), _sparse(E, K, at, dev, 2)
+    rows = None if E == 1 else torch.zeros(P, dtype=torch.int32, device=dev)
+    y = ops.grouped_gemm(x, w[:, None], _i32(np.arange(E + 1) * (P // E), dev), rows=rows, out=torch.full((P, 1), float("nan"), device=dev))
+    assert ops.operators16_status() == 0
+    xs, ws = x[:, at].double(), w[:, at].double()
+    # sums of eight products: the zeros beside them add nothing
+    ref, mag = (xs @ ws.T, xs.abs() @ ws.abs().T) if E == 1 else (ws @ xs.T, ws.abs() @ xs.abs().T)
+    _check(y, ref, mag * (16 * U), "long sum")
+    del x, w, y
+    torch.cuda.empty_cache()
