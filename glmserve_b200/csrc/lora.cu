@@ -724,10 +724,12 @@ lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b
         const bool leader = tc5::elect_one();
         uint32_t st = 0, ph = 0;
         const uint32_t ring = tma ? kTcStages : kTcLin;
+        const int ahead = tma ? kTcStages : kTcStages + kTcLin;      // tiles that need no MMA before them
         uint64_t *fullb = tma ? b_full : lin_full, *emptyb = tma ? b_empty : lin_empty;
         LoraTile tile{-1, 0, 0};
         for (int u = u_beg; u < u_end && !tc5::warp_set(abort_flag); ++u) {
             if (u == u_beg || u % FB == 0) tile = lora_tile<kTcNT>(a, pre, u / FB, 0);
+            if (u - u_beg == ahead) pdl_wait();    // bounded waits count from where the first launch has ended, which may take its time
             if (!tc5::warp_wait(&emptyb[st], ph ^ 1u, kTcWaitLimit)) { lora_timeout(abort_flag); break; }
             if (leader) {
                 const int f0 = u % FB * 128;
@@ -742,6 +744,7 @@ lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b
             }
             if (++st == ring) { st = 0; ph ^= 1u; }
         }
+        pdl_wait();
         for (uint32_t j = 0; j < ring && !tc5::warp_set(abort_flag); ++j) {           // the last tiles are done with, their signals in
             tc5::warp_wait(&emptyb[st], ph ^ 1u, kTcWaitLimit);
             if (++st == ring) { st = 0; ph ^= 1u; }
@@ -760,6 +763,7 @@ lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b
         for (int u = u_beg; u < u_end && !tc5::warp_set(abort_flag); ++u) {
             if (u == u_beg || u % FB == 0) { tile = lora_tile<kTcNT>(a, pre, u / FB, 0); rank = rank_of(a, tile.ad); }
             uint8_t* at = smem + st * kTcABytes;
+            if (u - u_beg == kTcStages) pdl_wait();
             if (tma) {
                 if (!tc5::warp_wait(&b_full[st], ph, kTcWaitLimit)) { lora_timeout(abort_flag); break; }
                 if (rank & 15) {
@@ -810,6 +814,7 @@ lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b
             if (lane == 0) mbar_arrive(&b_ready[st]);
             if (++st == kTcStages) { st = 0; ph ^= 1u; }
         }
+        pdl_wait();
         if (!tma)
             for (int j = 0; j < kTcStages && !tc5::warp_set(abort_flag); ++j) {       // the last MMAs' signals have arrived
                 tc5::warp_wait(&b_empty[st], ph ^ 1u, kTcWaitLimit);
@@ -826,6 +831,7 @@ lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b
             if (u == u_beg || u % FB == 0) {
                 tile = lora_tile<kTcNT>(a, pre, u / FB, 0);
                 kgs = (rank_of(a, tile.ad) + 15) / 16;
+                if (u == u_beg) pdl_wait();
                 if (!tc5::warp_wait(v_full, vph, kTcWaitLimit)) { lora_timeout(abort_flag); break; }
                 vph ^= 1u;
             }

@@ -4,7 +4,7 @@ that keep at least 21 bits (2^-21 of every product); y is rounded once."""
 import numpy as np
 import pytest
 
-from test_gpu_expert16 import HALF, TINY, U, _check, _i32, _randn
+from test_gpu_expert16 import HALF, TINY, U, _check, _i32, _randn, _sparse
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -283,3 +283,21 @@ def test_lora_products_next_to_the_largest_fp32(dev, case):
     y = ops.lora_add(y0.clone(), x, A, B, offs, rows)
     value = ((2 - 2.0 ** -7) * 2.0 ** 127 + 1.25 * 2.0 ** 119) * 2.0 ** -10      # exact in fp32
     assert torch.equal(y, torch.where(ids[:, None] >= 0, torch.full_like(y0, value), y0))
+
+
+@pytest.mark.parametrize("R", [8, 7])            # B by TMA, and laid out by hand
+def test_lora_long_sum(dev, R):
+    """The second launch starts early and waits for the first, whose eight blocks take 2^21 steps along K each."""
+    from glmserve_b200 import ops
+    n, K, N = 17, 1 << 30, 160001
+    at = torch.tensor([0, 5, 70, K // 3, K // 2, K - 65, K - 2, K - 1], device=dev)
+    x, A, B = _sparse(n, K, at, dev, 1), _sparse(R, K, at, dev, 2), _randn((1, N, R), torch.bfloat16, dev, 3)
+    y = ops.lora_add(torch.zeros((n, N), device=dev), x, A[None], B, _i32([0, n], dev), torch.arange(n, dtype=torch.int32, device=dev))
+    assert ops.operators16_status() == 0
+    xs, As, Bs = x[:, at].double(), A[:, at].double(), B[0].double()
+    v, va = xs @ As.T, xs.abs() @ As.abs().T
+    # sums of eight products and of R: the zeros beside them add nothing
+    ref, mag = v @ Bs.T, va @ Bs.abs().T
+    _check(y, ref, mag * (18 * U) + v.abs() @ Bs.abs().T * ((R + 8) * U + 2.0 ** -21) + HALF[torch.float32] * ref.abs(), "long sum")
+    del x, A, y
+    torch.cuda.empty_cache()
