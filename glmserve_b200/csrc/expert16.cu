@@ -273,6 +273,14 @@ grouped_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_w, co
             }
             if (!dead && leader) tc5::commit(&acc_full[buf]);
         }
+        // after a time-out: no MMA is at work, and no signal on its way, when the block ends (otherwise the others have
+        // waited for all of them)
+        if (tc5::warp_set(abort_flag)) {
+            if (st == 0) { st = (uint32_t)stages; ph ^= 1u; }
+            tc5::warp_wait(&empty[st - 1], ph, kGrWaitLimit);      // (at once where there was none)
+            if (dead) --tl;                                        // (counted, but not announced)
+            if (tl) tc5::warp_wait(&acc_full[(tl - 1) & 1u], ((tl - 1) >> 1) & 1u, kGrWaitLimit);
+        }
     } else if (warp >= 4) {                // ---- epilogue: this thread's TMEM lane = weight row
         const int q = warp & 3, row = q * 32 + lane;
         uint32_t tl = 0;

@@ -194,6 +194,14 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
                 }
                 if (!dead && leader) tc5::commit2(&acc_full[buf]);
             }
+            // after a time-out: no MMA is at work, and no signal on its way, when the blocks end (otherwise the others have
+            // waited for all of them)
+            if (tc5::warp_set(abort_flag)) {
+                if (st == 0) { st = kPrStages; ph ^= 1u; }
+                tc5::warp_wait(&empty[st - 1], ph, kGrWaitLimit);      // (at once where there was none)
+                if (dead) --tl;                                        // (counted, but not announced)
+                if (tl) tc5::warp_wait(&acc_full[(tl - 1) & 1u], ((tl - 1) >> 1) & 1u, kGrWaitLimit);
+            }
         }
     } else if (warp >= 4) {                // ---- epilogue: this thread's TMEM lane = weight row of this CTA
         // two groups of four warps take 16 token columns in turn

@@ -857,6 +857,13 @@ lora_expand_tc_kernel(const LoraArgs a, const __grid_constant__ CUtensorMap tm_b
             }
             if (++st == kTcStages) { st = 0; ph ^= 1u; }
         }
+        // after a time-out: no MMA is at work, and no signal on its way, when the block ends (otherwise the others have
+        // waited for all of them)
+        if (tc5::warp_set(abort_flag) && n) {
+            if (st == 0) { st = kTcStages; ph ^= 1u; }
+            tc5::warp_wait(&b_empty[st - 1], ph, kTcWaitLimit);
+            tc5::warp_wait(&acc_full[(n - 1) % kTcGroups], ((n - 1) / kTcGroups) & 1u, kTcWaitLimit);
+        }
     } else if (warp >= 4) {                // ---- v of a tile, then y of this group's units
         const int e = tid - 128, group = (warp - 4) >> 2, q = warp & 3;
         for (int us = u_beg; us < u_end;) {                // units of one tile
