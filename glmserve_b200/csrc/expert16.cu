@@ -69,7 +69,7 @@ __device__ __forceinline__ void gr_timeout(volatile int* abort_flag) {
 // [kFewSlots] in shared memory; block 0 leaves the offsets and the slots' places in memory.  All threads call, and meet.
 __device__ __forceinline__ void few_lists(const GroupedArgs& a, int* off, int* tok, int* id) {
     for (int i = threadIdx.x; i < kFewSlots; i += blockDim.x) {
-        const int v = i < a.P ? __ldg(a.ids + i) : -1;
+        const int v = i < a.P ? a.ids[i] : -1;
         id[i] = v >= 0 && v < a.E ? v : a.E;               // what is nobody's sorts behind the last expert
         tok[i] = 0;
     }
@@ -410,8 +410,7 @@ dispatch_few_kernel(const GroupedArgs a, int* tok) {
 // eight slots, which spreads a few tokens over more blocks.
 template <typename O, int U>
 __global__ void __launch_bounds__(256)
-combine16_kernel(const float* __restrict__ y, const int* __restrict__ ids, const int* __restrict__ slot_pos,
-                 const float* __restrict__ w, int topk, int H, int E, O* __restrict__ out) {
+combine16_kernel(const float* y, const int* ids, const int* slot_pos, const float* w, int topk, int H, int E, O* out) {
     const int64_t t = U == 1 ? blockIdx.y : blockIdx.x;
     __shared__ int s_pos[256];
     __shared__ float s_w[256];
@@ -426,10 +425,10 @@ combine16_kernel(const float* __restrict__ y, const int* __restrict__ ids, const
         __syncthreads();
         if (k0 + (int)threadIdx.x < topk) {
             const int64_t i = t * topk + k0 + threadIdx.x;
-            const int id = __ldg(ids + i);
+            const int id = ids[i];
             const bool have = id >= 0 && id < E;
-            s_pos[threadIdx.x] = have ? __ldg(slot_pos + i) : -1;
-            s_w[threadIdx.x] = have ? __ldg(w + i) : 0.f;
+            s_pos[threadIdx.x] = have ? slot_pos[i] : -1;
+            s_w[threadIdx.x] = have ? w[i] : 0.f;
         }
         __syncthreads();
         const int kn = min(256, topk - k0);

@@ -225,7 +225,7 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
                 tc5::tmem_ld16(tmem + ((uint32_t)(q * 32) << 16) + buf * kPrNT + (uint32_t)c0, v);
                 // which of the 16 tokens exist
                 int r = lane < 16 && c0 + lane < it.cnt ? 0 : -1;
-                if (a.rows && r == 0) r = __ldg(a.rows + it.p0 + c0 + lane);
+                if (a.rows && r == 0) r = a.rows[it.p0 + c0 + lane];
                 const uint32_t live = __ballot_sync(0xffffffffu, r >= 0 && r < a.n);
                 tc5::tmem_ld_wait();
                 constexpr int NC = GU ? 8 : 16;        // columns this thread finishes, from column cb on
@@ -287,14 +287,13 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
 // Rows named by the list, in order: a warp takes a row, eight 16-byte loads a lane on their way.  Rows that do not exist
 // are left out (their results are not stored).
 __global__ void __launch_bounds__(256)
-gather_rows_kernel(const uint4* __restrict__ x, const int* __restrict__ rows, const int* __restrict__ offsets, int n, int P, int K8,
-                   int E, uint4* __restrict__ out) {
+gather_rows_kernel(const uint4* x, const int* rows, const int* offsets, int n, int P, int K8, int E, uint4* out) {
     pdl_trigger();
     pdl_wait();
     const int end = seg_bound(offsets, E, P);
     const int64_t p = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
     if (p >= end) return;
-    const int r = __ldg(rows + p);
+    const int r = rows[p];
     if (r < 0 || r >= n) return;
     const uint4* src = x + (int64_t)r * K8;
     uint4* dst = out + p * K8;
@@ -302,7 +301,7 @@ gather_rows_kernel(const uint4* __restrict__ x, const int* __restrict__ rows, co
         uint4 v[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u)
-            if (c + u * 32 < K8) v[u] = __ldg(src + c + u * 32);
+            if (c + u * 32 < K8) v[u] = src[c + u * 32];
 #pragma unroll
         for (int u = 0; u < 8; ++u)
             if (c + u * 32 < K8) dst[c + u * 32] = v[u];

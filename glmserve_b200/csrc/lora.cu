@@ -28,7 +28,7 @@ struct LoraArgs {
 constexpr int kShWarps = 8;
 
 __device__ __forceinline__ int rank_of(const LoraArgs& a, int ad) {
-    return a.ranks ? min(max(__ldg(a.ranks + ad), 0), a.R) : a.R;
+    return a.ranks ? min(max(a.ranks[ad], 0), a.R) : a.R;
 }
 
 constexpr int kMaxRank = 256, kMaxSplit = 8;
@@ -62,13 +62,18 @@ template <> __device__ __forceinline__ void mma_k16<__half>(float (&d)[4], uint3
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // ---- first launch: v ---------------------------------------------------------------------------
+// Early: the kernel may be there while its inputs are written (before the second launch of two stands an ordinary one).
+template <bool Early, typename V> __device__ __forceinline__ V load_in(const V* p) {
+    if constexpr (Early) return *p;
+    else return __ldg(p);
+}
 // This warp's share of D[rank, row] for eight rows of one adapter and 16 * MT ranks from r0 on: the 32-column chunks
 // c0, c0 + stride, ... of the sum over K.
-template <typename T, int MT>
+template <typename T, int MT, bool Early>
 __device__ __forceinline__ void shrink_sum(const LoraArgs& a, const LoraTile& tile, int rank, int r0, int c0, int stride, float (&acc)[MT][4]) {
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const T* A = reinterpret_cast<const T*>(a.A) + ((int64_t)tile.ad * a.R + r0) * a.K + t * 8;
-    const int row = g < tile.cnt ? __ldg(a.rows + tile.p0 + g) : -1;
+    const int row = g < tile.cnt ? a.rows[tile.p0 + g] : -1;
     const bool xin = row >= 0 && row < a.n;
     const T* xr = reinterpret_cast<const T*>(a.x) + (int64_t)(xin ? row : 0) * a.K + t * 8;
     const uint4 zero = make_uint4(0, 0, 0, 0);
@@ -80,13 +85,13 @@ __device__ __forceinline__ void shrink_sum(const LoraArgs& a, const LoraTile& ti
         for (int u = 0; u < U; ++u) {
             const int k = (c0 + u * stride) * 32;
             const bool in = k + t * 8 < a.K;
-            fx[u] = in && xin ? __ldg(reinterpret_cast<const uint4*>(xr + k)) : zero;
+            fx[u] = in && xin ? load_in<Early>(reinterpret_cast<const uint4*>(xr + k)) : zero;
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int r = m * 16 + h * 8 + g;  // what lies behind the adapter's rank counts as zero
-                    fa[u][m][h] = in && r0 + r < rank ? __ldg(reinterpret_cast<const uint4*>(A + (int64_t)r * a.K + k)) : zero;
+                    fa[u][m][h] = in && r0 + r < rank ? load_in<Early>(reinterpret_cast<const uint4*>(A + (int64_t)r * a.K + k)) : zero;
                 }
         }
 #pragma unroll
@@ -135,7 +140,7 @@ lora_shrink_kernel(const LoraArgs a) {
     const int r0 = blockIdx.z * 16 * MT, rank = rank_of(a, tile.ad);
     if (r0 >= rank) return;
     float acc[MT][4] = {};
-    shrink_sum<T, MT>(a, tile, rank, r0, blockIdx.y * kShWarps + (threadIdx.x >> 5), kShWarps * a.S, acc);
+    shrink_sum<T, MT, false>(a, tile, rank, r0, blockIdx.y * kShWarps + (threadIdx.x >> 5), kShWarps * a.S, acc);
     shrink_add<MT>(acc, s_red, [&](int c, int r, float s) {
         if (c < tile.cnt && r0 + r < rank) a.part[((int64_t)blockIdx.y * a.P + tile.p0 + c) * a.R + r0 + r] = s;
     });
@@ -177,7 +182,7 @@ lora_shrink_wide_kernel(const LoraArgs a) {
     bool xin[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int c = q0 + 32 * i, row = c < tile.cnt ? __ldg(a.rows + tile.p0 + c) : -1;
+        const int c = q0 + 32 * i, row = c < tile.cnt ? a.rows[tile.p0 + c] : -1;
         xin[i] = row >= 0 && row < a.n;
         xs[i] = reinterpret_cast<const T*>(a.x) + (int64_t)(xin[i] ? row : 0) * a.K + piece * 8;
     }
@@ -395,7 +400,7 @@ __device__ __forceinline__ void stage_v(int cnt, int rank, F of, uint4* s_v, flo
 
 // One warp's way through features of a tile of 16 * MT rows, 32 at a time.  KG: groups of 16 ranks whose B values are
 // loaded ahead together with y (0: any number of ranks, B loaded in turn).
-template <typename T, typename Y, int MT, int KG>
+template <typename T, typename Y, int MT, int KG, bool Early>
 struct Expand {
     static constexpr int NS = Split<T>::N;
     struct Ahead { Raw8<Y> y[2 * MT]; uint2 b[KG ? KG : 1][4]; };
@@ -411,7 +416,7 @@ struct Expand {
           kgs((rk + 15) / 16), f_end(end), vec_b(flags & 1), vec_y(flags & 2) {
 #pragma unroll
         for (int m = 0; m < 2 * MT; ++m) {
-            const int c = m * 8 + ((threadIdx.x & 31) >> 2), r = c < tile.cnt ? __ldg(a.rows + tile.p0 + c) : -1;
+            const int c = m * 8 + ((threadIdx.x & 31) >> 2), r = c < tile.cnt ? a.rows[tile.p0 + c] : -1;
             row[m] = r < a.n ? r : -1;
         }
     }
@@ -422,7 +427,7 @@ struct Expand {
         uint2 w = make_uint2(0, 0);
         if (f < a.N) {
             const T* br = B + (int64_t)f * a.R + r;
-            if (vec_b && r + 4 <= rank) w = __ldg(reinterpret_cast<const uint2*>(br));
+            if (vec_b && r + 4 <= rank) w = load_in<Early>(reinterpret_cast<const uint2*>(br));
             else {
                 const unsigned short* bs = reinterpret_cast<const unsigned short*>(br);
                 if (r < rank) w.x = bs[0];
@@ -532,10 +537,10 @@ lora_expand_kernel(const LoraArgs a, int feats, int flags) {
         pdl_wait();                                      // this launch does not end before the first
         return;
     }
-    const float sc = a.scales ? __ldg(a.scales + tile.ad) : 1.f;
-    const Expand<T, Y, MT, KG> ex(a, tile, rank, s_v, s_scale, min(a.N, (int)(blockIdx.y + 1) * feats), flags);
+    const float sc = a.scales ? a.scales[tile.ad] : 1.f;
+    const Expand<T, Y, MT, KG, false> ex(a, tile, rank, s_v, s_scale, min(a.N, (int)(blockIdx.y + 1) * feats), flags);
     int f0 = blockIdx.y * feats + (threadIdx.x >> 5) * 32;
-    typename Expand<T, Y, MT, KG>::Ahead q;
+    typename Expand<T, Y, MT, KG, false>::Ahead q;
     ex.load(q, f0);                                      // B and y do not wait for the first launch
     pdl_wait();                                          // v comes from it
     // 32-row tiles take ranks up to 64, which registers hold where v would be read twice (8192 rows of 6144 to 6144 at rank
@@ -567,12 +572,12 @@ lora_cluster_kernel(const LoraArgs a, int feats, int flags) {
     const LoraTile tile = lora_tile<8>(a, pre, blockIdx.x / kClusterBlocks, descending);
     const int rank = tile.ad < 0 ? 0 : rank_of(a, tile.ad), block = (int)tc5::cluster_rank(), warp = threadIdx.x >> 5;
     if (rank == 0) return;                               // (the same for all blocks of the cluster)
-    const float sc = a.scales ? __ldg(a.scales + tile.ad) : 1.f;
-    const Expand<T, Y, 1, KG> ex(a, tile, rank, s_v, s_scale, min(a.N, (block + 1) * feats), flags);
+    const float sc = a.scales ? a.scales[tile.ad] : 1.f;
+    const Expand<T, Y, 1, KG, true> ex(a, tile, rank, s_v, s_scale, min(a.N, (block + 1) * feats), flags);
     int f0 = block * feats + warp * 32;
     float acc[KG][4] = {};
-    shrink_sum<T, KG>(a, tile, rank, 0, block * kShWarps + warp, kShWarps * kClusterBlocks, acc);
-    typename Expand<T, Y, 1, KG>::Ahead q;
+    shrink_sum<T, KG, true>(a, tile, rank, 0, block * kShWarps + warp, kShWarps * kClusterBlocks, acc);
+    typename Expand<T, Y, 1, KG, true>::Ahead q;
     ex.load(q, f0);                                      // on its way while the parts of v are put together
     shrink_add<KG>(acc, s_red, [&](int c, int r, float s) { s_part[r * 8 + c] = s; });
     tc5::cluster_sync_all();
@@ -631,10 +636,10 @@ __device__ __forceinline__ void stage_v_rows(const LoraArgs& a, const LoraTile& 
     const int c = e >> 3, p8 = e & 7;
     const bool in = c < tile.cnt;
     if (p8 == 0) {
-        const int r = in ? __ldg(a.rows + tile.p0 + c) : -1;
+        const int r = in ? a.rows[tile.p0 + c] : -1;
         s_off[c] = r >= 0 && r < a.n ? (int64_t)r * a.N : -1;
     }
-    const float sc = a.scales ? __ldg(a.scales + tile.ad) : 1.f;
+    const float sc = a.scales ? a.scales[tile.ad] : 1.f;
     float v[8], top = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {

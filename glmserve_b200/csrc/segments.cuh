@@ -91,7 +91,9 @@ inline int sm_count_of(int dev) {
 // Programmatic dependent launch: a kernel started with launch_after() may begin before the one ahead of it in the stream
 // has ended, once all of that one's blocks have called pdl_trigger(); it touches nothing that another kernel writes, or
 // still reads, before pdl_wait(), which returns when the kernel ahead is complete.  Every kernel here waits, so what a
-// kernel two places ahead wrote is there as well.
+// kernel two places ahead wrote is there as well.  What it reads may still be written while it is already there (unless an
+// ordinary launch stands between), so none of that goes through the read-only path (__ldg, const __restrict__): it asks for
+// data that no one writes meanwhile, and its loads may be moved ahead of the wait.
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

@@ -301,3 +301,35 @@ def test_lora_long_sum(dev, R):
     _check(y, ref, mag * (18 * U) + v.abs() @ Bs.abs().T * ((R + 8) * U + 2.0 ** -21) + HALF[torch.float32] * ref.abs(), "long sum")
     del x, A, y
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("n,nA,R", [(40, 20, 16), (120, 2, 32), (700, 5, 24)])      # one launch, and two
+def test_lists_made_right_before_the_call(dev, n, nA, R):
+    """The dispatch lets the next kernel start early: every call must see the lists, x and y as they are at its place in
+    the stream, while the same buffers are rewritten between the calls."""
+    from glmserve_b200 import ops
+    rng = np.random.default_rng(n)
+    K, N = 264, 520
+    A, B = _randn((nA, R, K), torch.bfloat16, dev, 1, 0.1), _randn((nA, N, R), torch.bfloat16, dev, 2)
+    ids = [_i32(rng.integers(-1, nA, n), dev)[:, None].contiguous() for _ in range(6)]
+    xs = [_randn((n, K), torch.bfloat16, dev, 3 + i) for i in range(6)]
+    want = []
+    for i, x in zip(ids, xs):
+        offs, rows, _ = ops.moe_dispatch(i, nA)
+        torch.cuda.synchronize()
+        y = ops.lora_add(torch.zeros((n, N), device=dev), x, A, B, offs, rows)
+        g = ops.grouped_gemm(x, A, offs, rows=rows, out=torch.zeros((n, R), dtype=torch.bfloat16, device=dev))
+        torch.cuda.synchronize()
+        want.append((y, g))
+    x, cur = torch.empty_like(xs[0]), torch.empty_like(ids[0])
+    got = []
+    for _ in range(10):
+        for i in range(6):
+            x.copy_(xs[i]), cur.copy_(ids[i])
+            y, g = torch.zeros((n, N), device=dev), torch.zeros((n, R), dtype=torch.bfloat16, device=dev)
+            offs, rows, _ = ops.moe_dispatch(cur, nA)
+            ops.lora_add(y, x, A, B, offs, rows)
+            offs, rows, _ = ops.moe_dispatch(cur, nA)
+            ops.grouped_gemm(x, A, offs, rows=rows, out=g)
+            got.append((i, y, g))
+    assert all(torch.equal(y, want[i][0]) and torch.equal(g, want[i][1]) for i, y, g in got)
