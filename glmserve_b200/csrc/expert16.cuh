@@ -48,12 +48,11 @@ __device__ __forceinline__ void epilogue_sync(int bar) { asm volatile("barrier.c
 // here is a third of an epilogue's instructions; where 1 + exp passes 2^126 this one gives 0 for a silu below 2^-119.)
 __device__ __forceinline__ float swiglu(float g, float u) { return __fmul_rn(__fdividef(g, 1.0f + expf(-g)), u); }
 
-// The two kernels; types as in gsb_grouped_gemm (a.w2 given: SwiGLU of two products, y of x's type).
-int launch_grouped_split(const GroupedArgs& a, int type, int y_type, cudaStream_t s);
 // status words of the kernels in the other files, cleared
 int take_pair_status();
 int take_lora_status();
-// scratch (16-byte aligned, grouped_pair_scratch_bytes): a copy of the rows in expert order, used when a.rows is given
+// The kernel for many rows; types as in gsb_grouped_gemm (a.w2 given: SwiGLU of two products, y of x's type).  scratch
+// (16-byte aligned, grouped_pair_scratch_bytes): a copy of the rows in expert order, used when a.rows is given
 size_t grouped_pair_scratch_bytes(int P, int K);
 int launch_grouped_pair(const GroupedArgs& a, int type, int y_type, void* scratch, cudaStream_t s);
 

@@ -250,7 +250,7 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
                     for (int j = 0; j < NC; ++j) d[j] = __uint_as_float(v[j]);
                 }
                 Y* o = y + (int64_t)(it.p0 + c0 + cb) * a.N + f;
-                if (sizeof(Y) == 2 && vec) {
+                if (GU || (sizeof(Y) == 2 && vec)) {      // (h has rows of whole 16-byte pieces, from the workspace's border on)
 #pragma unroll
                     for (int j = 0; j < NC; ++j) turn[j * 32 + lane] = GU ? h_from_f<Y>(d[j]) : from_f<Y>(d[j]);
                     __syncwarp();
@@ -265,11 +265,11 @@ grouped_pair_kernel(const GroupedArgs a, const __grid_constant__ CUtensorMap tm_
                     __syncwarp();
                 } else if (live == 0xffffu && f - lane + 32 <= a.N) {
 #pragma unroll
-                    for (int j = 0; j < NC; ++j, o += a.N) *o = GU ? h_from_f<Y>(d[j]) : from_f<Y>(d[j]);
+                    for (int j = 0; j < NC; ++j, o += a.N) *o = from_f<Y>(d[j]);
                 } else {
 #pragma unroll
                     for (int j = 0; j < NC; ++j)
-                        if (f < a.N && ((live >> (cb + j)) & 1u)) o[(int64_t)j * a.N] = GU ? h_from_f<Y>(d[j]) : from_f<Y>(d[j]);
+                        if (f < a.N && ((live >> (cb + j)) & 1u)) o[(int64_t)j * a.N] = from_f<Y>(d[j]);
                 }
             }
             tc5::fence_before();

@@ -154,9 +154,6 @@ lora_shrink_kernel(const LoraArgs a) {
 constexpr int kWdRows = 64, kWdStages = 4;
 template <int MT> constexpr int wd_stage_bytes() { return (kWdRows + 16 * MT) * 128; }
 
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, bool valid) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
@@ -194,21 +191,21 @@ lora_shrink_wide_kernel(const LoraArgs a) {
             const bool in = step * 64 + piece * 8 < a.K;
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                cp16(base + (uint32_t)((q0 + 32 * i) * 128) + sw, in && xin[i] ? xs[i] + step * 64 : xs[i], in && xin[i]);
+                tc5::cp_async16(base + (uint32_t)((q0 + 32 * i) * 128) + sw, in && xin[i] ? xs[i] + step * 64 : xs[i], in && xin[i]);
 #pragma unroll
             for (int i = 0; i < (RT + 31) / 32; ++i) {
                 const int r = q0 + 32 * i;
                 const bool have = in && r < RT && r0 + r < rank;    // what lies behind the adapter's rank counts as zero
-                if (r < RT) cp16(base + (uint32_t)((kWdRows + r) * 128) + sw, have ? A + (int64_t)r * a.K + step * 64 : A, have);
+                if (r < RT) tc5::cp_async16(base + (uint32_t)((kWdRows + r) * 128) + sw, have ? A + (int64_t)r * a.K + step * 64 : A, have);
             }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        tc5::cp_async_commit();
     };
     for (int i = 0; i < kWdStages - 1; ++i) copy(k_lo + i);
     const int wr = (warp & 3) * 16, wk = warp >> 2;        // this warp's rows, and its half of the step
     float acc[2 * MT][4] = {};
     for (int step = k_lo; step < k_hi; ++step) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kWdStages - 2) : "memory");
+        tc5::cp_async_wait<kWdStages - 2>();
         __syncthreads();                                   // the step is there, and the stage copied into next is free
         copy(step + kWdStages - 1);
         const uint32_t base = ring + (uint32_t)((step - k_lo) % kWdStages) * SB;
@@ -228,7 +225,7 @@ lora_shrink_wide_kernel(const LoraArgs a) {
             }
         }
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    tc5::cp_async_wait<0>();
     __syncthreads();
     // the second half's sums are added to the first's
     float* red = reinterpret_cast<float*>(s_ring);
