@@ -524,6 +524,10 @@ extern "C" int gsb_grouped_gemm(const void* x, const void* w, int type, const in
     const size_t need = rows ? gsb_grouped_gemm_workspace_bytes(P, in, E) : 0;
     if (need && (!workspace || misaligned(workspace, 256))) return GSB_ERR_INVALID_ARG;
     if (need > workspace_bytes) return GSB_ERR_WORKSPACE;
+    const __int128 y_bytes = (__int128)P * out * type_bytes(y_type);
+    if (overlap(y, y_bytes, x, (__int128)n * in * 2) || overlap(y, y_bytes, w, (__int128)E * out * in * 2) ||
+        overlap(y, y_bytes, expert_offsets, (E + 1) * 4) || overlap(y, y_bytes, rows, (__int128)P * 4))
+        return GSB_ERR_INVALID_ARG;
     GroupedArgs a{};
     a.x = x; a.w = w; a.offsets = expert_offsets; a.rows = rows;
     a.n = n; a.P = P; a.K = in; a.N = out; a.E = E; a.y = y;
@@ -552,6 +556,9 @@ extern "C" int gsb_moe_expert_ffn_w16(const void* x, const int* topk_ids, const 
     if (!workspace || misaligned(workspace, 256)) return GSB_ERR_INVALID_ARG;
     const Ffn16Ws ws = carve16(n, topk, hidden, moe_inter, E, workspace);
     if (workspace_bytes < ws.total) return GSB_ERR_WORKSPACE;
+    // (x has been read when the last launch writes out; the ids and weights are read by it)
+    const __int128 out_bytes = (__int128)n * hidden * type_bytes(out_type), slot_bytes = (__int128)n * topk * 4;
+    if (overlap(out, out_bytes, topk_ids, slot_bytes) || overlap(out, out_bytes, topk_weights, slot_bytes)) return GSB_ERR_INVALID_ARG;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     GroupedArgs g{};
     g.x = x; g.w = gate_w; g.w2 = up_w; g.offsets = ws.offsets; g.rows = ws.tok;

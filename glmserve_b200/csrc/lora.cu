@@ -1102,6 +1102,11 @@ extern "C" int gsb_lora_add(const void* x, const void* A, const void* B, int typ
     const size_t need = gsb_lora_scratch_bytes(P, max_rank, n_adapters);
     if (need && (!scratch || misaligned(scratch, 256))) return GSB_ERR_INVALID_ARG;
     if (scratch_bytes < need) return GSB_ERR_WORKSPACE;
+    const __int128 y_bytes = (__int128)n * out * (y_type == GSB_TYPE_F32 ? 4 : 2), per = (__int128)n_adapters * max_rank * 2;
+    if (overlap(y, y_bytes, x, (__int128)n * in * 2) || overlap(y, y_bytes, A, per * in) || overlap(y, y_bytes, B, per * out) ||
+        overlap(y, y_bytes, adapter_offsets, (n_adapters + 1) * 4) || overlap(y, y_bytes, rows, (__int128)P * 4) ||
+        overlap(y, y_bytes, ranks, n_adapters * 4) || overlap(y, y_bytes, scales, n_adapters * 4))
+        return GSB_ERR_INVALID_ARG;
     LoraArgs a{};
     a.x = x; a.A = A; a.B = B; a.offsets = adapter_offsets; a.rows = rows; a.ranks = ranks; a.scales = scales;
     a.n = n; a.P = P; a.K = in; a.N = out; a.nA = n_adapters; a.R = max_rank;

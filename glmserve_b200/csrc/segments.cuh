@@ -113,5 +113,10 @@ inline int launch_after(K kernel, dim3 grid, int threads, size_t smem, int clust
 }
 
 inline bool misaligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a != 0; }
+// whether two pieces of memory share a byte; sizes are products of up to three dimensions (below 2^73), null has none
+inline bool overlap(const void* p, __int128 p_bytes, const void* q, __int128 q_bytes) {
+    const __int128 a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+    return p && q && a < b + q_bytes && b < a + p_bytes;
+}
 
 }  // namespace gsb

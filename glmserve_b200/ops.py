@@ -139,7 +139,8 @@ def grouped_gemm(x, w, expert_offsets, rows=None, out=None, out_dtype=None):
     ``expert_offsets[e] <= p < expert_offsets[e + 1]``.  x bf16/fp16 [n,K], w the same type [E,N,K],
     expert_offsets int32 [E+1] and rows int32 [P] as ``moe_dispatch`` returns them (offsets, sorted_token_ids);
     without ``rows`` row p is x[p].  Returns y [P,N] of x's type (or float32 with ``out_dtype`` / ``out``).  Rows
-    that no segment covers are left as they were in ``out``; without ``out`` their contents are undefined."""
+    that no segment covers are left as they were in ``out``; without ``out`` their contents are undefined.  ``out``
+    shares no memory with the inputs."""
     dev, dtype = x.get_device(), x.dtype
     if dev < 0 or _TYPE.get(dtype, 0) == 0 or not _on(dev, dtype, x, w) or not _on(dev, torch.int32, expert_offsets, rows):
         raise ValueError("grouped_gemm: expected contiguous tensors on one CUDA device: x [n,K] and w [E,N,K] of "
@@ -166,7 +167,7 @@ def grouped_gemm(x, w, expert_offsets, rows=None, out=None, out_dtype=None):
 def moe_expert_ffn_w16(x, topk_ids, topk_w, gate_w, up_w, down_w, out=None, out_dtype=None):
     """``moe_expert_ffn`` with bf16/fp16 activations and weights on the tensor cores: x [n,H], topk_ids int32 and
     topk_w float32 [n,topk], gate_w/up_w [E,I,H], down_w [E,H,I] -> out [n,H] of x's type (or float32).  A slot
-    whose id is outside [0,E) adds nothing (padding, or an expert on another GPU)."""
+    whose id is outside [0,E) adds nothing (padding, or an expert on another GPU).  ``out`` may be x."""
     dev, dtype = x.get_device(), x.dtype
     if dev < 0 or _TYPE.get(dtype, 0) == 0 or not _on(dev, dtype, x, gate_w, up_w, down_w) or \
             not _on(dev, torch.int32, topk_ids) or not _on(dev, torch.float32, topk_w):
@@ -195,7 +196,8 @@ def lora_add(y, x, A, B, adapter_offsets, rows, ranks=None, scales=None):
     B [nA,N,R] of the same type, y [n,N] float32 (what ``gemm_w4a16`` returns) or x's type, ranks int32 [nA]
     (columns of B and rows of A behind an adapter's rank are not used), scales float32 [nA].  The lists come from
     ``moe_dispatch(adapter_ids[:, None], nA)``, once per batch: offsets and sorted_token_ids; an id of -1 = no
-    adapter.  ``rows`` may be longer than the segments: what lies behind the last one is ignored."""
+    adapter.  ``rows`` may be longer than the segments: what lies behind the last one is ignored; a row must not be listed
+    twice.  y shares no memory with the inputs."""
     dev, dtype = x.get_device(), x.dtype
     if dev < 0 or _TYPE.get(dtype, 0) == 0 or not _on(dev, dtype, x, A, B) or \
             not _on(dev, torch.int32, adapter_offsets, rows, ranks) or not _on(dev, torch.float32, scales):

@@ -127,7 +127,7 @@ enum { GSB_TYPE_F32 = 0, GSB_TYPE_BF16 = 1, GSB_TYPE_F16 = 2 };
  * or F32).  Sums in fp32, one rounding at the end.  Rows of y that no segment covers, or whose rows[p] is outside
  * [0,n), are left as they were; an expert with an empty segment costs nothing.  Offsets are clamped to [0,P]; with
  * offsets that descend nothing is written.
- * in % 8 == 0, E <= 1024, P, in and out <= 2^30; x and w 16-byte aligned; y must not overlap the inputs.  workspace: with a row
+ * in % 8 == 0, E <= 1024, P, in and out <= 2^30; x and w 16-byte aligned; y must not overlap the inputs (refused).  workspace: with a row
  * list gsb_grouped_gemm_workspace_bytes() bytes (0 for few rows per expert: then it may be NULL), 256-byte aligned, any
  * contents; two calls that may overlap on the GPU need a workspace each. */
 GSB_API size_t gsb_grouped_gemm_workspace_bytes(int P, int in, int E);
@@ -139,11 +139,11 @@ GSB_API int gsb_grouped_gemm(const void* x, const void* w, int type, const int* 
  * out[t] = sum_k w[t,k] * down(silu(gate x) * up x), slots added in order.  x [n,hidden], gate_w/up_w
  * [E,moe_inter,hidden], down_w [E,hidden,moe_inter] of `type`; out [n,hidden] of out_type (`type`, or F32) is
  * OVERWRITTEN.  A slot whose id is outside [0,E) adds nothing (padding, or an expert that lives on another GPU);
- * a token without a slot gets zeros.  Sums in fp32; silu(gate x) * up x is rounded once to `type`; in fp16 finite
- * values saturate at +-65504, infinities and NaN stay what they are.  hidden and moe_inter multiples of 8, E <= 1024,
- * n * topk and each dimension <= 2^30 (hidden <= 65535 * 4096 for 256 tokens or more); all pointers but ids and
- * weights 16-byte aligned; workspace 256-byte aligned, any contents; two calls that may overlap on the GPU need a
- * workspace each. */
+ * a token without a slot gets zeros.  out may be x; over the ids or weights it is refused.  Sums in fp32; silu(gate x)
+ * * up x is rounded once to `type`; in fp16 finite values saturate at +-65504, infinities and NaN stay what they are.
+ * hidden and moe_inter multiples of 8, E <= 1024, n * topk and each dimension <= 2^30 (hidden <= 65535 * 4096 for 256
+ * tokens or more); all pointers but ids and weights 16-byte aligned; workspace 256-byte aligned, any contents; two
+ * calls that may overlap on the GPU need a workspace each. */
 GSB_API size_t gsb_moe_expert_ffn_w16_workspace_bytes(int n, int topk, int hidden, int moe_inter, int E);
 GSB_API int gsb_moe_expert_ffn_w16(const void* x, const int* topk_ids, const float* topk_weights,
                                    const void* gate_w, const void* up_w, const void* down_w, int type,
@@ -157,7 +157,7 @@ GSB_API int gsb_moe_expert_ffn_w16(const void* x, const int* topk_ids, const flo
  * behind an adapter's rank is not used, whatever it holds; scales f32 [n_adapters] (NULL: 1).  The lists are those
  * of gsb_moe_dispatch on one adapter id a row (topk = 1, E = n_adapters, an id outside the range = no adapter), made
  * once per batch and used for every projection of the model; rows that no list names are left as they were, indices
- * outside [0,n) are skipped, a row must not be listed twice; y must not overlap the inputs.  A x is kept in fp32 and B
+ * outside [0,n) are skipped, a row must not be listed twice; y must not overlap the inputs (refused).  A x is kept in fp32 and B
  * applied to it without rounding it to `type` (it enters the products in parts, so an infinity in B may give NaN; with
  * F16, entries of A x below 2^-37 of their row's largest are off by up to 2^-61 of the largest); y is rounded once.  in % 8 == 0, 1 <= max_rank <= 256, n_adapters <= 1024, P, in and out <= 2^30; x and A 16-byte aligned;
  * scratch of gsb_lora_scratch_bytes() bytes (0 for few rows: then it may be NULL), 256-byte aligned, any contents, not

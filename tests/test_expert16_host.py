@@ -91,3 +91,31 @@ def test_ffn_refuses_what_its_last_launch_could_not_cover():
     """256 tokens or more of over 65535 * 4096 features: before anything is launched (fewer tokens: no such limit)."""
     assert _ffn(n=256, H=65535 * 4096 + 8, nb=1 << 62) == 7
     assert _ffn(n=255, H=65535 * 4096 + 8) == WORKSPACE and _ffn(n=256, H=65535 * 4096) == WORKSPACE
+
+
+FAR = 1 << 40       # the other buffers, away from the pair that shares memory
+
+
+@pytest.mark.parametrize("kw", [
+    dict(x=P16), dict(x=P16 + 48), dict(x=P16 - 512 + 16), dict(w=P16 - 2 * 32 * 64 * 2 + 16), dict(w=P16 + 192, rows=0),
+    dict(offs=P16 + 4), dict(rows=P16 + 252), dict(y=P16 + 2, x=P16 - 496), dict(yt=0, x=P16 + 496),
+    dict(x=8 * FAR - (1 << 30) * 8 * 2 + 16, n=1 << 30, inn=8, y=8 * FAR), dict(w=P16 + 16, inn=1 << 30, out=1 << 30, E=1024)])
+def test_grouped_gemm_refuses_a_result_over_its_inputs(kw):
+    """y: four rows of 32, 256 bytes from P16 (512 in fp32)."""
+    far = dict(x=FAR, w=2 * FAR, offs=3 * FAR, rows=4 * FAR, y=P16)
+    assert _grouped(**{**far, **kw}) == INVALID
+
+
+@pytest.mark.parametrize("kw", [dict(ids=P16 + 508), dict(wt=P16), dict(wt=P16 - 28), dict(ot=0, wt=P16 + 1020)])
+def test_ffn_refuses_a_result_over_its_ids_or_weights(kw):
+    far = dict(x=FAR, ids=2 * FAR, wt=3 * FAR, g=4 * FAR, u=5 * FAR, d=6 * FAR, ws=7 * FAR, out=P16)
+    assert _ffn(**{**far, **kw}) == INVALID
+
+
+@pytest.mark.parametrize("kw", [
+    dict(x=P16), dict(x=P16 + 496), dict(x=P16 - 496), dict(A=P16 + 16), dict(A=P16 - 2 * 8 * 64 * 2 + 16), dict(B=P16 + 510),
+    dict(offs=P16), dict(rows=P16 + 508), dict(ranks=P16 + 4), dict(scales=P16 - 4), dict(yt=1, B=P16 + 254)])
+def test_lora_refuses_a_result_over_its_inputs(kw):
+    """y: four rows of 32 in fp32, 512 bytes from P16 (256 in 16 bits)."""
+    far = dict(x=FAR, A=2 * FAR, B=3 * FAR, offs=4 * FAR, rows=5 * FAR, sc=6 * FAR, y=P16)
+    assert _lora(**{**far, **kw}) == INVALID

@@ -470,3 +470,11 @@ def test_grouped_gemm_sum_that_takes_a_second(dev, E, P, K):
     _check(y, ref, mag * (16 * U), "long sum")
     del x, w, y
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("case", [1, 5, 8, 10])          # lists in the kernel, the pair kernel, a cluster, few slots
+def test_expert_ffn_in_place(dev, case):
+    from glmserve_b200 import ops
+    x, *rest = _ffn_case(case, torch.bfloat16, dev)
+    want = ops.moe_expert_ffn_w16(x, *rest)
+    assert ops.moe_expert_ffn_w16(x, *rest, out=x) is x and torch.equal(x, want)
