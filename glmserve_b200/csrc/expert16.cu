@@ -387,6 +387,13 @@ int run_grouped_any(const GroupedArgs& a, int y_type, cudaStream_t s) {
     return y_type == GSB_TYPE_F32 ? run_grouped<T, float, false>(a, s) : run_grouped<T, T, false>(a, s);
 }
 
+// The kernel for many rows above 16 rows per expert on average: the host knows the length of the list, not what is in it.
+// Few rows against many, us, 32 experts of 6144 to 2048: 8 rows an expert 124 and 136, 16 rows 126 and 137, 20 rows 149 and
+// 138, 32 rows 181 and 141; the same with Zipf-like loads (exponent 1.1): 131 and 136, 141 and 138, 159 and 137, 190 and
+// 140.  8 experts of 4096 to 4096: 8 rows 45 and 51, 16 rows 54 and 52, 32 rows 70 and 53.  Small products change places
+// later (16 experts of 1024 to 512: 24 rows 8.0 and 10.1, 32 rows 11.6 and 10.6).  Where the average says little it can be
+// wrong: all rows on one of 32 experts, 256 rows 44 and 28, 512 rows 83 and 29; and a shard whose list is mostly slots of
+// other GPUs (FFN, 32 of 256 experts, 6144 x 2048): 128 tokens 359 and 379, 512 tokens 394 and 400, 1024 tokens 514 and 422.
 bool use_pair(int P, int E) { return P / E > 16; }
 
 int launch_grouped(GroupedArgs a, int type, int y_type, void* scratch, cudaStream_t s) {

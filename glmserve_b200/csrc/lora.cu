@@ -1053,12 +1053,14 @@ int run_lora(const LoraArgs& a, cudaStream_t s) {
     if (wide) st = a.R <= 16 ? run_shrink_wide<T, 1>(a, s) : a.R <= 32 ? run_shrink_wide<T, 2>(a, s) : run_shrink_wide<T, 4>(a, s);
     else st = a.R <= 16 ? run_shrink<T, 1>(a, s) : a.R <= 32 ? run_shrink<T, 2>(a, s) : run_shrink<T, 4>(a, s);
     if (st) return st;
-    // Measured over 16 .. 8192 rows, 901 .. 6144 features, 2 .. 32 adapters.  16-row tiles with B loaded ahead while there
-    // are few rows (rank 64, 256 rows of 1024: 11 us against 13 for 32-row tiles and 16 for tcgen05); 32-row tiles halve the
-    // reads of B above (rank 16, 8192 rows of 6144: 111 us against 135 and 120).  tcgen05 where fp32 outputs and the rank
-    // are large (rank 64, 8192 rows of 6144: 103 us against 165; rank 32: 99 and 133; 16-bit y: 116 and 106) and for
-    // outputs whose rows are not 16-byte pieces, which the others take value by value (8192 rows of 3941, rank 16: 75 us
-    // against 217; rank 49: 125 and 213).
+    // Times of a whole call on the device, 8 adapters, bf16.  16-row tiles with B loaded ahead while there are few rows (rank
+    // 64, 256 rows of 1024 to 1024: 11 us against 13 for 32-row tiles and 16 for tcgen05); 32-row tiles halve the reads of B
+    // above (rank 16, 8192 rows of 6144 to 6144: 111 us against 135).  tcgen05 where fp32 outputs and the rank are large,
+    // against 32-row tiles, 8192 rows of 256 to 6144: rank 64 103 us and 169, rank 32 100 and 144, rank 16 98 and 102; 2048
+    // rows of 256 to 4096: 31 and 41, 30 and 32, 29 and 24; rank 49, whose B it lays out itself, 159 and 191, 39 and 44.
+    // With a 16-bit y its lanes move 2 bytes at a time: rank 64 110 and 109, rank 32 105 and 84, rank 49 160 and 139 (fp16
+    // 110 and 120, 104 and 90, 162 and 145).  And tcgen05 for outputs whose rows are not 16-byte pieces, which the others
+    // take value by value (8192 rows of 256 to 3941: rank 16 74 us against 235, rank 49 108 and 197).
     const int64_t outputs = (int64_t)a.P * a.N;
     const bool pieces = expand_flags<Y>(a) & 2, rows8 = a.R % 8 == 0;
     const int64_t enough = !pieces ? 5 << 19 : sizeof(Y) == 2 ? INT64_MAX : a.R > 32 ? (rows8 ? 6 << 20 : 20 << 20) : a.R > 16 && rows8 ? 12 << 20 : INT64_MAX;
