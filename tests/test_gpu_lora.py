@@ -4,7 +4,8 @@ that keep at least 21 bits (2^-21 of every product); y is rounded once."""
 import numpy as np
 import pytest
 
-from test_gpu_expert16 import HALF, TINY, U, _check, _i32, _randn, _sparse
+from test_gpu_expert16 import HALF, TINY, U, _check, _i32, _randn
+from test_gpu_expert16 import _sparse
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
